@@ -24,7 +24,7 @@ CSRC = os.path.dirname(os.path.abspath(__file__))
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + ["-lineinfo", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
                            "--expt-relaxed-constexpr"]
-HEADERS = ["common.cuh", "attention_tc_static.h", "tc5_common.cuh"]
+HEADERS = ["common.cuh", "attention_tc_static.h", "tc5_common.cuh", "q8.cuh"]
 
 _loaded: Dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()
@@ -247,6 +247,7 @@ def loaded_libraries() -> Dict[str, "CheckedLibrary"]:
 VARIANTS = {"skinny_gemm": [None, {"KLLM_BIAS": 1}], "skinny_gemm_f32": [None, {"KLLM_BIAS": 1}],
             "attention_tc": [{"KLLM_HD": hd} for hd in list(range(16, 129, 16)) + [160, 192, 224, 256]]
             + [{"KLLM_HD": hd, "KLLM_VD": vd} for hd, vd in ((32, 64), (64, 128), (128, 64), (128, 256))],
+            "attention_q8": [{"KLLM_HD": hd} for hd in range(32, 257, 32)],
             "attention_tcgen05": [{"KLLM_HD": hd} for hd in (64, 128)],
             "attention_tcgen05_ptmem": [{"KLLM_HD": hd} for hd in (64, 128)]}
 

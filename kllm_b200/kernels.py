@@ -1034,6 +1034,177 @@ def attention_prefill_tcgen05(out, q, kcache, vcache, q_start, start_pos, block_
     _check(lib, name, rc)
 
 
+# ---- the paged cache in 8 bits -------------------------------------------------------------------------------------------
+
+Q8_DTYPE = torch.float8_e4m3fn        # what a cache in 8 bits holds, beside one float32 power of two per page and kv head
+Q8_HEAD_DIMS = tuple(range(32, 257, 32))
+Q8_MAX_PAGE = 4096
+
+
+def _check_q8(what, kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim):
+    """The stores, scales and table that the kernels of the cache in 8 bits share."""
+    if kcache.dtype != Q8_DTYPE or vcache.dtype != Q8_DTYPE or not kcache.is_contiguous() or not vcache.is_contiguous():
+        raise KernelError(f"{what}: the caches must be contiguous float8_e4m3fn tensors")
+    if kcache.dim() != 4 or kcache.shape[1] != n_kv or kcache.shape[3] != head_dim or vcache.shape != kcache.shape:
+        raise KernelError(f"{what}: cache layout must be [pages, n_kv, page_size, head_dim], keys and values alike")
+    for t in (kscale, vscale):
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != kcache.shape[:2]:
+            raise KernelError(f"{what}: scales must be contiguous float32 [pages, n_kv]")
+    if head_dim not in Q8_HEAD_DIMS:
+        raise KernelError(f"{what}: head size {head_dim} is not a multiple of 32 up to 256")
+    if n_kv <= 0 or n_heads <= 0 or n_heads % n_kv:
+        raise KernelError(f"{what}: {n_heads} heads are not a multiple of {n_kv} kv heads")
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: the block table must be [requests, pages of a request]")
+    _i32(block_table, "block_table")
+
+
+def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_sin: Optional[torch.Tensor],
+                   positions: torch.Tensor, token_req: Optional[torch.Tensor], q_start: torch.Tensor,
+                   block_table: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                   vscale: torch.Tensor, n_heads: int, n_kv: int, head_dim: int) -> None:
+    """Rotary encoding of a step's tokens and the write of their keys and values into a cache in 8 bits
+    (csrc/cache_q8.cu): ``q_out`` [n, H*hd] gets the rotated queries (it may be ``q``), the pages of ``kcache`` / ``vcache``
+    (float8_e4m3fn [pages, G, page_size, hd]) the rotated keys and the values, ``kscale`` / ``vscale`` (float32 [pages, G])
+    the pages' scales.  A stored number stands for e4m3 * scale.
+
+    A page's scale is a power of two 2^e, -48 <= e <= 48: the smallest with max|x| <= 448 * 2^e over the rows that are
+    stored, and not below that of the rows which the page holds already; these are stored again under a scale that has
+    grown.  A step that writes a page's first slot starts the page anew.  Numbers beyond 448 * 2^48 are stored as that.
+    A token whose key or value (of a head) holds an infinity or NaN is stored with NaN keys and zero values: the rows that
+    attend to it become NaN, and no others.
+
+    Rows ``q_start[s] .. q_start[s + 1]`` are request s's, at consecutive ``positions``; ``token_req`` None: every request
+    brings one token.  ``cos_sin``: float32 [positions, rotary width], None: no rotation.  Tokens with a negative position
+    or one behind the table of angles are neither rotated nor stored, those without a page not stored; rows behind the last
+    request are left as they are.  No page may belong to two requests of a step."""
+    _check_q8("rope_append_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
+    _i32(positions, "positions"); _i32(token_req, "token_req"); _i32(q_start, "q_start")
+    n = q.shape[0]
+    dt = q.dtype
+    dtype_code(dt)
+    if q_out.dtype != dt or k.dtype != dt or v.dtype != dt:
+        raise KernelError("rope_append_q8: q, k, v and q_out must have one dtype")
+    Q, K = n_heads * head_dim, n_kv * head_dim
+    if q.shape[1] != Q or q_out.shape != q.shape or k.shape != (n, K) or v.shape != (n, K):
+        raise KernelError("rope_append_q8: q and q_out [n, heads * head_dim], k and v [n, kv heads * head_dim]")
+    if q.stride(1) != 1 or q_out.stride(1) != 1 or k.stride(1) != 1 or v.stride(1) != 1:
+        raise KernelError("rope_append_q8: rows must be dense")
+    if kcache.shape[2] > Q8_MAX_PAGE:
+        raise KernelError(f"rope_append_q8: pages of {kcache.shape[2]} tokens, at most {Q8_MAX_PAGE}")
+    R = q_start.numel() - 1
+    if positions.numel() < n or R < 0 or block_table.shape[0] < R or (
+            token_req.numel() < n if token_req is not None else n > R):
+        raise KernelError("rope_append_q8: positions and token_req per token, a table row and a q_start per request "
+                          "(token_req None: one token per request)")
+    n_pos = rot = 0
+    if cos_sin is not None:
+        n_pos, rot = cos_sin.shape
+        if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or rot % 2 or rot > head_dim:
+            raise KernelError("rope_append_q8: cos_sin must be contiguous float32 [positions, even rotary width <= head_dim]")
+    _cuda(q_out, q, k, v, cos_sin, positions, token_req, q_start, block_table, kcache, vcache, kscale, vscale)
+    lib = load_library("cache_q8")
+    rc = lib.kllm_rope_append_q8(_p(q_out), q_out.stride(0), _p(q), q.stride(0), _p(k), k.stride(0), _p(v), v.stride(0),
+                                 _p(cos_sin), n_pos, _p(positions), _p(token_req), _p(q_start), R, _p(block_table),
+                                 block_table.shape[1], _p(kcache), _p(vcache), _p(kscale), _p(vscale), kcache.shape[0], n,
+                                 n_heads, n_kv, head_dim, rot, kcache.shape[2], dtype_code(dt), _stream())
+    _check(lib, "cache_q8", rc)
+
+
+def decode_q8_parts(n_tokens: int, n_kv: int, group: int, head_dim: int, ctx_bound: int) -> tuple:
+    """(ranges, CTAs of a cluster) into which a token's context of up to ``ctx_bound`` keys is cut."""
+    most = 16 if head_dim <= 128 else 8
+    subs = next(s for s in range(1, group + 1) if group % s == 0 and group // s <= most)
+    base = max(1, n_tokens * n_kv * subs)
+    blocks = max(1, -(-ctx_bound // 128))
+    want = max(1, min(blocks, 3 * sm_count() // base))
+    cluster = 1
+    while cluster < 8 and cluster * 2 <= want:
+        cluster *= 2
+    return max(1, want // cluster) if cluster == 8 else 1, cluster
+
+
+def _check_q8_rows(what, out, q, n_heads, head_dim):
+    dtype_code(q.dtype)
+    if out.dtype != q.dtype or q.dim() != 2 or q.shape[1] != n_heads * head_dim or q.stride(1) != 1 or out.shape != q.shape \
+            or not out.is_contiguous():
+        raise KernelError(f"{what}: q [n, heads * head_dim] with dense rows, out contiguous of the same shape and dtype")
+
+
+def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                        vscale: torch.Tensor, positions: torch.Tensor, token_req: Optional[torch.Tensor],
+                        block_table: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, window: int, scale: float,
+                        ctx_bound: int) -> None:
+    """Attention of single tokens over a cache in 8 bits (csrc/attention_q8.cu; stores and scales as ``rope_append_q8``
+    leaves them): row t, at ``positions[t]`` of request ``token_req[t]`` (None: request t), sees its request's keys up to
+    its own place (``window`` W > 0: the last W of them).  bfloat16 or float32 ``q`` and ``out`` [n, H*hd].  ``ctx_bound``:
+    no context is longer; it only decides into how many parts the contexts are cut.  Keys whose table entry names no page
+    are not seen; a row that sees none (a negative position, say) becomes zeros."""
+    _check_q8("attention_decode_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
+    _check_q8_rows("attention_decode_q8", out, q, n_heads, head_dim)
+    _i32(positions, "positions"); _i32(token_req, "token_req")
+    n, R = q.shape[0], block_table.shape[0]
+    if positions.numel() < n or (token_req.numel() < n if token_req is not None else R < n):
+        raise KernelError("attention_decode_q8: a position (and a request) per token")
+    _cuda(out, q, kcache, vcache, kscale, vscale, positions, token_req, block_table)
+    bound = min(int(ctx_bound), int(window)) if window and window > 0 else int(ctx_bound)
+    ranges, cluster = decode_q8_parts(n, n_kv, n_heads // n_kv, head_dim, bound)
+    part_o = part_ml = None
+    if ranges > 1:
+        part_o = torch.empty((n, n_heads, ranges, head_dim), dtype=torch.float32, device=q.device)
+        part_ml = torch.empty((n, n_heads, ranges, 2), dtype=torch.float32, device=q.device)
+    lib = load_library("attention_q8", {"KLLM_HD": head_dim})
+    rc = lib.kllm_attention_decode_q8(_p(out), _p(part_o), _p(part_ml), _p(q), q.stride(0), _p(kcache), _p(vcache), _p(kscale),
+                                      _p(vscale), _p(positions), _p(token_req), _p(block_table), block_table.shape[1],
+                                      kcache.shape[0], n, R, n_heads, n_kv, head_dim, kcache.shape[2], int(window or 0), scale,
+                                      ranges, cluster, dtype_code(q.dtype), _stream())
+    _check(lib, "attention_q8", rc)
+    global launches
+    if ranges > 1:
+        launches += 1       # the kernel that joins the ranges
+
+
+def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                         vscale: torch.Tensor, q_start: torch.Tensor, start_pos: torch.Tensor, block_table: torch.Tensor,
+                         n_requests: int, n_heads: int, n_kv: int, head_dim: int, window: int, scale: float,
+                         ctx_bound: int) -> None:
+    """Attention of portions over a cache in 8 bits: request s brings rows q_start[s]..q_start[s+1] that start at cache
+    position start_pos[s]; their own keys are in the cache already.  Otherwise as ``attention_decode_q8``; rows that belong
+    to no request are left as they are."""
+    _check_q8("attention_prefill_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
+    _check_q8_rows("attention_prefill_q8", out, q, n_heads, head_dim)
+    _i32(q_start, "q_start"); _i32(start_pos, "start_pos")
+    R = int(n_requests)
+    if R < 0 or q_start.numel() < R + 1 or start_pos.numel() < R or block_table.shape[0] < R:
+        raise KernelError("attention_prefill_q8: q_start, start_pos and the block table must cover the requests")
+    _cuda(out, q, kcache, vcache, kscale, vscale, q_start, start_pos, block_table)
+    lib = load_library("attention_q8", {"KLLM_HD": head_dim})
+    rc = lib.kllm_attention_prefill_q8(_p(out), _p(q), q.stride(0), _p(kcache), _p(vcache), _p(kscale), _p(vscale), _p(q_start),
+                                       _p(start_pos), _p(block_table), block_table.shape[1], kcache.shape[0], q.shape[0], R,
+                                       n_heads, n_kv, head_dim, kcache.shape[2], int(window or 0), scale, dtype_code(q.dtype),
+                                       _stream())
+    _check(lib, "attention_q8", rc)
+
+
+def attention_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                 vscale: torch.Tensor, ctx, block_table: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, window: int,
+                 scale: float) -> None:
+    """Causal GQA attention of a step's tokens over a cache in 8 bits, by the kernel that fits: steps of single tokens and
+    the single tokens at the head of a mixed step take ``attention_decode_q8``, the portions behind them
+    ``attention_prefill_q8`` (a single token there would walk its whole context with one CTA)."""
+    if ctx.all_single:
+        return attention_decode_q8(out, q, kcache, vcache, kscale, vscale, ctx.positions, ctx.token_req, block_table, n_heads,
+                                   n_kv, head_dim, window, scale, ctx.split_bound or ctx.max_ctx)
+    singles = 0
+    while singles < ctx.n_requests and ctx.host_n_new and ctx.host_n_new[singles] == 1:
+        singles += 1
+    if singles:
+        attention_decode_q8(out[:singles], q[:singles], kcache, vcache, kscale, vscale, ctx.positions[:singles], None,
+                            block_table[:singles], n_heads, n_kv, head_dim, window, scale, ctx.max_ctx)
+    attention_prefill_q8(out, q, kcache, vcache, kscale, vscale, ctx.q_start[singles:], ctx.start_pos[singles:],
+                         block_table[singles:], ctx.n_requests - singles, n_heads, n_kv, head_dim, window, scale, ctx.max_ctx)
+
+
 _status_words = {}      # device index -> int32 tensor that kernels set when a bounded wait runs out
 
 

@@ -1,0 +1,122 @@
+"""What the faces of the cache in 8 bits refuse, and how contexts are cut: no GPU needed."""
+import pytest
+import torch
+
+from kllm_b200 import kernels
+from kllm_b200.kernels import KernelError
+
+H, G, HD, PS, R, N = 8, 2, 64, 16, 3, 5
+
+
+def operands():
+    f8 = lambda *s: torch.zeros(*s, dtype=torch.uint8).view(torch.float8_e4m3fn)  # noqa: E731
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    return dict(q=torch.zeros(N, H * HD), out=torch.zeros(N, H * HD), k=torch.zeros(N, G * HD), v=torch.zeros(N, G * HD),
+                cos_sin=torch.zeros(40, HD), positions=i(0, 1, 2, 3, 4), token_req=i(0, 0, 1, 2, 2), q_start=i(0, 2, 3, 5),
+                start_pos=i(0, 2, 3), table=torch.zeros(R, 3, dtype=torch.int32), kcache=f8(7, G, PS, HD),
+                vcache=f8(7, G, PS, HD), kscale=torch.ones(7, G), vscale=torch.ones(7, G), n_heads=H, n_kv=G, head_dim=HD)
+
+
+def append(o):
+    kernels.rope_append_q8(o["out"], o["q"], o["k"], o["v"], o["cos_sin"], o["positions"], o["token_req"], o["q_start"], o["table"],
+                           o["kcache"], o["vcache"], o["kscale"], o["vscale"], o["n_heads"], o["n_kv"], o["head_dim"])
+
+
+def decode(o):
+    kernels.attention_decode_q8(o["out"], o["q"], o["kcache"], o["vcache"], o["kscale"], o["vscale"], o["positions"], o["token_req"],
+                                o["table"], o["n_heads"], o["n_kv"], o["head_dim"], 0, 0.125, 40)
+
+
+def prefill(o):
+    kernels.attention_prefill_q8(o["out"], o["q"], o["kcache"], o["vcache"], o["kscale"], o["vscale"], o["q_start"], o["start_pos"],
+                                 o["table"], R, o["n_heads"], o["n_kv"], o["head_dim"], 0, 0.125, 40)
+
+
+CALLS = {"append": append, "decode": decode, "prefill": prefill}
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_sound_call_gets_as_far_as_the_device(call):
+    with pytest.raises(KernelError, match="not on a CUDA device"):
+        CALLS[call](operands())
+
+
+def strided(t, dim=-1):
+    return torch.cat([t, t], dim=dim).narrow(dim, 0, t.shape[dim]) if dim != -1 else torch.stack([t, t], dim=-1)[..., 0]
+
+
+BAD = {
+    "key store of another type": lambda o: o.update(kcache=o["kcache"].to(torch.bfloat16)),
+    "value store of bytes": lambda o: o.update(vcache=o["vcache"].view(torch.uint8)),
+    "stores of two shapes": lambda o: o.update(vcache=o["vcache"][:6]),
+    "another head count": lambda o: o.update(n_kv=4),
+    "heads no multiple of kv heads": lambda o: o.update(n_heads=7),
+    "no kv heads": lambda o: o.update(n_kv=0),
+    "another head size": lambda o: o.update(head_dim=32),
+    "scales in bfloat16": lambda o: o.update(kscale=o["kscale"].bfloat16()),
+    "scales per page": lambda o: o.update(vscale=o["vscale"][:, :1].contiguous()),
+    "strided scales": lambda o: o.update(vscale=strided(o["vscale"])),
+    "strided store": lambda o: o.update(kcache=torch.cat([o["kcache"].view(torch.uint8)] * 2, dim=1)[:, :G].view(torch.float8_e4m3fn)),
+    "table of 64-bit entries": lambda o: o.update(table=o["table"].long()),
+    "flat table": lambda o: o.update(table=o["table"].view(-1)),
+    "positions of 64 bits": lambda o: o.update(positions=o["positions"].long(), start_pos=o["start_pos"].long()),
+    "float16 queries": lambda o: o.update({k: o[k].half() for k in ("q", "out", "k", "v")}),
+    "out of another type": lambda o: o.update(out=o["out"].bfloat16()),
+    "out of another shape": lambda o: o.update(out=o["out"][:, :-1]),
+    "queries of another width": lambda o: o.update(q=torch.zeros(N, H * HD + 4)),
+    "queries without dense rows": lambda o: o.update(q=strided(o["q"])),
+}
+
+
+@pytest.mark.parametrize("what", BAD)
+@pytest.mark.parametrize("call", CALLS)
+def test_refused(call, what):
+    o = operands()
+    BAD[what](o)
+    with pytest.raises(KernelError) as e:
+        CALLS[call](o)
+    assert "CUDA device" not in str(e.value)          # looked at before the device is
+
+
+@pytest.mark.parametrize("what,change", [
+    ("k of another type", lambda o: o.update(k=o["k"].bfloat16())),
+    ("v of another width", lambda o: o.update(v=o["v"][:, :HD])),
+    ("k without dense rows", lambda o: o.update(k=strided(o["k"]))),
+    ("angles in 64 bits", lambda o: o.update(cos_sin=o["cos_sin"].double())),
+    ("an odd rotary width", lambda o: o.update(cos_sin=torch.zeros(40, 33))),
+    ("a rotary width beyond the head", lambda o: o.update(cos_sin=torch.zeros(40, 2 * HD))),
+    ("too few positions", lambda o: o.update(positions=o["positions"][:4])),
+    ("no table row for a request", lambda o: o.update(table=o["table"][:2])),
+    ("several tokens of a request without token_req", lambda o: o.update(token_req=None)),
+    ("pages of 4097 tokens", lambda o: o.update({k: torch.zeros(2, G, 4097, HD, dtype=torch.uint8).view(torch.float8_e4m3fn)
+                                                 for k in ("kcache", "vcache")} | dict(kscale=torch.ones(2, G), vscale=torch.ones(2, G)))),
+])
+def test_append_refuses(what, change):
+    o = operands()
+    change(o)
+    with pytest.raises(KernelError) as e:
+        append(o)
+    assert "CUDA device" not in str(e.value)
+
+
+def test_attention_refuses_missing_rows():
+    o = operands()
+    o.update(token_req=None)                       # five rows, three requests
+    with pytest.raises(KernelError, match="per token"):
+        decode(o)
+    o = operands()
+    o.update(q_start=o["q_start"][:3])
+    with pytest.raises(KernelError, match="cover the requests"):
+        prefill(o)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 7, 64, 500])
+@pytest.mark.parametrize("n_kv,group,hd", [(4, 8, 64), (8, 4, 128), (32, 1, 128), (1, 32, 128), (1, 1, 256), (8, 12, 256)])
+@pytest.mark.parametrize("ctx", [1, 127, 128, 129, 2048, 131072, 2 ** 31 - 1])
+def test_parts_of_a_context(tokens, n_kv, group, hd, ctx, monkeypatch):
+    monkeypatch.setattr(kernels, "sm_count", lambda: 148)
+    ranges, cluster = kernels.decode_q8_parts(tokens, n_kv, group, hd, ctx)
+    assert cluster in (1, 2, 4, 8) and ranges >= 1
+    assert ranges == 1 or cluster == 8
+    blocks = -(-ctx // 128)
+    assert ranges * cluster <= max(1, blocks), "a part for every 128 keys at most"
