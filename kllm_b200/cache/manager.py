@@ -22,6 +22,11 @@ Beside the pages, every request holds one state slot.  A mixer with per-request
 state of fixed size (``StateNeed``) gets a tensor [max_requests, *shape] per layer
 (a layer may ask for several, told apart by name), and the slot's rows are zeroed when a request opens.  Models without such a mixer
 hold and return their slots all the same.
+
+The pages may be kept in 8 bits (``cache_dtype=torch.float8_e4m3fn``): every layer must say that its kernels take that
+(``PagedKVNeed.eight_bits``), and beside the e4m3 stores a layer then has a float32 scale per page and kv head for its
+keys and one for its values, which the appending kernel keeps (csrc/q8.cuh).  A page that is handed out again needs no clearing: its
+first slot is always the first to be written, and that starts its scales anew.
 """
 from __future__ import annotations
 
@@ -93,6 +98,8 @@ class CacheGroup:
                                              # values are the keys (then v_store is k_store)
     k_store: Optional[torch.Tensor] = None   # [len(slots), pages, kv heads, page_size, head_dim]
     v_store: Optional[torch.Tensor] = None   # [len(slots), pages, kv heads, page_size, value size]
+    k_scale: Optional[torch.Tensor] = None   # pages in 8 bits: float32 [len(slots), pages, kv heads]
+    v_scale: Optional[torch.Tensor] = None
 
     @property
     def window(self) -> Optional[int]:
@@ -114,15 +121,21 @@ class RequestCache:
 
 class CacheManager:
     def __init__(self, needs: Sequence, page_size: int, num_pages: int, max_requests: int,
-                 dtype: torch.dtype = torch.float32, device="cpu", allocate: bool = True):
+                 dtype: torch.dtype = torch.float32, device="cpu", allocate: bool = True,
+                 cache_dtype: Optional[torch.dtype] = None):
         """``needs[i]`` is what cache slot i asks for: None, a PagedKVNeed, a
-        StateNeed, or a list of them.  ``num_pages`` is the size of every group's pool."""
+        StateNeed, or a list of them.  ``num_pages`` is the size of every group's pool.  ``dtype`` is the model's;
+        the pages are kept in ``cache_dtype``: the same (None) or float8_e4m3fn."""
         if page_size <= 0:
             raise ValueError(f"page_size must be positive, got {page_size}")
         self.page_size = page_size
         self.num_pages = num_pages
         self.max_requests = max_requests
         self.dtype = dtype
+        self.cache_dtype = cache_dtype or dtype
+        self.eight_bits = self.cache_dtype == torch.float8_e4m3fn
+        if not self.eight_bits and self.cache_dtype != dtype:
+            raise ValueError(f"pages are kept in the model's dtype ({dtype}) or in float8_e4m3fn, not in {cache_dtype}")
         self.device = torch.device(device)
         self.groups: List[CacheGroup] = []
         self.slot_group: Dict[int, int] = {}       # cache slot -> group index
@@ -145,6 +158,9 @@ class CacheManager:
                             item.value_heads != item.n_kv_heads or item.value_dim > item.head_dim)):
                         raise ValueError(f"cache slot {slot}: {item.value_heads} value heads of {item.value_dim} under "
                                          f"{item.n_kv_heads} key heads of {item.head_dim}")
+                    if self.eight_bits and not item.eight_bits:
+                        raise ValueError(f"cache slot {slot}: this kind of layer does not take a cache in 8 bits "
+                                         f"({item.n_kv_heads} key heads of {item.head_dim})")
                     key = (item.n_kv_heads, item.head_dim, item.window, item.value_dim, item.values_are_keys,
                            item.value_heads, item.keep_first)
                     g = by_key.get(key)
@@ -173,7 +189,13 @@ class CacheManager:
             for g in self.groups:
                 L, G, hd, vd = len(g.slots), g.need.n_kv_heads, g.need.head_dim, g.need.value_dim
                 Gv = g.need.value_heads
-                if g.need.values_are_keys:
+                if self.eight_bits:
+                    g.storage = torch.zeros((L, 2, num_pages, G, page_size, hd), dtype=torch.uint8, device=self.device)
+                    stores = g.storage.view(self.cache_dtype)
+                    g.k_store, g.v_store = stores[:, 0], stores[:, 1]
+                    scales = torch.ones((2, L, num_pages, G), dtype=torch.float32, device=self.device)
+                    g.k_scale, g.v_scale = scales[0], scales[1]
+                elif g.need.values_are_keys:
                     g.storage = torch.zeros((L, num_pages, G, page_size, hd), dtype=dtype, device=self.device)
                     g.k_store = g.v_store = g.storage
                 elif Gv != G:
@@ -198,18 +220,23 @@ class CacheManager:
     def bytes_per_page(self) -> int:
         """Device bytes that one more page in EVERY group's pool costs: keys and values of
         all layers of all groups (the pools have the same number of pages)."""
-        esize = torch.empty((), dtype=self.dtype).element_size()
-        return sum(len(g.slots) * self.page_size * g.need.stored_per_token * esize
-                   for g in self.groups)
+        return sum(self._page_bytes(g) for g in self.groups)
+
+    def _page_bytes(self, g: CacheGroup) -> int:
+        """Device bytes of one page of a group's layers, scales included."""
+        esize = torch.empty((), dtype=self.cache_dtype).element_size()
+        scales = 4 * (g.need.n_kv_heads + g.need.value_heads) if self.eight_bits else 0
+        return len(g.slots) * (self.page_size * g.need.stored_per_token * esize + scales)
 
     @classmethod
-    def pages_within(cls, needs: Sequence, page_size: int, dtype: torch.dtype, budget_bytes: int) -> int:
+    def pages_within(cls, needs: Sequence, page_size: int, dtype: torch.dtype, budget_bytes: int,
+                     cache_dtype: Optional[torch.dtype] = None) -> int:
         """How many pages per pool fit ``budget_bytes`` of device memory: the budget over
         ``bytes_per_page()`` (the reference's rule, pages = budget / (layers * 2 * page *
         kv width * element size); it sized a pool by a fixed count first and ran out of
         memory on a larger model, docs/JOURNAL.md:364-367, tools/modal_lab.py:232-240).
         Raises when not even one page fits."""
-        per = cls(needs, page_size, 1, max_requests=1, dtype=dtype, allocate=False).bytes_per_page()
+        per = cls(needs, page_size, 1, max_requests=1, dtype=dtype, allocate=False, cache_dtype=cache_dtype).bytes_per_page()
         if per == 0:
             return 1                  # no paged cache in this model: one page that nobody takes
         pages = int(budget_bytes) // per
@@ -219,10 +246,8 @@ class CacheManager:
 
     def bytes_per_token_full(self) -> int:
         """Cache bytes that one more token of context costs in the groups that keep
-        every key."""
-        esize = torch.empty((), dtype=self.dtype).element_size()
-        return sum(len(g.slots) * g.need.stored_per_token * esize
-                   for g in self.groups if g.window is None)
+        every key (scales, which a page's tokens share, rounded up)."""
+        return -(-sum(self._page_bytes(g) for g in self.groups if g.window is None) // self.page_size)
 
     def pages_ever_needed(self, total_tokens: int) -> List[int]:
         """Per group, the most pages a request of ``total_tokens`` tokens must hold at one
@@ -353,14 +378,17 @@ class CacheManager:
         """One ``LayerCache`` per cache slot, with this step's device block tables."""
         out = []
         for slot in range(self.n_slots):
-            k = v = table = None
+            k = v = table = k_scale = v_scale = None
             if slot in self.slot_group:
                 g = self.groups[self.slot_group[slot]]
                 layer = self.slot_layer[slot]
                 k, v = g.k_store[layer], g.v_store[layer]
+                if self.eight_bits:
+                    k_scale, v_scale = g.k_scale[layer], g.v_scale[layer]
                 table = block_tables[g.index]
             out.append(LayerCache(k=k, v=v, block_table=table, state=self.state.get(slot),
-                                  writes=True, page_size=self.page_size, states=self.named_states.get(slot, {})))
+                                  writes=True, page_size=self.page_size, k_scale=k_scale, v_scale=v_scale,
+                                  states=self.named_states.get(slot, {})))
         return out
 
     # ---- checks for tests and debugging -------------------------------------

@@ -28,6 +28,7 @@ from .step import StepEntry, StepRunner
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32,
            "fp32": torch.float32}
+_CACHE_DTYPES = {"": None, "float8_e4m3fn": torch.float8_e4m3fn, "float8_e4m3": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn}
 
 
 @dataclass
@@ -41,6 +42,7 @@ class Options:
     max_batch: int = 8            # most requests in one step
     dtype: str = "bfloat16"       # "bfloat16" (serving) or "float32" (true 32-bit)
     cuda_graphs: bool = True      # replay decode steps as CUDA graphs
+    cache_dtype: str = ""         # "" (the model's) or "float8_e4m3fn": keys and values in 8 bits, a scale per page and kv head
 
     def fill(self) -> "Options":
         o = Options(**self.__dict__)
@@ -57,6 +59,8 @@ class Options:
             o.max_batch = 8
         if o.dtype not in _DTYPES:
             raise ValueError(f"dtype {o.dtype!r}: choose bfloat16 or float32")
+        if o.cache_dtype not in _CACHE_DTYPES:
+            raise ValueError(f"cache dtype {o.cache_dtype!r}: choose float8_e4m3fn, or nothing for the model's")
         return o
 
 
@@ -118,9 +122,10 @@ class Engine:
             del tensors
             if opts.num_blocks <= 0:
                 opts.num_blocks = CacheManager.pages_within(self.model.cache_needs(), opts.block_size,
-                                                            self.dtype, opts.cache_bytes)
+                                                            self.dtype, opts.cache_bytes, _CACHE_DTYPES[opts.cache_dtype])
             self.cache = CacheManager(self.model.cache_needs(), opts.block_size, opts.num_blocks,
-                                      max_requests=opts.max_batch, dtype=self.dtype, device=self.device)
+                                      max_requests=opts.max_batch, dtype=self.dtype, device=self.device,
+                                      cache_dtype=_CACHE_DTYPES[opts.cache_dtype])
         self.runner = StepRunner(self.model, self.cache, opts.max_step_tokens, opts.max_batch, opts.max_seq,
                                  use_graphs=opts.cuda_graphs)
         self.sampler = Sampler(self.device)

@@ -3,7 +3,7 @@ logits.  It samples nothing.  It drives the engine's own model, step function,
 cache manager and kernels, the ones that generation uses.
 
     trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N [--trace FILE]
-              [--page-size P] [--max-requests R]
+              [--page-size P] [--max-requests R] [--cache-dtype float8_e4m3fn]
 
 Steps come on standard input (or from ``--trace FILE``), one JSON object a line:
 
@@ -41,6 +41,7 @@ def main(argv=None) -> int:
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--max-requests", type=int, default=4, help="requests that may be live at a time (state slots)")
     ap.add_argument("--device", type=int, default=0)
+    ap.add_argument("--cache-dtype", default="", choices=["", "float8_e4m3fn"], help="float8_e4m3fn: the cache in 8 bits")
     ap.add_argument("--trace", default="", help="read the steps from this file instead of standard input")
     args = ap.parse_args(argv)
     if args.max_tokens <= 0 or args.page_size <= 0 or 64 % args.page_size:
@@ -60,7 +61,8 @@ def main(argv=None) -> int:
     pages = -(-args.max_tokens // args.page_size)
     eng = Engine(args.model, Options(device=args.device, dtype=args.dtype, max_seq=max_pos,
                                      block_size=args.page_size, num_blocks=pages,
-                                     max_step_tokens=max(args.max_tokens, 1), max_batch=max(1, args.max_requests)))
+                                     max_step_tokens=max(args.max_tokens, 1), max_batch=max(1, args.max_requests),
+                                     cache_dtype=args.cache_dtype))
     live = {}
     held = {}       # request id -> tokens fed so far (the position of its next token)
     index = []

@@ -1039,6 +1039,7 @@ def attention_prefill_tcgen05(out, q, kcache, vcache, q_start, start_pos, block_
 Q8_DTYPE = torch.float8_e4m3fn        # what a cache in 8 bits holds, beside one float32 power of two per page and kv head
 Q8_HEAD_DIMS = tuple(range(32, 257, 32))
 Q8_MAX_PAGE = 4096
+Q8_MAX_GROUP = 64                     # query heads over one kv head
 
 
 def _check_q8(what, kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim):

@@ -211,7 +211,16 @@ class PagedAttention:
     def cache_need(self):
         return PagedKVNeed(self.n_kv * self.maps, self.head_dim, self.window,
                            None if self.v_head_dim == self.head_dim else self.v_head_dim,
-                           n_v_heads=self.n_kv if self.maps > 1 else None, keep_first=self.keep_first)
+                           n_v_heads=self.n_kv if self.maps > 1 else None, keep_first=self.keep_first,
+                           eight_bits=self._takes_eight_bits())
+
+    def _takes_eight_bits(self):
+        """Whether the kernels of a cache in 8 bits serve this layer: plain scores over values of the keys' size, stored by the
+        rotary part or as they are."""
+        return (not self._prepares and self.score_slopes is None and self.v_head_dim == self.head_dim
+                and not self.exact_weights and not self.segment and not self.keep_first
+                and self.head_dim in kernels.Q8_HEAD_DIMS and self.n_heads // self.n_kv <= kernels.Q8_MAX_GROUP
+                and (self.position is None or getattr(self.position, "writes_eight_bits", False)))
 
     def _split(self, qkv, writes):
         q = qkv[:, :self.q_dim]
@@ -271,6 +280,8 @@ class PagedAttention:
         if (self.score_slopes is not None or self.v_head_dim != self.head_dim or self.exact_weights or self.segment
                 or self.keep_first):
             table = None          # ... and has no bias on its scores, one head size, bfloat16 weights, a plain window
+        if cache.k_scale is not None:
+            table = None          # ... and a cache in the model's dtype
         wide = (table is not None and cache.writes and ctx.all_single and self.dtype == torch.float32
                 and kernels.attention_decode_f32_fits(self.n_heads, self.n_kv, self.head_dim))
         if wide or (table is not None and cache.writes and ctx.all_single and self.dtype == torch.bfloat16 and group <= 16
@@ -293,10 +304,17 @@ class PagedAttention:
             return attn
         if self.position is not None:
             self.position.apply(q, k, v, ctx, cache, self.n_heads, self.n_kv)
+        elif cache.writes and cache.k_scale is not None:
+            kernels.rope_append_q8(q, q, k, v, None, ctx.positions, ctx.token_req, ctx.q_start, cache.block_table, cache.k, cache.v,
+                                   cache.k_scale, cache.v_scale, self.n_heads, self.n_kv, self.head_dim)
         elif cache.writes:
             kernels.rope_append(q, k, v, None, ctx.positions, ctx.token_req, cache.block_table,
                                 cache.k, cache.v, self.n_heads, self.n_kv, self.head_dim)
         attn = torch.empty((n, self.o_dim), dtype=self.dtype, device=q.device)
+        if cache.k_scale is not None:
+            kernels.attention_q8(attn, q, cache.k, cache.v, cache.k_scale, cache.v_scale, ctx, cache.block_table, self.n_heads,
+                                 self.n_kv, self.head_dim, self.window or 0, self.scale)
+            return attn
         kernels.attention(attn, q, cache.k, cache.v, ctx, cache.block_table, self.n_heads, self.n_kv,
                           self.head_dim, self.window or 0, self.scale, score_slopes=self.score_slopes,
                           v_head_dim=self.v_head_dim, exact_weights=self.exact_weights, segment=self.segment,

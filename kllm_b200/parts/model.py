@@ -9,6 +9,7 @@ backend/model.cu:1181-1188; here the caller names the rows).
 """
 from __future__ import annotations
 
+import dataclasses
 from typing import Dict, List, Optional
 
 import torch
@@ -100,7 +101,11 @@ class DecoderModel:
         needs = []
         for slot in range(self.n_cache_slots):
             block = self.blocks[self._writer_block[slot]]
-            needs.append((block if hasattr(block, "cache_need") else block.mixer).cache_need())
+            need = (block if hasattr(block, "cache_need") else block.mixer).cache_need()
+            if isinstance(need, PagedKVNeed) and need.eight_bits and not all(
+                    getattr(self.blocks[c.block].mixer.cache_need(), "eight_bits", False) for c in self.schedule if c.cache == slot):
+                need = dataclasses.replace(need, eight_bits=False)      # another layer reads this slot, and cannot
+            needs.append(need)
         return needs
 
     # ---- one step --------------------------------------------------------
@@ -124,8 +129,7 @@ class DecoderModel:
         for i, call in enumerate(schedule):
             cache = caches[call.cache]
             if cache.writes != call.writes_cache:
-                cache = LayerCache(cache.k, cache.v, cache.block_table, cache.state,
-                                   writes=call.writes_cache, page_size=cache.page_size, states=cache.states)
+                cache = dataclasses.replace(cache, writes=call.writes_cache)
             layer = self.blocks[call.block]
             if call.entry is not None:
                 if hasattr(pending, "settle"):

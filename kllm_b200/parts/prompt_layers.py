@@ -76,6 +76,8 @@ class PromptLayers:
                 or not kernels.USE_TCGEN05 or self.head_dim not in kernels.TCGEN05_HEAD_DIMS):
             return False
         c = caches[self.slots[0]]
+        if c.k_scale is not None:          # a cache in 8 bits: the parts' own forward
+            return False
         return kernels.prompt_layers_ready() and all(
             caches[i].block_table is c.block_table and caches[i].k.shape[2] == c.page_size for i in self.slots)
 

@@ -8,7 +8,8 @@ how the reference forms its angles (backend/model.cu:176-178).
 
 Interface of a position part used by the attention mixer:
 ``apply(q, k, v, ctx, cache, n_heads, n_kv_heads)`` rotates q in place and, when the
-layer writes its cache, stores rotated k and v into the pages.  Optional:
+layer writes its cache, stores rotated k and v into the pages (``writes_eight_bits = True``: into those of a cache in
+8 bits as well, where ``cache.k_scale`` is there).  Optional:
 ``full_rotary_table()`` returns the cos/sin table when the whole head is rotated, for
 a mixer whose kernel can do the rotation itself.
 """
@@ -72,6 +73,8 @@ def rotary_frequencies(dims: int, base: float, scaling=None):
 
 
 class RotaryEmbedding:
+    writes_eight_bits = True
+
     def __init__(self, spec: PartSpec, env: BuildEnv):
         self.head_dim = int(spec.params["head_dim"])
         self.theta = float(spec.params["theta"])
@@ -96,6 +99,10 @@ class RotaryEmbedding:
 
     def apply(self, q, k, v, ctx, cache, n_heads, n_kv_heads):
         writes = cache.writes and cache.k is not None
+        if writes and cache.k_scale is not None:
+            kernels.rope_append_q8(q, q, k, v, self.cos_sin, ctx.positions, ctx.token_req, ctx.q_start, cache.block_table,
+                                   cache.k, cache.v, cache.k_scale, cache.v_scale, n_heads, n_kv_heads, self.head_dim)
+            return
         kernels.rope_append(q, k, v, self.cos_sin, ctx.positions, ctx.token_req,
                             cache.block_table if writes else None,
                             cache.k if writes else None, cache.v if writes else None,

@@ -101,7 +101,9 @@ class PagedKVNeed:
     keys'; with a ``v_head_dim`` below ``head_dim`` the values are the first ``v_head_dim`` elements
     of that row (a row that carries something beside the latent for the keys alone).
     n_v_heads: the heads of the value store where they are fewer than the key heads (None: the
-    same): n_kv_heads / n_v_heads neighbouring key heads attend over one value head."""
+    same): n_kv_heads / n_v_heads neighbouring key heads attend over one value head.
+    eight_bits: the layer writes and reads a cache in 8 bits too (``LayerCache.k_scale``), where the engine is asked
+    for one."""
     n_kv_heads: int
     head_dim: int
     window: Optional[int] = None
@@ -109,6 +111,7 @@ class PagedKVNeed:
     values_are_keys: bool = False
     n_v_heads: Optional[int] = None
     keep_first: int = 0
+    eight_bits: bool = field(default=False, compare=False)
 
     @property
     def value_dim(self) -> int:

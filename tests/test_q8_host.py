@@ -120,3 +120,74 @@ def test_parts_of_a_context(tokens, n_kv, group, hd, ctx, monkeypatch):
     assert ranges == 1 or cluster == 8
     blocks = -(-ctx // 128)
     assert ranges * cluster <= max(1, blocks), "a part for every 128 keys at most"
+
+
+# ---- the manager and the options -----------------------------------------------------------------------------------------
+
+def test_manager_keeps_pages_in_eight_bits():
+    from kllm_b200.cache.manager import CacheManager
+    from kllm_b200.parts.spec import PagedKVNeed
+    full, near = PagedKVNeed(2, 64, eight_bits=True), PagedKVNeed(2, 64, window=32, eight_bits=True)
+    m = CacheManager([full, near, full], 16, 5, max_requests=2, dtype=torch.bfloat16, cache_dtype=torch.float8_e4m3fn)
+    tables = {g.index: torch.zeros(1, 1, dtype=torch.int32) for g in m.groups}
+    for c in m.layer_caches(tables):
+        assert c.k.dtype == c.v.dtype == torch.float8_e4m3fn and c.k.shape == (5, 2, 16, 64) and c.k.is_contiguous()
+        assert c.k_scale.shape == c.v_scale.shape == (5, 2) and c.k_scale.dtype == torch.float32 and c.k_scale.is_contiguous()
+    assert m.layer_caches(tables)[0].k_scale.data_ptr() != m.layer_caches(tables)[2].k_scale.data_ptr()
+    assert m.bytes_per_page() == 3 * (16 * 2 * 2 * 64 + 2 * 2 * 4)
+    assert m.bytes_per_token_full() == -(-2 * (16 * 2 * 2 * 64 + 2 * 2 * 4) // 16)
+    wide = CacheManager([full, near, full], 16, 5, max_requests=2, dtype=torch.bfloat16)
+    assert all(c.k_scale is None and c.k.dtype == torch.bfloat16 for c in wide.layer_caches(tables))
+    assert wide.bytes_per_page() == 3 * 16 * 2 * 2 * 64 * 2 and wide.bytes_per_token_full() == 2 * 2 * 2 * 64 * 2
+    budget = 100 * m.bytes_per_page()
+    assert CacheManager.pages_within([full, near, full], 16, torch.bfloat16, budget, torch.float8_e4m3fn) == 100
+    assert CacheManager.pages_within([full, near, full], 16, torch.bfloat16, budget) == 50
+
+
+def test_manager_refuses_layers_that_cannot():
+    from kllm_b200.cache.manager import CacheManager
+    from kllm_b200.parts.spec import PagedKVNeed
+    with pytest.raises(ValueError, match="does not take a cache in 8 bits"):
+        CacheManager([PagedKVNeed(2, 64, eight_bits=True), PagedKVNeed(2, 64)], 16, 5, max_requests=2,
+                     cache_dtype=torch.float8_e4m3fn)
+    with pytest.raises(ValueError, match="model's dtype"):
+        CacheManager([PagedKVNeed(2, 64, eight_bits=True)], 16, 5, max_requests=2, dtype=torch.float32, cache_dtype=torch.bfloat16)
+
+
+def test_which_layers_take_it():
+    from kllm_b200.config.base import build_model_spec, parse_config
+    from kllm_b200 import models  # noqa: F401
+    from kllm_b200.parts.model import DecoderModel
+
+    def needs(head_dim, **params):
+        cfg = {"architectures": ["LlamaForCausalLM"], "num_hidden_layers": 1, "hidden_size": 64, "num_attention_heads": 4,
+               "num_key_value_heads": 2, "head_dim": head_dim, "intermediate_size": 64, "vocab_size": 64, "max_position_embeddings": 64}
+        spec = build_model_spec(parse_config(cfg))
+        spec.blocks[0].mixer.params.update(params)
+        return [n.eight_bits for n in DecoderModel(spec, torch.float32, "cpu").cache_needs()]
+    assert needs(64) == [True] and needs(32, window=16) == [True] and needs(64, position=None) == [True]
+    assert needs(16) == [False] and needs(48) == [False]
+    for other in (dict(segment=8), dict(exact_weights=True), dict(v_head_dim=32), dict(score_slopes="geometric"),
+                  dict(window=16, keep_first=2)):
+        assert needs(64, **other) == [False], other
+
+
+def test_a_reader_that_cannot_keeps_the_slot_wide():
+    from kllm_b200 import models  # noqa: F401
+    from kllm_b200.config.base import build_model_spec, parse_config
+    from kllm_b200.parts.model import DecoderModel
+    from kllm_b200.parts.spec import LayerCall
+    cfg = {"architectures": ["LlamaForCausalLM"], "num_hidden_layers": 3, "hidden_size": 64, "num_attention_heads": 4,
+           "num_key_value_heads": 2, "head_dim": 32, "intermediate_size": 64, "vocab_size": 64, "max_position_embeddings": 64}
+    for reader, want in ((dict(score_slopes="geometric"), [False, True]), ({}, [True, True])):
+        spec = build_model_spec(parse_config(cfg))
+        spec.blocks[1].mixer.params.update(reader)
+        spec.schedule = [LayerCall(0, 0), LayerCall(1, 0, writes_cache=False), LayerCall(2, 1)]
+        assert [n.eight_bits for n in DecoderModel(spec, torch.float32, "cpu").cache_needs()] == want
+
+
+def test_options_name_it():
+    from kllm_b200.engine.engine import Options
+    assert Options().fill().cache_dtype == "" and Options(cache_dtype="float8_e4m3fn").fill().cache_dtype == "float8_e4m3fn"
+    with pytest.raises(ValueError, match="cache dtype"):
+        Options(cache_dtype="int8").fill()
