@@ -19,6 +19,8 @@
 // key becomes zeros.
 #include "q8.cuh"
 
+#include <atomic>
+
 #ifndef KLLM_HD
 #error "compile with -DKLLM_HD=<head size, a multiple of 32 up to 256>"
 #endif
@@ -68,28 +70,42 @@ template <int N> __device__ __forceinline__ void split(float x, __half (&p)[N]) 
 
 // ---- single tokens ---------------------------------------------------------------------------------------------------
 //
-// What bounds it: bytes.  Every warp walks its own tiles of keys with no shared memory and no meeting: a lane's loads of a
-// key tile are the tensor core's operand itself.  Keys are the M side (A, 16 keys x 16 dims), the heads of the group the N
-// side (8 at a time): lane (g, t) = (lane / 4, lane % 4) holds rows g and g + 8, and because the order of the dims under a
-// sum is free, its dims are 16 neighbours of every 64 (one 16-byte load), the same for the queries.  The second product
-// takes values as A with the dims as M: lane (g, t) holds HD / 8 neighbouring dims of keys 2t, 2t + 1, 2t + 8, 2t + 9, two
-// keys' bytes are interleaved (prmt) and converted to the pairs that the operand wants, and the weights, whose layout
-// is (key, head), become the B operand by an 8 x 8 transposition in registers (movmatrix).  A tile's keys are loaded while
-// the values before them are used, a tile's values while its scores are computed.
+// What bounds it: bytes.  Every warp walks its own tiles of keys, which it requests ahead into a ring of its own in shared
+// memory (cp.async), without meeting other warps.  The tensor core's operands are read from there as they lie: keys are
+// the M side (A, 16 keys x 16 dims), the heads of the group the N side (8 at a time); lane (g, t) = (lane / 4, lane % 4)
+// holds rows g and g + 8, and because the order of the dims under a sum is free, its dims are 16 neighbours of every 64
+// (one 16-byte read), the same for the queries.  The second product takes values as A with the dims as M: lane (g, t)
+// holds HD / 8 neighbouring dims of rows 2t, 2t + 1, 2t + 8, 2t + 9; two rows' bytes are interleaved (prmt) and converted
+// to the pairs that the operand wants, and the weights, whose layout is (key, head), become the B operand by an 8 x 8
+// transposition in registers (movmatrix).  Row r of a tile is key r ^ (r >> 1 & 1) of it, and the 16-byte pieces of key j lie
+// at piece ^ swizzle(j): with both, neither kind of read meets a bank twice at head sizes 64 and 128.
 
 constexpr int DEC_KT = HD <= 128 ? 32 : 16;              // keys of a warp's tile
 constexpr int DEC_MT = DEC_KT / 16;
 constexpr int DEC_WARPS = 4;
+constexpr int DEC_STAGES = HD <= 32 ? 4 : HD <= 64 ? 3 : 2;
 constexpr int KW = HD % 64 == 0 ? 4 : 2;                 // words of a lane's piece of a key row
 constexpr int KC = HD / (16 * KW);                       // pieces of a key row (16 * KW dims each)
 constexpr int VW = HD / 32;                              // words of a lane's piece of a value row
+constexpr int PIECES = HD / 16;                          // 16-byte pieces of a row
+constexpr int DEC_TILE = DEC_KT * HD;                    // bytes of a tile of keys (or values)
+constexpr int DEC_META = DEC_KT * 8;                     // a tile's scales: (key scale, value scale) per key
+constexpr int DEC_RING = DEC_STAGES * 2 * DEC_TILE + (DEC_STAGES + 1) * DEC_META;
+
+__device__ __forceinline__ int dec_swizzle(int key) {
+    return PIECES == 8 || PIECES == 16 ? (key & 6) ^ ((key & 1) << 2) : PIECES == 4 ? (key >> 1) & 2 : 0;
+}
+__device__ __forceinline__ int dec_key(int row) { return row ^ ((row >> 1) & 1); }
 
 template <typename T, int NG> struct DecodeShape {
     static constexpr int NQ = Parts<T>::Q;
     static constexpr int QREGS = HD / 16 * 2 * NQ * NG;
     static constexpr bool Q_IN_REGS = QREGS <= 32;
-    // CTAs an SM: what the registers of a lane allow without spills
-    static constexpr int CTAS = HD <= 64 ? (NG == 1 ? 5 : 4) : HD <= 128 ? (NG == 1 ? 4 : 3) : 2;
+    static constexpr int Q_BYTES = Q_IN_REGS ? 0 : HD / 16 * NQ * NG * 32 * 8;
+    static constexpr int SUM_BYTES = DEC_WARPS * 8 * NG * HD * 4;     // over the rings, when they are done with
+    static constexpr int SMEM = Q_BYTES + (DEC_WARPS * DEC_RING > SUM_BYTES ? DEC_WARPS * DEC_RING : SUM_BYTES);
+    // CTAs an SM, by shared memory and registers
+    static constexpr int CTAS = HD <= 64 ? 4 : HD <= 128 ? 3 : 2;
 };
 
 struct DecodeArgs {
@@ -106,27 +122,40 @@ struct DecodeArgs {
     const int* token_req;
     const int* block_table;
     int max_blocks, n_pages, n_requests, n_heads, n_kv, subs, heads_per_cta, page_size, window, ranges;
+    bool q_by_four;              // rows of queries may be read four numbers at a time
     float scale;
 };
 
-template <int W> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&r)[W]) {
-    if constexpr (W % 4 == 0) {
+// four numbers of a row of queries, zeros where the row is none
+template <typename T> __device__ __forceinline__ void load4(const T* p, bool there, bool by_four, float (&x)[4]) {
+    x[0] = x[1] = x[2] = x[3] = 0.f;
+    if (!there) return;
+    if (!by_four) {
 #pragma unroll
-        for (int i = 0; i < W; i += 4) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + 4 * i));
-            r[i] = v.x; r[i + 1] = v.y; r[i + 2] = v.z; r[i + 3] = v.w;
-        }
-    } else if constexpr (W % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < W; i += 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p + 4 * i));
-            r[i] = v.x; r[i + 1] = v.y;
-        }
+        for (int i = 0; i < 4; i++) x[i] = to_f32(p[i]);
+    } else if constexpr (sizeof(T) == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u);
+        x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
     } else {
-#pragma unroll
-        for (int i = 0; i < W; i++) r[i] = __ldg(reinterpret_cast<const uint32_t*>(p + 4 * i));
+        const float4 w = *reinterpret_cast<const float4*>(p);
+        x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
     }
 }
+template <int W> __device__ __forceinline__ void read_words(unsigned addr, uint32_t* r) {
+    if constexpr (W == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+    else if constexpr (W == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];\n" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+    else asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(r[0]) : "r"(addr));
+}
+// bytes 16, or 0: the place is filled with zeros
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(unsigned dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ unsigned cluster_size() {
     unsigned r;
@@ -141,12 +170,38 @@ __device__ __forceinline__ unsigned cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
 }
-__device__ __forceinline__ float peer_load(const float* p, unsigned rank) {
-    unsigned a = (unsigned)__cvta_generic_to_shared(p), b;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(b) : "r"(a), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(b));
+__device__ __forceinline__ unsigned peer_addr(const void* p, unsigned rank) {
+    unsigned b;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(b) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+    return b;
+}
+__device__ __forceinline__ float2 peer_load2(const void* p, unsigned rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(peer_addr(p, rank)));
     return v;
+}
+__device__ __forceinline__ float4 peer_load4(const void* p, unsigned rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_addr(p, rank)));
+    return v;
+}
+// What a part with reference m and sum l counts beside the reference of all parts.  A part without a seen key has -inf and 0;
+// one that met only NaN has -inf and NaN, which stays.
+__device__ __forceinline__ float part_factor(float m, float l, float all) {
+    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - all);
+}
+__device__ __forceinline__ void add_scaled(float4& x, float f, const float4& y) {
+    x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+}
+// x / l, zeros where no key was seen
+template <typename T> __device__ __forceinline__ void store_row4(T* dst, const float4& x, float l) {
+    const float4 y = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x / l, x.y / l, x.z / l, x.w / l);
+    if constexpr (sizeof(T) == 2) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+        *reinterpret_cast<float4*>(dst) = y;
+    }
 }
 
 // grid: (ranges * cluster, kv heads * subgroups of heads, tokens), clusters along x; a cluster's CTAs take neighbouring
@@ -156,14 +211,12 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, (DecodeShape<T, NG>::CTAS))
 attn_decode_q8_kernel(const DecodeArgs a) {
     constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P, NH = 8 * NG;
     constexpr bool Q_IN_REGS = DecodeShape<T, NG>::Q_IN_REGS;
-    constexpr int QSM = HD / 16 * NQ * NG * 32;                       // uint2 per lane: [kk][part][ng][lane]
-    extern __shared__ __align__(16) unsigned char smem[];
-    uint2* sq = reinterpret_cast<uint2*>(smem);                       // the queries as operands
-    float* so = reinterpret_cast<float*>(smem + QSM * 8);             // [warps][NH][HD], then the CTA's sum [NH][HD]
+    using Shape = DecodeShape<T, NG>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    uint2* sq = reinterpret_cast<uint2*>(smem);                       // the queries as operands: [kk][part][ng][lane]
+    float* so = reinterpret_cast<float*>(smem + Shape::Q_BYTES);      // [warps][NH][HD], then the CTA's sum [NH][HD]
     __shared__ float s_ml[DEC_WARPS][NH][2];                          // references and sums of the warps
-    __shared__ float s_cta[NH][2];                                    // ... of the CTA
-    __shared__ float s_factor[NH];                                    // log2(e) scale 2^(the row's power), NaN: the row is
-    __shared__ int s_amax[NH];
+    __shared__ __align__(8) float s_cta[NH][2];                                    // ... of the CTA
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
@@ -173,54 +226,6 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     const int p = (req >= 0 && req < a.n_requests) ? a.positions[token] : -1;
     const int hi = p + 1, lo = (a.window > 0 && hi > a.window) ? hi - a.window : 0;
 
-    // queries: largest magnitude per head, then the operand's words
-    const T* q = (const T*)a.q + (int64_t)token * a.q_stride + (int64_t)head0 * HD;
-    if (tid < NH) s_amax[tid] = 0;
-    __syncthreads();
-    for (int h = warp; h < nh; h += DEC_WARPS) {
-        int m = 0;
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) m = max(m, __float_as_int(to_f32(q[h * HD + i * 32 + lane])) & 0x7fffffff);
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0) s_amax[h] = m;
-    }
-    __syncthreads();
-    if (tid < NH) s_factor[tid] = s_amax[tid] >= 0x7f800000 ? __int_as_float(0x7fffffff)
-                                                            : a.scale * kLog2e * q8_pow2(-row_shift(s_amax[tid]));
-    for (int u = tid; u < HD / 16 * NG * 32; u += DEC_WARPS * 32) {
-        const int l = u & 31, ng = (u >> 5) % NG, kk = (u >> 5) / NG;
-        const int h = ng * 8 + (l >> 2), t = l & 3;
-        // dims of the step's k = 2t, 2t + 1 and 2t + 8, 2t + 9: four neighbours of lane t's piece
-        const int d = (kk / KW) * (16 * KW) + t * (4 * KW) + (kk % KW) * 4;
-        __half parts[4][NQ];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float x = 0.f;
-            if (h < nh && s_amax[h] < 0x7f800000) x = to_f32(q[h * HD + d + i]) * q8_pow2(row_shift(s_amax[h]));
-            split<NQ>(x, parts[i]);
-        }
-#pragma unroll
-        for (int j = 0; j < NQ; j++) {
-            const __half2 w0 = __halves2half2(parts[0][j], parts[1][j]), w1 = __halves2half2(parts[2][j], parts[3][j]);
-            sq[((kk * NQ + j) * NG + ng) * 32 + l] = make_uint2(*reinterpret_cast<const uint32_t*>(&w0), *reinterpret_cast<const uint32_t*>(&w1));
-        }
-    }
-    __syncthreads();
-    uint2 qr[Q_IN_REGS ? HD / 16 * NQ * NG : 1];
-    if constexpr (Q_IN_REGS) {
-#pragma unroll
-        for (int i = 0; i < HD / 16 * NQ * NG; i++) qr[i] = sq[i * 32 + lane];
-    }
-    float factor[NG][2], m_ref[NG][2], l_run[NG][2];
-#pragma unroll
-    for (int ng = 0; ng < NG; ng++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            factor[ng][i] = s_factor[ng * 8 + 2 * t4 + i];
-            m_ref[ng][i] = -INFINITY;
-            l_run[ng][i] = 0.f;
-        }
-
     // this warp's tiles: the token's tiles [first, last) in one part per CTA, a part's tiles in turn over the warps
     const int parts = gridDim.x, part = blockIdx.x;
     const int first = lo / DEC_KT, last = (hi + DEC_KT - 1) / DEC_KT;      // tiles start at multiples of their size
@@ -228,44 +233,73 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     const int tile_lo = first + part * per, tile_hi = min(last, tile_lo + per);
 
     const int* table = a.block_table + (int64_t)(req < 0 ? 0 : req) * a.max_blocks;
-    // what a lane knows of key tile * DEC_KT + lane % DEC_KT: its row in the stores (-1: not seen), its scales' exponents
-    auto lookup = [&](int tile, int& row, float& kmul, int& ev) {
-        row = -1; kmul = 0.f; ev = 0;
+    // A lane looks after key tile * DEC_KT + lane % DEC_KT: its page (-1: not seen), read from the table a tile ahead of the
+    // copies that need it, then its row in the stores.
+    auto find = [&](int tile, int& page, int& slot) {
+        page = -1; slot = 0;
         const int key = tile * DEC_KT + (lane & (DEC_KT - 1));
         if (tile >= tile_hi || key < lo || key >= hi) return;
         const int lp = key / a.page_size;
-        if (lp >= a.max_blocks) return;
-        const int page = __ldg(table + lp);
-        if ((unsigned)page >= (unsigned)a.n_pages) return;
-        const int cell = page * a.n_kv + kvh;
-        row = cell * a.page_size + key - lp * a.page_size;
-        kmul = __ldg(a.kscale + cell);
-        ev = q8_exponent(__ldg(a.vscale + cell));
+        slot = key - lp * a.page_size;
+        if (lp < a.max_blocks) page = __ldg(table + lp);
     };
-    uint32_t kr[DEC_MT][2][KC][KW], vr[DEC_MT][4][VW];
-    auto load_k = [&](int row) {
+    const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + Shape::Q_BYTES + warp * DEC_RING;
+    const unsigned meta = ring + DEC_STAGES * 2 * DEC_TILE;
+    // Copies of 16 bytes, COPIES a lane and tile.  Sixteen keys of one page, all seen, lie one behind the other: their
+    // copies differ by constants (765 instructions a tile of 32 keys at head size 128 with a look-up per row, !!! with this).
+    constexpr int COPIES = DEC_KT * PIECES / 32;
+    const bool blocks = a.page_size % 16 == 0;
+    int rows[COPIES];                     // of the tile that is being requested; -1: not seen.  In blocks: the first two, a row each
+    bool whole = false;
+    auto request_blocks = [&](unsigned dst, const uint8_t* store) {
+        const uint8_t* src[DEC_MT];
 #pragma unroll
-        for (int mt = 0; mt < DEC_MT; mt++)
+        for (int b = 0; b < DEC_MT; b++) src[b] = store + (int64_t)rows[b] * HD;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = max(__shfl_sync(0xffffffffu, row, mt * 16 + i * 8 + g8), 0);
-                const uint8_t* src = a.kcache + (int64_t)r * HD + t4 * (4 * KW);
-#pragma unroll
-                for (int c = 0; c < KC; c++) load_words<KW>(src + c * (16 * KW), kr[mt][i][c]);
-            }
+        for (int i = 0; i < COPIES; i++) {
+            const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
+            const int b = DEC_MT == 2 ? (COPIES % 2 == 0 ? i / (COPIES / 2) : key >> 4) : 0;
+            copy16(dst + key * HD + ((piece ^ dec_swizzle(key)) << 4), (b ? src[DEC_MT - 1] : src[0]) + (u * 16 - b * 16 * HD), true);
+        }
     };
-    auto load_v = [&](int row) {
+    auto request_k = [&](int stage, int meta_slot, int page, int slot) {
+        const bool there = (unsigned)page < (unsigned)a.n_pages;
+        const int cell = there ? page * a.n_kv + kvh : 0;
+        const int row = there ? cell * a.page_size + slot : -1;
+        if (lane < DEC_KT) {
+            copy4(meta + meta_slot * DEC_META + lane * 8, a.kscale + cell, there);
+            copy4(meta + meta_slot * DEC_META + lane * 8 + 4, a.vscale + cell, there);
+        }
+        whole = blocks && __all_sync(0xffffffffu, there);
+        if (whole) {
+            rows[0] = __shfl_sync(0xffffffffu, row, 0);
+            if constexpr (DEC_MT == 2) rows[1] = __shfl_sync(0xffffffffu, row, 16);
+            request_blocks(ring + stage * 2 * DEC_TILE, a.kcache);
+            copies_commit();
+            return;
+        }
 #pragma unroll
-        for (int mt = 0; mt < DEC_MT; mt++)
+        for (int i = 0; i < COPIES; i++) {
+            const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
+            rows[i] = __shfl_sync(0xffffffffu, row, key);
+            copy16(ring + stage * 2 * DEC_TILE + key * HD + ((piece ^ dec_swizzle(key)) << 4),
+                   a.kcache + (int64_t)max(rows[i], 0) * HD + piece * 16, rows[i] >= 0);
+        }
+        copies_commit();
+    };
+    auto request_v = [&](int stage) {
+        if (whole) {
+            request_blocks(ring + stage * 2 * DEC_TILE + DEC_TILE, a.vcache);
+            copies_commit();
+            return;
+        }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = __shfl_sync(0xffffffffu, row, mt * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1));
-                load_words<VW>(a.vcache + (int64_t)max(r, 0) * HD + g8 * (HD / 8), vr[mt][i]);
-                if (r < 0) {                         // what is not seen may hold anything, NaN too
-#pragma unroll
-                    for (int w = 0; w < VW; w++) vr[mt][i][w] = 0;
-                }
-            }
+        for (int i = 0; i < COPIES; i++) {
+            const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
+            copy16(ring + stage * 2 * DEC_TILE + DEC_TILE + key * HD + ((piece ^ dec_swizzle(key)) << 4),
+                   a.vcache + (int64_t)max(rows[i], 0) * HD + piece * 16, rows[i] >= 0);
+        }
+        copies_commit();
     };
     float o[HD / 16][NG][4];
 #pragma unroll
@@ -275,14 +309,66 @@ attn_decode_q8_kernel(const DecodeArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) o[i][ng][j] = 0.f;
 
-    int row, row_next, ev, ev_next;
-    float kmul, kmul_next;
-    int tile = tile_lo + warp;
-    lookup(tile, row, kmul, ev);
-    if (tile < tile_hi) { load_k(row); load_v(row); }
-    for (; tile < tile_hi; tile += DEC_WARPS) {
-        const bool more = tile + DEC_WARPS < tile_hi;
-        lookup(tile + DEC_WARPS, row_next, kmul_next, ev_next);
+    int page[DEC_STAGES + 1], slot[DEC_STAGES + 1];
+#pragma unroll
+    for (int i = 0; i <= DEC_STAGES; i++) find(tile_lo + warp + i * DEC_WARPS, page[i], slot[i]);
+#pragma unroll
+    for (int i = 0; i < DEC_STAGES; i++) {
+        request_k(i, i, page[i], slot[i]);
+        request_v(i);
+    }
+    // Queries, while the first tiles are on their way: lane (g, t) holds its dims of head g, four lanes a head.  What does not
+    // fit the registers (the parts of float32 queries) goes through shared memory, a quarter by each warp.
+    const T* q = (const T*)a.q + (int64_t)token * a.q_stride + (int64_t)head0 * HD;
+    uint2 qr[Q_IN_REGS ? HD / 16 * NQ * NG : 1];
+    float factor[NG][2], m_ref[NG][2], l_run[NG][2];
+#pragma unroll
+    for (int ng = 0; ng < NG; ng++) {
+        const int h = ng * 8 + g8;
+        float x[HD / 16][4];
+        int m = 0;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++) {
+            // dims of the step's k = 2t, 2t + 1 and 2t + 8, 2t + 9: four neighbours of lane t's piece
+            load4(q + h * HD + (kk / KW) * (16 * KW) + t4 * (4 * KW) + (kk % KW) * 4, h < nh, a.q_by_four, x[kk]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) m = max(m, __float_as_int(x[kk][i]) & 0x7fffffff);
+        }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const bool finite = m < 0x7f800000;
+        const float up = finite ? q8_pow2(row_shift(m)) : 0.f;
+        const float f = finite ? a.scale * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);   // NaN: the row is
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            factor[ng][i] = __shfl_sync(0xffffffffu, f, (2 * t4 + i) * 4);
+            m_ref[ng][i] = -INFINITY;
+            l_run[ng][i] = 0.f;
+        }
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++) {
+            __half parts[4][NQ];
+#pragma unroll
+            for (int i = 0; i < 4; i++) split<NQ>(finite ? x[kk][i] * up : 0.f, parts[i]);
+#pragma unroll
+            for (int j = 0; j < NQ; j++) {
+                const __half2 w0 = __halves2half2(parts[0][j], parts[1][j]), w1 = __halves2half2(parts[2][j], parts[3][j]);
+                const uint2 w = make_uint2(*reinterpret_cast<const uint32_t*>(&w0), *reinterpret_cast<const uint32_t*>(&w1));
+                const int at = (kk * NQ + j) * NG + ng;
+                if constexpr (Q_IN_REGS) qr[at] = w;
+                else if (kk % DEC_WARPS == warp) sq[at * 32 + lane] = w;
+            }
+        }
+    }
+    if constexpr (!Q_IN_REGS) __syncthreads();
+    int page_next = page[DEC_STAGES], slot_next = slot[DEC_STAGES];   // of the tile that is requested next
+    int stage = 0, meta_slot = 0;
+    for (int tile = tile_lo + warp; tile < tile_hi; tile += DEC_WARPS) {
+        const int page_now = page_next, slot_now = slot_next;
+        find(tile + (DEC_STAGES + 1) * DEC_WARPS, page_next, slot_next);
+        copies_wait<2 * DEC_STAGES - 1>();                            // this tile's keys and scales
+        __syncwarp();
+        const unsigned k_at = ring + stage * 2 * DEC_TILE, v_at = k_at + DEC_TILE;
         float s[DEC_MT][NG][4];
 #pragma unroll
         for (int mt = 0; mt < DEC_MT; mt++)
@@ -291,10 +377,25 @@ attn_decode_q8_kernel(const DecodeArgs a) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) s[mt][ng][j] = 0.f;
 #pragma unroll
-        for (int c = 0; c < KC; c++)
+        for (int c = 0; c < KC; c++) {
+            uint32_t kr[DEC_MT][2][KW];
+#pragma unroll
+            for (int mt = 0; mt < DEC_MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int key = mt * 16 + i * 8 + dec_key(g8);
+                    const int piece = KW == 4 ? c * 4 + t4 : c * 2 + (t4 >> 1);
+                    read_words<KW>(k_at + key * HD + ((piece ^ dec_swizzle(key)) << 4) + (KW == 4 ? 0 : (t4 & 1) * 8), kr[mt][i]);
+                }
 #pragma unroll
             for (int w = 0; w < KW; w++) {
                 const int kk = c * KW + w;
+                uint32_t ka[DEC_MT][4];
+#pragma unroll
+                for (int mt = 0; mt < DEC_MT; mt++) {
+                    q8_to_f16x4(kr[mt][0][w], ka[mt][0], ka[mt][2]);
+                    q8_to_f16x4(kr[mt][1][w], ka[mt][1], ka[mt][3]);
+                }
 #pragma unroll
                 for (int j = NQ - 1; j >= 0; j--)                   // the smallest part first
 #pragma unroll
@@ -302,30 +403,30 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                         const int at = (kk * NQ + j) * NG + ng;
                         const uint2 b = Q_IN_REGS ? qr[Q_IN_REGS ? at : 0] : sq[at * 32 + lane];
 #pragma unroll
-                        for (int mt = 0; mt < DEC_MT; mt++)
-                            mma16816(s[mt][ng], q8_to_f16x2(kr[mt][0][c][w] & 0xffffu), q8_to_f16x2(kr[mt][1][c][w] & 0xffffu),
-                                     q8_to_f16x2(kr[mt][0][c][w] >> 16), q8_to_f16x2(kr[mt][1][c][w] >> 16), b.x, b.y);
+                        for (int mt = 0; mt < DEC_MT; mt++) mma16816(s[mt][ng], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
                     }
             }
-        if (more) load_k(row_next);
+        }
+        __syncwarp();                                                 // everybody has read this tile's keys
+        request_k(stage, meta_slot == 0 ? DEC_STAGES : meta_slot - 1, page_now, slot_now);
         // scores, in units of log2, with the values' exponents
         bool grown = false;
-        float inv[DEC_MT][2];                       // 2^-ev of the lane's keys g8 and g8 + 8
+        float inv[DEC_MT][2];                       // 2^-ev of the lane's keys
 #pragma unroll
         for (int mt = 0; mt < DEC_MT; mt++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int src = mt * 16 + i * 8 + g8;
-                const int r = __shfl_sync(0xffffffffu, row, src);
-                const float km = __shfl_sync(0xffffffffu, kmul, src);
-                const int e = __shfl_sync(0xffffffffu, ev, src);
+                float scales[2];                    // of the key's page; zeros: not seen
+                read_words<2>(meta + meta_slot * DEC_META + (mt * 16 + i * 8 + dec_key(g8)) * 8, reinterpret_cast<uint32_t*>(scales));
+                const int e = q8_exponent(scales[1]);
+                const bool seen = scales[1] != 0.f;
                 inv[mt][i] = q8_pow2(-e);
 #pragma unroll
                 for (int ng = 0; ng < NG; ng++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         float& x = s[mt][ng][2 * i + j];
-                        x = r < 0 ? -INFINITY : fmaf(x * km, factor[ng][j], (float)e);
+                        x = seen ? fmaf(x * scales[0], factor[ng][j], (float)e) : -INFINITY;
                         grown = grown || x > m_ref[ng][j] + kMoveAt;
                     }
             }
@@ -374,24 +475,47 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                         pb[mt][k][ng][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hh));
                     }
                 }
+        copies_wait<2 * DEC_STAGES - 1>();                            // this tile's values
+        __syncwarp();
 #pragma unroll
-        for (int mt = 0; mt < DEC_MT; mt++)
+        for (int mt = 0; mt < DEC_MT; mt++) {
+            uint32_t vr[4][VW];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int key = mt * 16 + (i >> 1) * 8 + dec_key(2 * t4 + (i & 1)), f = dec_swizzle(key);
+                const unsigned at = v_at + key * HD;
+                if constexpr (HD == 64) {
+                    read_words<2>(at + (((g8 >> 1) ^ f) << 4) + (g8 & 1) * 8, vr[i]);
+                } else if constexpr (HD % 128 == 0) {
+#pragma unroll
+                    for (int w = 0; w < VW; w += 4) read_words<4>(at + ((g8 * (VW / 4) + w / 4) ^ f) * 16, vr[i] + w);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < VW; w++) read_words<1>(at + g8 * (HD / 8) + w * 4, vr[i] + w);
+                }
+            }
 #pragma unroll
             for (int w = 0; w < VW; w++)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {              // dims 4w, 4w + 1, then 4w + 2, 4w + 3
                     const unsigned sel = half ? 0x7362u : 0x5140u;
-                    const uint32_t x = __byte_perm(vr[mt][0][w], vr[mt][1][w], sel), y = __byte_perm(vr[mt][2][w], vr[mt][3][w], sel);
-                    const uint32_t a0 = q8_to_f16x2(x & 0xffffu), a1 = q8_to_f16x2(x >> 16);
-                    const uint32_t a2 = q8_to_f16x2(y & 0xffffu), a3 = q8_to_f16x2(y >> 16);
+                    const uint32_t x = __byte_perm(vr[0][w], vr[1][w], sel), y = __byte_perm(vr[2][w], vr[3][w], sel);
+                    uint32_t a0, a1, a2, a3;
+                    q8_to_f16x4(x, a0, a1);
+                    q8_to_f16x4(y, a2, a3);
 #pragma unroll
                     for (int k = NP - 1; k >= 0; k--)
 #pragma unroll
                         for (int ng = 0; ng < NG; ng++) mma16816(o[2 * w + half][ng], a0, a1, a2, a3, pb[mt][k][ng][0], pb[mt][k][ng][1]);
                 }
-        if (more) load_v(row_next);
-        row = row_next; kmul = kmul_next; ev = ev_next;
+        }
+        __syncwarp();                                                 // everybody has read this tile's values
+        request_v(stage);
+        stage = stage + 1 == DEC_STAGES ? 0 : stage + 1;
+        meta_slot = meta_slot == DEC_STAGES ? 0 : meta_slot + 1;
     }
+    copies_wait<0>();
+    __syncthreads();                                                  // the rings become the room for the sums
 
     // join: the warps of the CTA in order, then the CTAs of the cluster in order
 #pragma unroll
@@ -410,49 +534,59 @@ attn_decode_q8_kernel(const DecodeArgs a) {
             }
         }
     __syncthreads();
-    for (int u = tid; u < nh * HD; u += DEC_WARPS * 32) {
-        const int h = u / HD, d = u - h * HD;
+    for (int u = tid; u < nh * (HD / 4); u += DEC_WARPS * 32) {
+        const int h = u / (HD / 4), d = (u - h * (HD / 4)) * 4;
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < DEC_WARPS; w++) m = fmaxf(m, s_ml[w][h][0]);
-        float l = 0.f, x = 0.f;
+        float l = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < DEC_WARPS; w++) {
-            const float f = s_ml[w][h][0] == -INFINITY ? (s_ml[w][h][1] == 0.f ? 0.f : 1.f) : exp2f(s_ml[w][h][0] - m);
+            const float f = part_factor(s_ml[w][h][0], s_ml[w][h][1], m);
             l += f * s_ml[w][h][1];
-            x += f * so[(w * NH + h) * HD + d];
+            add_scaled(x, f, *reinterpret_cast<const float4*>(so + (w * NH + h) * HD + d));
         }
-        so[h * HD + d] = x;              // warp 0's place of this very number: nobody else reads it
+        *reinterpret_cast<float4*>(so + h * HD + d) = x;      // warp 0's place of these very numbers: nobody else reads it
         if (d == 0) { s_cta[h][0] = m; s_cta[h][1] = l; }
     }
     const unsigned C = cluster_size(), rank = cluster_rank();
     if (C > 1) cluster_sync(); else __syncthreads();
     const int range = blockIdx.x / C;
-    for (int u = rank * DEC_WARPS * 32 + tid; u < nh * HD; u += C * DEC_WARPS * 32) {
-        const int h = u / HD, d = u - h * HD;
-        float m, l, x;
+    for (int u = rank * DEC_WARPS * 32 + tid; u < nh * (HD / 4); u += C * DEC_WARPS * 32) {
+        const int h = u / (HD / 4), d = (u - h * (HD / 4)) * 4;
+        float m = -INFINITY, l = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         if (C == 1) {
-            m = s_cta[h][0]; l = s_cta[h][1]; x = so[u];
+            m = s_cta[h][0]; l = s_cta[h][1];
+            x = *reinterpret_cast<const float4*>(so + h * HD + d);
         } else {
-            m = -INFINITY;
-            for (unsigned c = 0; c < C; c++) m = fmaxf(m, peer_load(&s_cta[h][0], c));
-            l = 0.f; x = 0.f;
-            for (unsigned c = 0; c < C; c++) {
-                const float mc = peer_load(&s_cta[h][0], c), lc = peer_load(&s_cta[h][1], c);
-                const float f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : exp2f(mc - m);
-                l += f * lc;
-                x += f * peer_load(so + u, c);
+            float2 ml[8];
+            float4 px[8];
+#pragma unroll
+            for (unsigned c = 0; c < 8; c++) {
+                ml[c] = make_float2(-INFINITY, 0.f);
+                px[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c < C) {
+                    ml[c] = peer_load2(&s_cta[h][0], c);
+                    px[c] = peer_load4(so + h * HD + d, c);
+                }
+            }
+#pragma unroll
+            for (unsigned c = 0; c < 8; c++) m = fmaxf(m, ml[c].x);
+#pragma unroll
+            for (unsigned c = 0; c < 8; c++) {
+                const float f = part_factor(ml[c].x, ml[c].y, m);
+                l += f * ml[c].y;
+                add_scaled(x, f, px[c]);
             }
         }
         const int64_t at = (int64_t)token * a.n_heads + head0 + h;
         if (a.ranges == 1) {
-            reinterpret_cast<T*>(a.out)[at * HD + d] = from_f32<T>(l == 0.f ? 0.f : x / l);
+            store_row4(reinterpret_cast<T*>(a.out) + at * HD + d, x, l);
         } else {
-            a.part_o[(at * a.ranges + range) * HD + d] = x;
-            if (d == 0) {
-                a.part_ml[(at * a.ranges + range) * 2] = m;
-                a.part_ml[(at * a.ranges + range) * 2 + 1] = l;
-            }
+            *reinterpret_cast<float4*>(a.part_o + (at * a.ranges + range) * HD + d) = x;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.ranges + range) * 2) = make_float2(m, l);
         }
     }
     if (C > 1) cluster_sync();           // nobody leaves while another still reads its shared memory
@@ -460,31 +594,45 @@ attn_decode_q8_kernel(const DecodeArgs a) {
 
 // joins the ranges of a (token, head) in order
 template <typename T>
-__global__ void __launch_bounds__(HD) attn_decode_q8_join_kernel(T* __restrict__ out, const float* __restrict__ part_o,
-                                                                 const float* __restrict__ part_ml, int ranges) {
+__global__ void __launch_bounds__(HD / 4) attn_decode_q8_join_kernel(T* __restrict__ out, const float* __restrict__ part_o,
+                                                                     const float* __restrict__ part_ml, int ranges) {
     griddep_wait();
     griddep_launch();
     const int64_t at = blockIdx.x;
-    const int d = threadIdx.x;
+    const int d = threadIdx.x * 4;
+    const float2* ml = reinterpret_cast<const float2*>(part_ml) + at * ranges;
     float m = -INFINITY;
-    for (int r = 0; r < ranges; r++) m = fmaxf(m, part_ml[(at * ranges + r) * 2]);
-    float l = 0.f, x = 0.f;
+    for (int r = 0; r < ranges; r++) m = fmaxf(m, ml[r].x);
+    float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int r = 0; r < ranges; r++) {
-        const float mr = part_ml[(at * ranges + r) * 2], lr = part_ml[(at * ranges + r) * 2 + 1];
-        const float f = mr == -INFINITY ? (lr == 0.f ? 0.f : 1.f) : exp2f(mr - m);
-        l += f * lr;
-        x += f * part_o[(at * ranges + r) * HD + d];
+        const float f = part_factor(ml[r].x, ml[r].y, m);
+        l += f * ml[r].y;
+        add_scaled(x, f, *reinterpret_cast<const float4*>(part_o + (at * ranges + r) * HD + d));
     }
-    out[at * HD + d] = from_f32<T>(l == 0.f ? 0.f : x / l);
+    store_row4(out + at * HD + d, x, l);
+}
+
+// Once per device: more than 48 KB of dynamic shared memory for a kernel.
+cudaError_t open_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& opened) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (opened.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) opened.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 template <typename T, int NG>
 int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)HD / 16 * Parts<T>::Q * NG * 32 * 8 + (size_t)DEC_WARPS * 8 * NG * HD * 4;
+    constexpr size_t smem = DecodeShape<T, NG>::SMEM;
     static_assert(smem <= 227 * 1024, "shared memory");
     auto kernel = attn_decode_q8_kernel<T, NG>;
-    cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> opened{0};                           // devices on which the kernel may have its shared memory
+    cudaError_t e = smem > 48 * 1024 ? open_shared_memory((const void*)kernel, (int)smem, opened) : cudaSuccess;
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(a.ranges * cluster, a.n_kv * a.subs, n_tokens);
@@ -507,7 +655,7 @@ int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t s
         return (int)e;
     }
     if (a.ranges > 1) {
-        kllm_launch((attn_decode_q8_join_kernel<T>), dim3(n_tokens * a.n_heads), dim3(HD), 0, stream, (T*)a.out, (const float*)a.part_o,
+        kllm_launch((attn_decode_q8_join_kernel<T>), dim3(n_tokens * a.n_heads), dim3(HD / 4), 0, stream, (T*)a.out, (const float*)a.part_o,
                     (const float*)a.part_ml, a.ranges);
     }
     KLLM_LAUNCH_STATUS();
@@ -548,10 +696,9 @@ struct PrefillArgs {
 template <typename T>
 __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const PrefillArgs a) {
     constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P;
-    constexpr int PIECES = HD / 16;                       // 16-byte pieces of a stored row
     constexpr int LOADS = PRE_KEYS * PIECES / PRE_THREADS;   // pieces of K (and of V) a thread carries
     static_assert(PRE_KEYS * PIECES % PRE_THREADS == 0, "pieces per thread");
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     __half* sq = reinterpret_cast<__half*>(smem);                     // [NQ][rows][PRE_LD]
     __half* sk = sq + NQ * PRE_ROWS * PRE_LD;                         // [keys][PRE_LD]
     __half* sv = sk + PRE_KEYS * PRE_LD;
@@ -795,7 +942,8 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
 template <typename T> int launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
     constexpr size_t smem = (size_t)(Parts<T>::Q * PRE_ROWS + 2 * PRE_KEYS) * PRE_LD * 2;
     static_assert(smem <= 226 * 1024, "shared memory");
-    const cudaError_t e = cudaFuncSetAttribute(attn_prefill_q8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> opened{0};
+    const cudaError_t e = open_shared_memory((const void*)attn_prefill_q8_kernel<T>, (int)smem, opened);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         snprintf(g_kllm_err, sizeof(g_kllm_err), "attention (8 bits): %zu bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
@@ -814,8 +962,8 @@ int check_common(int n_heads, int n_kv, int hd, int page_size, int n_pages, int 
     if (n_pages <= 0) KLLM_FAIL("attention (8 bits): a cache of %d pages", n_pages);
     if ((int64_t)n_pages * n_kv * page_size >= (1LL << 31)) KLLM_FAIL("attention (8 bits): a store of 2^31 rows or more");
     if (dtype != KLLM_F32 && dtype != KLLM_BF16) KLLM_FAIL("attention (8 bits): element type %d", dtype);
-    if ((((uintptr_t)kcache | (uintptr_t)vcache) & 15) || ((uintptr_t)out & 7))
-        KLLM_FAIL("attention (8 bits): the caches must be 16-byte aligned, out 8-byte");
+    if ((((uintptr_t)kcache | (uintptr_t)vcache) & 15) || ((uintptr_t)out & (dtype == KLLM_F32 ? 15 : 7)))
+        KLLM_FAIL("attention (8 bits): the caches must be 16-byte aligned, out to four of its numbers");
     return 0;
 }
 
@@ -845,7 +993,8 @@ extern "C" int kllm_attention_decode_q8(void* out, float* part_o, float* part_ml
     if ((int64_t)n_kv * subs > 65535) KLLM_FAIL("attention (8 bits): %d kv heads in %d parts each", n_kv, subs);
     DecodeArgs a{out, part_o, part_ml, q, q_stride, (const uint8_t*)kcache, (const uint8_t*)vcache, kscale, vscale, positions,
                  token_req, block_table, max_blocks, n_pages, n_requests, n_heads, n_kv, subs, gs / subs, page_size,
-                 window > 0 ? window : 0, ranges, scale};
+                 window > 0 ? window : 0, ranges,
+                 !(q_stride & 3) && !((uintptr_t)q & (dtype == KLLM_F32 ? 15 : 7)), scale};
     const cudaStream_t s = (cudaStream_t)stream;
     if constexpr (HD <= 128) {
         if (a.heads_per_cta > 8)

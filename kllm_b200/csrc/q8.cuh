@@ -40,6 +40,11 @@ __device__ __forceinline__ uint32_t q8_to_f16x2(uint32_t two) {
     asm("{\n.reg .b16 l;\ncvt.u16.u32 l, %1;\ncvt.rn.f16x2.e4m3x2 %0, l;\n}\n" : "=r"(r) : "r"(two));
     return r;
 }
+// four e4m3 numbers as two pairs of float16
+__device__ __forceinline__ void q8_to_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+        : "=r"(lo), "=r"(hi) : "r"(four));
+}
 // the nearest e4m3 numbers, ties to even; beyond +-448 they stay at it, NaN is NaN
 __device__ __forceinline__ uint32_t q8_pack2(float lo, float hi) {
     unsigned short r;
