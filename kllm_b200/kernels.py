@@ -1112,17 +1112,33 @@ def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     _check(lib, "cache_q8", rc)
 
 
-def decode_q8_parts(n_tokens: int, n_kv: int, group: int, head_dim: int, ctx_bound: int) -> tuple:
-    """(ranges, CTAs of a cluster) into which a token's context of up to ``ctx_bound`` keys is cut."""
+def decode_q8_parts(n_tokens: int, n_kv: int, group: int, head_dim: int, ctx_bound: int, wide: bool = False) -> tuple:
+    """(ranges, CTAs of a cluster) into which a token's context of up to ``ctx_bound`` keys is cut; ``wide``: float32 queries.
+
+    With P parts a CTA's chain of tiles is 1 / P as long, and the SMs start and join P times as many CTAs.  Measured, a CTA's
+    128 keys take 0.68 us at head size 64, 0.78 at 128 (float32 about twice that) while bandwidth is not the limit, a further
+    CTA on an SM costs 1.4 (2.7) us: the sum is least at P^2 = 0.49 (0.29) * blocks of 128 keys * SMs / pairs of token and kv
+    head.  Microseconds by parts: 16 x 4 pairs of size 64 at 2048 keys 1: 15.3, 2: 10.9, 4: 9.7, 8: 10.8; 64 x 4 1: 19.7,
+    2: 20.1, 4: 25.7; 8 x 8 of size 128 at 2048 1: 19.6, 2: 13.4, 4: 14.7; 64 x 8 at 1280 1: 41.7, 2: 44.2, 8: 102.  More than
+    one wave of CTAs never pays (2 x 32 of size 128 at 16384, bandwidth bound, 4: 58, 8: 65).
+
+    Up to eight parts are one cluster, which joins through distributed shared memory (1.5 us).  More parts are several ranges
+    of such clusters, joined by a second kernel (2 us more): 1 x 4 of size 64 at 2048 8: 6.3, 16: 7.4; 1 x 8 of size 128 at
+    131072 8: 109, 48: 53."""
     most = 16 if head_dim <= 128 else 8
     subs = next(s for s in range(1, group + 1) if group % s == 0 and group // s <= most)
     base = max(1, n_tokens * n_kv * subs)
     blocks = max(1, -(-ctx_bound // 128))
-    want = max(1, min(blocks, 3 * sm_count() // base))
+    sms = sm_count()
+    wave = sms * (4 if head_dim <= 64 else 3 if head_dim <= 128 else 2) // base
+    square = (0.49 if head_dim <= 64 else 0.29) * (2 if wide else 1) * blocks * sms / base
     cluster = 1
-    while cluster < 8 and cluster * 2 <= want:
+    while cluster < 8 and 4 * cluster * cluster <= square and 2 * cluster <= min(blocks, wave):
         cluster *= 2
-    return max(1, want // cluster) if cluster == 8 else 1, cluster
+    ranges = 1
+    if cluster == 8 and square >= 24 * 24:
+        ranges = max(1, min(int(square ** 0.5) // 8, wave // 8, blocks // 32))
+    return ranges, cluster
 
 
 def _check_q8_rows(what, out, q, n_heads, head_dim):
@@ -1149,7 +1165,7 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
         raise KernelError("attention_decode_q8: a position (and a request) per token")
     _cuda(out, q, kcache, vcache, kscale, vscale, positions, token_req, block_table)
     bound = min(int(ctx_bound), int(window)) if window and window > 0 else int(ctx_bound)
-    ranges, cluster = decode_q8_parts(n, n_kv, n_heads // n_kv, head_dim, bound)
+    ranges, cluster = decode_q8_parts(n, n_kv, n_heads // n_kv, head_dim, bound, q.dtype == torch.float32)
     part_o = part_ml = None
     if ranges > 1:
         part_o = torch.empty((n, n_heads, ranges, head_dim), dtype=torch.float32, device=q.device)
