@@ -19,8 +19,6 @@
 // key becomes zeros.
 #include "q8.cuh"
 
-#include <atomic>
-
 #ifndef KLLM_HD
 #error "compile with -DKLLM_HD=<head size, a multiple of 32 up to 256>"
 #endif
@@ -31,10 +29,6 @@ namespace {
 
 constexpr int HD = KLLM_HD;
 static_assert(HD % 32 == 0 && HD >= 32 && HD <= 256, "head sizes: multiples of 32 up to 256");
-constexpr float kMoveAt = 8.f;              // the reference moves when the maximum has grown by 2^8
-constexpr float kLift = 7.f;                // weights are carried 2^7 up: float16's range below 1
-constexpr float kLog2e = 1.4426950408889634f;
-
 template <typename T> struct Parts { static constexpr int Q = 1, P = 1; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 2; };
 
@@ -48,17 +42,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
 }
-// 2^x, the hardware approximation: 2^-22 off at most, far below half a step of what the weight is rounded to or summed with
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// The power of two that brings a row's largest magnitude m (its bits) to 2^14 <= m < 2^15, as an exponent; the other way
-// round it is in the row's factor.  Rows of zeros and of tiny numbers stop at 2^100.
-__device__ __forceinline__ int row_shift(int bits) { return min(14 + 127 - (bits >> 23), 100); }
-
 // part i of x: x = p0 + p1 + p2 + ..., each a float16 number
 template <int N> __device__ __forceinline__ void split(float x, __half (&p)[N]) {
 #pragma unroll
@@ -185,25 +168,6 @@ __device__ __forceinline__ float4 peer_load4(const void* p, unsigned rank) {
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_addr(p, rank)));
     return v;
 }
-// What a part with reference m and sum l counts beside the reference of all parts.  A part without a seen key has -inf and 0;
-// one that met only NaN has -inf and NaN, which stays.
-__device__ __forceinline__ float part_factor(float m, float l, float all) {
-    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - all);
-}
-__device__ __forceinline__ void add_scaled(float4& x, float f, const float4& y) {
-    x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
-}
-// x / l, zeros where no key was seen
-template <typename T> __device__ __forceinline__ void store_row4(T* dst, const float4& x, float l) {
-    const float4 y = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x / l, x.y / l, x.z / l, x.w / l);
-    if constexpr (sizeof(T) == 2) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    } else {
-        *reinterpret_cast<float4*>(dst) = y;
-    }
-}
-
 // grid: (ranges * cluster, kv heads * subgroups of heads, tokens), clusters along x; a cluster's CTAs take neighbouring
 // parts of a range and join through distributed shared memory
 template <typename T, int NG>
@@ -592,40 +556,6 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     if (C > 1) cluster_sync();           // nobody leaves while another still reads its shared memory
 }
 
-// joins the ranges of a (token, head) in order
-template <typename T>
-__global__ void __launch_bounds__(HD / 4) attn_decode_q8_join_kernel(T* __restrict__ out, const float* __restrict__ part_o,
-                                                                     const float* __restrict__ part_ml, int ranges) {
-    griddep_wait();
-    griddep_launch();
-    const int64_t at = blockIdx.x;
-    const int d = threadIdx.x * 4;
-    const float2* ml = reinterpret_cast<const float2*>(part_ml) + at * ranges;
-    float m = -INFINITY;
-    for (int r = 0; r < ranges; r++) m = fmaxf(m, ml[r].x);
-    float l = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int r = 0; r < ranges; r++) {
-        const float f = part_factor(ml[r].x, ml[r].y, m);
-        l += f * ml[r].y;
-        add_scaled(x, f, *reinterpret_cast<const float4*>(part_o + (at * ranges + r) * HD + d));
-    }
-    store_row4(out + at * HD + d, x, l);
-}
-
-// Once per device: more than 48 KB of dynamic shared memory for a kernel.
-cudaError_t open_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& opened) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (opened.load(std::memory_order_acquire) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) opened.fetch_or(bit, std::memory_order_release);
-    return e;
-}
-
 template <typename T, int NG>
 int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t stream) {
     constexpr size_t smem = DecodeShape<T, NG>::SMEM;
@@ -655,8 +585,8 @@ int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t s
         return (int)e;
     }
     if (a.ranges > 1) {
-        kllm_launch((attn_decode_q8_join_kernel<T>), dim3(n_tokens * a.n_heads), dim3(HD / 4), 0, stream, (T*)a.out, (const float*)a.part_o,
-                    (const float*)a.part_ml, a.ranges);
+        kllm_launch((q8_join_kernel<T, HD>), dim3(n_tokens * a.n_heads), dim3(HD / 4), 0, stream, (T*)a.out, (const float*)a.part_o,
+                    (const float*)a.part_ml, a.ranges, a.n_heads, (const int*)nullptr, 0);
     }
     KLLM_LAUNCH_STATUS();
 }

@@ -248,6 +248,7 @@ VARIANTS = {"skinny_gemm": [None, {"KLLM_BIAS": 1}], "skinny_gemm_f32": [None, {
             "attention_tc": [{"KLLM_HD": hd} for hd in list(range(16, 129, 16)) + [160, 192, 224, 256]]
             + [{"KLLM_HD": hd, "KLLM_VD": vd} for hd, vd in ((32, 64), (64, 128), (128, 64), (128, 256))],
             "attention_q8": [{"KLLM_HD": hd} for hd in range(32, 257, 32)],
+            "attention_q8_tcgen05": [{"KLLM_HD": hd} for hd in (64, 128)],
             "attention_tcgen05": [{"KLLM_HD": hd} for hd in (64, 128)],
             "attention_tcgen05_ptmem": [{"KLLM_HD": hd} for hd in (64, 128)]}
 

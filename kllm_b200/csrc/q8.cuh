@@ -17,6 +17,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace {
 
 constexpr int Q8_E_MIN = -48, Q8_E_MAX = 48;
@@ -55,6 +57,82 @@ __device__ __forceinline__ uint32_t q8_pack2(float lo, float hi) {
 __device__ __forceinline__ uint32_t q8_half2(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// ---- what the attention kernels share ----
+
+constexpr float kMoveAt = 8.f;              // the reference moves when the maximum has grown by 2^8
+constexpr float kLift = 7.f;                // weights are carried 2^7 up: float16's range below 1
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^x, the hardware approximation: 2^-22 off at most, far below half a step of what the weight is rounded to or summed with
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The power of two that brings a row's largest magnitude m (its bits) to 2^14 <= m < 2^15, as an exponent; the other way
+// round it is in the row's factor.  Rows of zeros and of tiny numbers stop at 2^100.
+__device__ __forceinline__ int row_shift(int bits) { return min(14 + 127 - (bits >> 23), 100); }
+
+// What a part with reference m and sum l counts beside the reference of all parts.  A part without a seen key has -inf and 0;
+// one that met only NaN has -inf and NaN, which stays.
+__device__ __forceinline__ float part_factor(float m, float l, float all) {
+    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - all);
+}
+__device__ __forceinline__ void add_scaled(float4& x, float f, const float4& y) {
+    x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+}
+// x / l, zeros where no key was seen
+template <typename T> __device__ __forceinline__ void store_row4(T* dst, const float4& x, float l) {
+    const float4 y = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x / l, x.y / l, x.z / l, x.w / l);
+    if constexpr (sizeof(T) == 2) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+        *reinterpret_cast<float4*>(dst) = y;
+    }
+}
+
+// joins the ranges of a (token, head) in order
+// (rows of tokens outside [q_start[0], q_start[n_requests]) are left alone; q_start NULL: all are joined)
+template <typename T, int HD>
+__global__ void __launch_bounds__(HD / 4) q8_join_kernel(T* __restrict__ out, const float* __restrict__ part_o,
+                                                         const float* __restrict__ part_ml, int ranges, int n_heads,
+                                                         const int* __restrict__ q_start, int n_requests) {
+    griddep_wait();
+    griddep_launch();
+    const int64_t at = blockIdx.x;
+    if (q_start) {
+        const int token = blockIdx.x / n_heads;
+        if (token < q_start[0] || token >= q_start[n_requests]) return;
+    }
+    const int d = threadIdx.x * 4;
+    const float2* ml = reinterpret_cast<const float2*>(part_ml) + at * ranges;
+    float m = -INFINITY;
+    for (int r = 0; r < ranges; r++) m = fmaxf(m, ml[r].x);
+    float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int r = 0; r < ranges; r++) {
+        const float f = part_factor(ml[r].x, ml[r].y, m);
+        l += f * ml[r].y;
+        add_scaled(x, f, *reinterpret_cast<const float4*>(part_o + (at * ranges + r) * HD + d));
+    }
+    store_row4(out + at * HD + d, x, l);
+}
+
+// Once per device: more than 48 KB of dynamic shared memory for a kernel.
+[[maybe_unused]] cudaError_t open_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& opened) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (opened.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) opened.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 }  // namespace

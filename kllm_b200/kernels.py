@@ -1181,6 +1181,15 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
         launches += 1       # the kernel that joins the ranges
 
 
+def prefill_q8_parts(n_tokens: int, n_requests: int, n_kv: int, group: int, ctx_bound: int) -> tuple:
+    """(row tiles of a CTA, parts of the keys) of the tcgen05 form of ``attention_prefill_q8``."""
+    sms = sm_count()
+    per_tile = 128 // group
+    ctas = (n_tokens // (2 * per_tile) + n_requests) * n_kv
+    splits = max(1, min(sms // ctas, -(-int(ctx_bound) // 128) // 4))
+    return 2, splits
+
+
 def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
                          vscale: torch.Tensor, q_start: torch.Tensor, start_pos: torch.Tensor, block_table: torch.Tensor,
                          n_requests: int, n_heads: int, n_kv: int, head_dim: int, window: int, scale: float,
@@ -1195,6 +1204,24 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
     if R < 0 or q_start.numel() < R + 1 or start_pos.numel() < R or block_table.shape[0] < R:
         raise KernelError("attention_prefill_q8: q_start, start_pos and the block table must cover the requests")
     _cuda(out, q, kcache, vcache, kscale, vscale, q_start, start_pos, block_table)
+    n = q.shape[0]
+    if (q.dtype == torch.bfloat16 and head_dim in TCGEN05_HEAD_DIMS and USE_TCGEN05 and n_heads // n_kv <= 128
+            and out.data_ptr() % 16 == 0):
+        row_tiles, splits = prefill_q8_parts(n, R, n_kv, n_heads // n_kv, ctx_bound)
+        part_o = part_ml = None
+        if splits > 1:
+            part_o = torch.empty((n, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
+            part_ml = torch.empty((n, n_heads, splits, 2), dtype=torch.float32, device=q.device)
+        lib = load_library("attention_q8_tcgen05", {"KLLM_HD": head_dim})
+        rc = lib.kllm_attention_prefill_q8_tcgen05(
+            _p(out), _p(part_o), _p(part_ml), _p(q), q.stride(0), _p(kcache), _p(vcache), _p(kscale), _p(vscale), _p(q_start),
+            _p(start_pos), _p(block_table), block_table.shape[1], kcache.shape[0], n, R, n_heads, n_kv, head_dim, kcache.shape[2],
+            int(window or 0), scale, row_tiles, splits, _p(status_word(q.device)), _stream())
+        _check(lib, "attention_q8_tcgen05", rc)
+        global launches
+        if splits > 1:
+            launches += 1
+        return
     lib = load_library("attention_q8", {"KLLM_HD": head_dim})
     rc = lib.kllm_attention_prefill_q8(_p(out), _p(q), q.stride(0), _p(kcache), _p(vcache), _p(kscale), _p(vscale), _p(q_start),
                                        _p(start_pos), _p(block_table), block_table.shape[1], kcache.shape[0], q.shape[0], R,
