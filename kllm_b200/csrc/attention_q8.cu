@@ -205,7 +205,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         if (tile >= tile_hi || key < lo || key >= hi) return;
         const int lp = key / a.page_size;
         slot = key - lp * a.page_size;
-        if (lp < a.max_blocks) page = __ldg(table + lp);
+        if (lp < a.max_blocks) page = load_early(table + lp);
     };
     const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + Shape::Q_BYTES + warp * DEC_RING;
     const unsigned meta = ring + DEC_STAGES * 2 * DEC_TILE;

@@ -12,10 +12,11 @@
 //                    shared memory as float16 (divided by a power of two), then per step reads its 128 scores, applies mask and
 //                    online softmax, and writes the weights as float16 over the scores; the second product reads
 //                    its A operand from there.
-//   warps 8-11       loader: a tile's bytes from the pages into registers a tile ahead, converted to float16 and stored in the
+//   warps 8-11, 12-15  loaders of keys and of values: a tile's bytes from the pages into registers a step ahead, converted to float16 and stored in the
 //                    128-byte-swizzled layout that the descriptors name (panels of 64 dims, 8-row groups of 1024 bytes,
 //                    the 16-byte piece index XORed with the row index modulo 8).
-//   warp 12          issues every tcgen05.mma, one elected thread.
+//   warp 16          issues every tcgen05.mma, one elected thread.
+//   warp 17          planner: a few steps ahead of the loader, the rows of a tile's keys and their pages' scales.
 //
 // Scales.  Within a tile's step all keys share one exponent eK and one eV: the loader multiplies every key row by
 // 2^(ek - eK) and every value row by 2^(ev - eV) as it converts, exactly, as long as the difference is within +-7
@@ -32,6 +33,8 @@
 // status word, every role leaves its loop, and the CTA frees its TMEM and returns.
 #include "q8.cuh"
 
+#include <limits.h>
+
 #ifndef KLLM_HD
 #error "compile with -DKLLM_HD=64 or 128"
 #endif
@@ -47,28 +50,40 @@ static_assert(HD == 64 || HD == 128, "head size 64 or 128");
 constexpr int PANELS = HD / 64;            // 64-dim panels of a row
 constexpr int ROWS = 128;                  // query rows of a tile = TMEM lanes
 constexpr int TILE = 128;                  // keys of a tile
-constexpr int THREADS = 512;
+constexpr int LOADERS = 128;               // threads that bring keys, and as many that bring values
+constexpr int THREADS = 640;
 constexpr int PANEL = 128 * 128;           // bytes of a panel: 128 rows of 64 float16
 constexpr int Q_BYTES = PANELS * PANEL;    // per row tile
 constexpr int KV_BYTES = PANELS * PANEL;   // keys or values of a tile
 constexpr int STAGES = HD == 64 ? 3 : 2;
-constexpr int NOTES = 4;                   // steps described at a time; see note_ring
+constexpr int SBUFS = HD == 64 ? 3 : 2;    // score buffers in TMEM, 128 columns each: taken in turn by the row tiles' steps
+constexpr int PLANS = 4;                   // steps that the planner is ahead of the loader
+constexpr int NOTES = 16;                  // steps described at a time; see Note
 constexpr int SMEM_BYTES = 1024 + 2 * Q_BYTES + STAGES * 2 * KV_BYTES;
 static_assert(SMEM_BYTES <= 226 * 1024, "shared memory");
-constexpr unsigned COL_S = 0, COL_O = 256; // scores / weights of the row tiles: 128 columns each; outputs: HD each
+constexpr unsigned COL_S = 0, COL_O = SBUFS * TILE;      // scores / weights, outputs of the row tiles (HD columns each)
 constexpr int TMEM_COLS = 512;
-constexpr int REGS_SOFTMAX = 168, REGS_LOADER = 120, REGS_ISSUER = 56;
-// setmaxnreg moves registers inside the CTA's own allocation (threads x registers at launch)
-static_assert(2 * REGS_SOFTMAX + REGS_LOADER + REGS_ISSUER <= THREADS / 128 * (65536 / THREADS), "setmaxnreg budget");
+static_assert(SBUFS * TILE + 2 * HD <= TMEM_COLS, "tensor memory");
+constexpr int REGS_SOFTMAX = 160, REGS_LOADER = 56, REGS_ISSUER = 48;
+// setmaxnreg moves registers inside the CTA's own allocation (threads x registers at launch, multiples of 8)
+static_assert(2 * REGS_SOFTMAX + 2 * REGS_LOADER + REGS_ISSUER <= THREADS / 128 * (65536 / THREADS / 8 * 8), "setmaxnreg budget");
+static_assert(PLANS + STAGES < NOTES, "notes");
 constexpr int PIECES = HD / 16;            // 16-byte pieces of a stored row
-constexpr int LOADS = TILE * PIECES / 128; // pieces of the keys (of the values) a loader thread carries
+constexpr int LOADS = TILE * PIECES / LOADERS;           // pieces of the keys (of the values) a loader thread carries
+constexpr int KEY_STEP = LOADERS / PIECES;               // its pieces' keys are so far apart
 constexpr int E_SPAN = 7;                  // how far a key's exponents may be from its step's
 
-// What the loader says of a step.  note_ring: the note of step t is written once the keys of step t - STAGES have been used,
-// for which both softmax groups have passed step t - STAGES - 1; with STAGES <= 3 nobody still reads step t - 4's.
+// What the planner says of a step to everybody.  The note of step t is written once the values of step t - PLANS are converted,
+// for which the products of step t - PLANS - STAGES are through: nobody still reads a note of an earlier step.
 struct Note {
     int key0, ek, ev, last;
     uint32_t member[4];                    // the keys of the tile that this step is for
+};
+// ... and to the loader: the keys' rows in the stores, and what they are multiplied with (2^difference as two float16; 0: not of
+// this step).
+struct __align__(16) Plan {               // read and written four words at a time
+    int row[TILE];
+    uint32_t kmul[TILE], vmul[TILE];
 };
 
 // Instruction descriptor: float32 accumulator, float16 A and B, M x N, B optionally MN-major.
@@ -100,6 +115,16 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __device__ __forceinline__ unsigned swz(int r, int ch) {
     return (unsigned)((r >> 3) * 1024 + (r & 7) * 128 + ((ch ^ (r & 7)) << 4));
 }
+__device__ __forceinline__ void tmem_ld8(unsigned taddr, float (&v)[8]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(unsigned taddr, const float (&v)[8]) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ void store16(unsigned addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -108,8 +133,32 @@ __device__ __forceinline__ uint32_t half2_times(uint32_t x, uint32_t m) {
     asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(x), "r"(m));
     return r;
 }
+// two float32 at a time
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // bits 0 .. n - 1
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// What a CTA is about, worked out by one thread.  Every role reads what it needs of it from shared memory: values that all roles
+// derive from registers are kept, or spilled, for all of them.
+struct Work {
+    int req, tok0, n_tok, tiles, pos0, lo, hi, tile_lo, tile_hi;     // request (-1: none), rows, row tiles in use, keys, tiles of keys
+};
 
 struct Args {
     bf16* out;
@@ -133,234 +182,332 @@ struct Args {
 __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const Args a) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t bar_k_full[STAGES], bar_k_empty[STAGES], bar_v_full[STAGES], bar_v_empty[STAGES];
-    __shared__ __align__(8) uint64_t bar_q_full[2], bar_s_full[2], bar_p_full[2], bar_o_full[2], bar_note[NOTES];
+    __shared__ __align__(8) uint64_t bar_q_full[2], bar_s_full[SBUFS], bar_p_full[SBUFS][2], bar_pv[2], bar_note[NOTES];
+    __shared__ __align__(8) uint64_t bar_plan_full[PLANS], bar_plan_empty[PLANS];
     __shared__ Note s_note[NOTES];
-    __shared__ int s_row[TILE], s_exp[TILE];               // the loader's keys: rows in the stores, exponents (INT_MIN: none)
-    __shared__ uint32_t s_left[4];
+    __shared__ Plan s_plan[PLANS];
+    static_assert(alignof(Plan) == 16 && sizeof(Plan) % 16 == 0, "four words at a time");
     __shared__ unsigned s_tmem;
-    __shared__ int s_req, s_tok0, s_abort;
-    const int split = blockIdx.x % a.splits, kvh = (blockIdx.x / a.splits) % a.n_kv;   // CTAs start in the order of blockIdx.x:
-    const int gs = a.n_heads / a.n_kv, tpt = a.tokens_per_tile, per_cta = tpt * a.row_tiles;     // longest key ranges first
+    __shared__ volatile Work s_work;
+    __shared__ int s_abort;
     const int warp = warp_index(), lane = threadIdx.x & 31;
     griddep_wait();
     griddep_launch();
     if (threadIdx.x == 0) {
-        int tile = (gridDim.x - 1 - blockIdx.x) / (a.n_kv * a.splits), req = -1, tok0 = 0;
+        // CTAs start in the order of blockIdx.x: longest key ranges first, all kv heads and parts of a range side by side
+        const int per_cta = a.tokens_per_tile * a.row_tiles, split = blockIdx.x % a.splits;
+        int tile = (gridDim.x - 1 - blockIdx.x) / (a.n_kv * a.splits), req = -1, tok0 = 0, first_row = 0, end = 0;
         for (int s = 0; s < a.n_requests; s++) {
             const int n = a.q_start[s + 1] - a.q_start[s];
             const int nt = (n + per_cta - 1) / per_cta;
-            if (tile < nt) { req = s; tok0 = a.q_start[s] + tile * per_cta; break; }
+            if (tile < nt) {
+                req = s;
+                first_row = a.q_start[s];
+                tok0 = first_row + tile * per_cta;
+                end = min(a.q_start[s + 1], a.n_tokens);
+                break;
+            }
             tile -= nt;
         }
-        if (req >= 0 && min(a.q_start[req + 1], a.n_tokens) <= tok0) req = -1;
-        s_req = req; s_tok0 = tok0; s_abort = 0;
+        if (req >= 0 && end <= tok0) req = -1;
+        s_work.req = req;
+        if (req >= 0) {
+            const int n_tok = min(per_cta, end - tok0), pos0 = a.start_pos[req] + (tok0 - first_row);
+            const int lo = (a.window > 0 && pos0 + 1 > a.window) ? pos0 + 1 - a.window : 0;
+            const int hi = max(pos0 + n_tok, 1);               // one tile at least: every role takes at least one step
+            // this part's tiles of keys; a part without any leaves zeros
+            const int first = lo / TILE, all = (hi + TILE - 1) / TILE - first, per = (all + a.splits - 1) / a.splits;
+            s_work.tok0 = tok0;
+            s_work.n_tok = n_tok;
+            s_work.tiles = n_tok > a.tokens_per_tile ? 2 : 1;
+            s_work.pos0 = pos0;
+            s_work.lo = lo;
+            s_work.hi = hi;
+            s_work.tile_lo = first + min(all, split * per);
+            s_work.tile_hi = first + min(all, (split + 1) * per);
+        }
+        s_abort = 0;
         for (int i = 0; i < STAGES; i++) {
-            mbar_init(&bar_k_full[i], 128); mbar_init(&bar_k_empty[i], 1);
-            mbar_init(&bar_v_full[i], 128); mbar_init(&bar_v_empty[i], 1);
+            mbar_init(&bar_k_full[i], LOADERS); mbar_init(&bar_k_empty[i], 1);
+            mbar_init(&bar_v_full[i], LOADERS); mbar_init(&bar_v_empty[i], 1);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&bar_q_full[i], ROWS); mbar_init(&bar_s_full[i], 1);
-            mbar_init(&bar_p_full[i], ROWS); mbar_init(&bar_o_full[i], 1);
+        for (int i = 0; i < SBUFS; i++) {
+            mbar_init(&bar_s_full[i], 1);
+            mbar_init(&bar_p_full[i][0], ROWS); mbar_init(&bar_p_full[i][1], ROWS);
         }
-        for (int i = 0; i < NOTES; i++) mbar_init(&bar_note[i], 128);
+        for (int i = 0; i < 2; i++) { mbar_init(&bar_q_full[i], ROWS); mbar_init(&bar_pv[i], 1); }
+        for (int i = 0; i < NOTES; i++) mbar_init(&bar_note[i], 32);
+        for (int i = 0; i < PLANS; i++) { mbar_init(&bar_plan_full[i], 32); mbar_init(&bar_plan_empty[i], 2 * LOADERS); }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     __syncthreads();
-    const int req = s_req;
-    if (req < 0) return;                       // the grid is an upper bound on the tiles
-    if (warp == 12) {
+    if (s_work.req < 0) return;                // the grid is an upper bound on the tiles
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    const int tok0 = s_tok0;
-    const int n_tok = min(per_cta, min(a.q_start[req + 1], a.n_tokens) - tok0);       // at least 1
-    const int tiles = n_tok > tpt ? 2 : 1;     // row tiles in use
-    const int pos0 = a.start_pos[req] + (tok0 - a.q_start[req]);
-    const int lo = (a.window > 0 && pos0 + 1 > a.window) ? pos0 + 1 - a.window : 0;
-    const int hi = max(pos0 + n_tok, 1);       // one tile at least: every role takes at least one step
-    // this part's tiles of keys
-    const int first = lo / TILE, all = (hi + TILE - 1) / TILE - first;
-    const int per_split = (all + a.splits - 1) / a.splits;
-    const int tile_lo = first + min(all, split * per_split), tile_hi = first + min(all, (split + 1) * per_split);
-    const bool nothing = tile_lo >= tile_hi;   // a part without keys: its rows' sums are zeros
     volatile int* abort_flag = &s_abort;
-    const unsigned base = (smem_u32(smem_raw) + 1023u) & ~1023u;       // swizzled tiles want 1024-byte alignment
-    const unsigned sQ = base, sK = base + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES;
+    volatile unsigned* tmem_at = &s_tmem;
+    const bool nothing = s_work.tile_lo >= s_work.tile_hi;
+    // swizzled tiles want 1024-byte alignment
+    auto shared_base = [&]() { return (smem_u32(smem_raw) + 1023u) & ~1023u; };
 
-    if (warp >= 12) {
+    if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_ISSUER));
-        if (warp == 12 && !nothing) {
-            // ---- the issuer: the first scores of both row tiles, then per step and row tile weights x values and the next scores
+        if (warp == 16 && !nothing) {
+            // ---- the issuer.  A job is a row tile's step; jobs go round the score buffers.  The scores of the first SBUFS jobs,
+            // then for every job weights x values and the scores of the job SBUFS behind it, whose buffer that product has read
+            // (the tensor core works in the order of issue).
+            const int tiles = s_work.tiles;
+            const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_at, 0), sQ = shared_base(), sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES;
             constexpr uint32_t IDESC_S = make_idesc_f16(ROWS, TILE, false), IDESC_O = make_idesc_f16(ROWS, HD, true);
             const uint32_t q_lo0 = desc_lo(sQ, 16), k_lo0 = desc_lo(sK, 16), v_lo0 = desc_lo(sV, PANEL);
-            auto issue_scores = [&](int x, int stage) {
-                const uint32_t q_lo = q_lo0 + (uint32_t)(x * (Q_BYTES >> 4)), k_lo = k_lo0 + (uint32_t)(stage * (KV_BYTES >> 4));
+            int s_step = 0, s_x = 0, s_buf = 0, ks = 0;        // the next scores: step, row tile, buffer; stage of its keys
+            unsigned kp = 0;
+            bool s_last = false, s_done = false;
+            auto next_scores = [&]() -> bool {
+                if (s_done) return true;
+                if (s_x == 0) {
+                    if (!mbar_wait_warp(&bar_note[s_step % NOTES], (unsigned)(s_step / NOTES) & 1u, abort_flag, a.status, 6) ||
+                        !mbar_wait_warp(&bar_k_full[ks], kp, abort_flag, a.status, 3))
+                        return false;
+                    s_last = s_note[s_step % NOTES].last != 0;
+                }
+                if (s_step == 0 && !mbar_wait_warp(&bar_q_full[s_x], 0, abort_flag, a.status, 2)) return false;
+                fence_async_smem();
+                tc_fence_after();
                 if (elect_one()) {
+                    const uint32_t q_lo = q_lo0 + (uint32_t)(s_x * (Q_BYTES >> 4)), k_lo = k_lo0 + (uint32_t)(ks * (KV_BYTES >> 4));
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++) {
                         const uint32_t off = (uint32_t)(((kk >> 2) * PANEL + (kk & 3) * 32) >> 4);
-                        umma_words(tmem + COL_S + x * TILE, q_lo + off, k_lo + off, IDESC_S, kk > 0);
+                        umma_words(tmem + COL_S + s_buf * TILE, q_lo + off, k_lo + off, IDESC_S, kk > 0);
                     }
-                    umma_commit(&bar_s_full[x]);
-                    if (x == tiles - 1) umma_commit(&bar_k_empty[stage]);
+                    umma_commit(&bar_s_full[s_buf]);
+                    if (s_x == tiles - 1) umma_commit(&bar_k_empty[ks]);
                 }
                 __syncwarp();
+                s_buf = s_buf + 1 == SBUFS ? 0 : s_buf + 1;
+                if (++s_x == tiles) {
+                    s_x = 0;
+                    s_step++;
+                    s_done = s_last;
+                    if (++ks == STAGES) { ks = 0; kp ^= 1u; }
+                }
+                return true;
             };
             bool ok = true;
-            for (int x = 0; ok && x < tiles; x++) ok = mbar_wait_warp(&bar_q_full[x], 0, abort_flag, a.status, 2);
-            ok = ok && mbar_wait_warp(&bar_k_full[0], 0, abort_flag, a.status, 3);
-            if (ok) {
-                fence_async_smem();
-                tc_fence_after();
-                for (int x = 0; x < tiles; x++) issue_scores(x, 0);
-            }
-            int ks = STAGES == 1 ? 0 : 1, vs = 0;              // stages of the next scores' keys and of these values
-            unsigned kp = 0, vp = 0;                           // and their parities
-            for (int step = 0; ok; step++) {
+            for (int i = 0; ok && i < SBUFS; i++) ok = next_scores();
+            int step = 0, x = 0, buf = 0, vs = 0;              // of the next product
+            unsigned pp = 0, vp = 0;
+            while (ok) {
                 const bool last = s_note[step % NOTES].last != 0;
-                ok = mbar_wait_warp(&bar_v_full[vs], vp, abort_flag, a.status, 4);
-                for (int x = 0; ok && x < tiles; x++) {
-                    // the weights are in tensor memory and the output is rescaled
-                    ok = mbar_wait_warp(&bar_p_full[x], (unsigned)step & 1u, abort_flag, a.status, 5);
+                if (x == 0) ok = mbar_wait_warp(&bar_v_full[vs], vp, abort_flag, a.status, 4);
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    // half of the weights are in tensor memory, and the output is rescaled
+                    ok = ok && mbar_wait_warp(&bar_p_full[buf][half], pp, abort_flag, a.status, 5);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint32_t v_lo = v_lo0 + (uint32_t)(vs * (KV_BYTES >> 4));
 #pragma unroll
-                        for (int kk = 0; kk < TILE / 16; kk++)
-                            umma_tmem_a_words(tmem + COL_O + x * HD, tmem + COL_S + x * TILE + (unsigned)(kk * 8),
+                        for (int kk = half * (TILE / 32); kk < (half + 1) * (TILE / 32); kk++)
+                            umma_tmem_a_words(tmem + COL_O + x * HD, tmem + COL_S + buf * TILE + (unsigned)(kk * 8),
                                               v_lo + (uint32_t)(kk * (2048 >> 4)), IDESC_O, step > 0 || kk > 0);
-                        if (x == tiles - 1) umma_commit(&bar_v_empty[vs]);
-                        if (last) umma_commit(&bar_o_full[x]);
+                        if (half == 1) {
+                            umma_commit(&bar_pv[x]);
+                            if (x == tiles - 1) umma_commit(&bar_v_empty[vs]);
+                        }
                     }
                     __syncwarp();
-                    if (!last) {
-                        if (x == 0) {
-                            ok = mbar_wait_warp(&bar_k_full[ks], kp, abort_flag, a.status, 6);
-                            if (!ok) break;
-                            fence_async_smem();
-                            tc_fence_after();
-                        }
-                        issue_scores(x, ks);           // in issue order behind the product that reads the columns it overwrites
+                }
+                ok = ok && next_scores();
+                if (!ok || (last && x == tiles - 1)) break;
+                if (++buf == SBUFS) { buf = 0; pp ^= 1u; }
+                if (++x == tiles) {
+                    x = 0;
+                    step++;
+                    if (++vs == STAGES) { vs = 0; vp ^= 1u; }
+                }
+            }
+        }
+        if (warp == 17 && !nothing) {
+            // ---- the planner: which keys a step is for, where they lie, what they are multiplied with.  A lane looks after four
+            // neighbouring keys of a tile.  Where these lie in one page (page sizes in steps of four) pages are read two tiles
+            // ahead of their step, scales one; otherwise each when it is needed.
+            const int lo = s_work.lo, hi = s_work.hi, tile_hi = s_work.tile_hi, kvh = (blockIdx.x / a.splits) % a.n_kv;
+            const int* table = a.block_table + (int64_t)s_work.req * a.max_blocks;
+            const bool quads = a.page_size % 4 == 0;
+            int page = -1, first_row = -1;
+            float ksc = 1.f, vsc = 1.f;
+            auto page_of = [&](int key) {
+                const int lp = key / a.page_size;
+                return key < hi && lp < a.max_blocks ? load_early(table + lp) : -1;
+            };
+            auto place = [&](int pg, int key) {
+                first_row = -1;
+                if ((unsigned)pg >= (unsigned)a.n_pages) return;
+                const int cell = pg * a.n_kv + kvh;
+                first_row = cell * a.page_size + key % a.page_size;
+                ksc = load_early(a.kscale + cell);
+                vsc = load_early(a.vscale + cell);
+            };
+            auto exponents = [&]() { return (q8_exponent(ksc) << 16) | (q8_exponent(vsc) & 0xffff); };
+            int key = s_work.tile_lo * TILE + lane * 4;        // the lane's first
+            if (quads) {
+                place(page_of(key), key);
+                page = page_of(key + TILE);
+            }
+            bool ok = true;
+            int step = 0;
+#pragma unroll 1
+            for (int tile = s_work.tile_lo; ok && tile < tile_hi; tile++, key += TILE) {
+                int at[4], exps[4];                            // rows in the stores, exponents of the scales (INT_MIN: no key)
+                if (quads) {
+                    const int e = exponents();
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const bool there = first_row >= 0 && key + i >= lo && key + i < hi;
+                        at[i] = there ? first_row + i : -1;
+                        exps[i] = there ? e : INT_MIN;
+                    }
+                    place(page, key + TILE);
+                    page = page_of(key + 2 * TILE);
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 4; i++) {
+                        place(key + i >= lo ? page_of(key + i) : -1, key + i);
+                        const int r = first_row, e = r < 0 ? INT_MIN : exponents();
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (j == i) { at[j] = r; exps[j] = e; }
                     }
                 }
-                if (last) break;
-                if (++ks == STAGES) { ks = 0; kp ^= 1u; }
-                if (++vs == STAGES) { vs = 0; vp ^= 1u; }
+                bool done = false;
+#pragma unroll 1
+                while (ok && !done) {
+                    // the first key that is left names the step's exponents; those near enough join it
+                    const int mine = exps[0] != INT_MIN ? exps[0] : exps[1] != INT_MIN ? exps[1] : exps[2] != INT_MIN ? exps[2] : exps[3];
+                    const unsigned have = __ballot_sync(0xffffffffu, mine != INT_MIN);
+                    const int lead = have ? __shfl_sync(0xffffffffu, mine, __ffs(have) - 1) : 0;
+                    const int ek = lead >> 16, ev = (int)(short)(lead & 0xffff);
+                    uint32_t kmul[4], vmul[4], bits = 0;
+                    bool left = false;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int dk = (exps[i] >> 16) - ek, dv = (int)(short)(exps[i] & 0xffff) - ev;
+                        const bool in = exps[i] != INT_MIN && abs(dk) <= E_SPAN && abs(dv) <= E_SPAN;
+                        kmul[i] = in ? (uint32_t)(dk + 15) * 0x04000400u : 0u;
+                        vmul[i] = in ? (uint32_t)(dv + 15) * 0x04000400u : 0u;
+                        if (in) { bits |= 1u << i; exps[i] = INT_MIN; }
+                        left = left || exps[i] != INT_MIN;
+                    }
+                    done = !__any_sync(0xffffffffu, left);
+                    // eight lanes' four bits are a word
+                    uint32_t word = bits << ((lane & 7) * 4);
+#pragma unroll
+                    for (int d = 1; d < 8; d <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, d);
+                    const int p = step % PLANS;
+                    ok = mbar_wait_warp(&bar_plan_empty[p], ((unsigned)(step / PLANS) & 1u) ^ 1u, abort_flag, a.status, 12);
+                    if (!ok) break;
+                    Note& note = s_note[step % NOTES];
+                    if ((lane & 7) == 0) note.member[lane >> 3] = word;
+                    if (lane == 0) { note.key0 = tile * TILE; note.ek = ek; note.ev = ev; note.last = done && tile + 1 == tile_hi; }
+                    *reinterpret_cast<int4*>(&s_plan[p].row[lane * 4]) = make_int4(at[0], at[1], at[2], at[3]);
+                    *reinterpret_cast<uint4*>(&s_plan[p].kmul[lane * 4]) = make_uint4(kmul[0], kmul[1], kmul[2], kmul[3]);
+                    *reinterpret_cast<uint4*>(&s_plan[p].vmul[lane * 4]) = make_uint4(vmul[0], vmul[1], vmul[2], vmul[3]);
+                    mbar_arrive(&bar_note[step % NOTES]);
+                    mbar_arrive(&bar_plan_full[p]);
+                    step++;
+                }
             }
         }
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_LOADER));
-        // ---- loader ------------------------------------------------------------------------
-        const int tid = threadIdx.x - 256;
-        const int* table = a.block_table + (int64_t)req * a.max_blocks;
-        int row = -1, exps = INT_MIN;                      // of key tile * 128 + tid
-        auto lookup = [&](int tile) {
-            row = -1; exps = INT_MIN;
-            const int key = tile * TILE + tid;
-            if (tile >= tile_hi || key < lo || key >= hi) return;
-            const int lp = key / a.page_size;
-            if (lp >= a.max_blocks) return;
-            const int page = __ldg(table + lp);
-            if ((unsigned)page >= (unsigned)a.n_pages) return;
-            const int cell = page * a.n_kv + kvh;
-            row = cell * a.page_size + key - lp * a.page_size;
-            exps = (q8_exponent(__ldg(a.kscale + cell)) << 16) | (q8_exponent(__ldg(a.vscale + cell)) & 0xffff);
-        };
-        // a thread's pieces: their keys differ by whole groups of 128 / PIECES
-        const int piece = tid % PIECES, key_off = tid / PIECES;
-        const bool odd_first = PIECES == 8 && piece >= 4;      // the panels of a row at a time on different banks
-        uint4 kraw[LOADS], vraw[LOADS];
-        auto convert = [&](const uint4 (&raw)[LOADS], unsigned dst, int shift_of, int e_step) {
+        // ---- loaders, one group for the keys and one for the values: a step's bytes into registers while the step before is
+        // being used, converted in pairs, float16 into the stages
+        if (!nothing) {
+            const bool values = warp >= 12;
+            const int tid = threadIdx.x & 127;
+            const unsigned stages = shared_base() + 2 * Q_BYTES + (values ? STAGES * KV_BYTES : 0);
+            const uint8_t* store = values ? a.vcache : a.kcache;
+            uint64_t* full = values ? bar_v_full : bar_k_full;
+            uint64_t* empty = values ? bar_v_empty : bar_k_empty;
+            // a thread's pieces are of keys KEY_STEP apart
+            const int piece = tid % PIECES, key_off = tid / PIECES;
+            const bool odd_first = PIECES == 8 && piece >= 4;  // the panels of a row at a time on different banks
+            const unsigned place = (unsigned)((piece >> 2) * PANEL) + swz(key_off, (piece & 3) * 2 + (odd_first ? 1 : 0));
+            store += piece * 16;
+            uint4 raw[LOADS];
+            auto fetch = [&](int p) {
 #pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int key = key_off + i * (128 / PIECES);
-                const int ee = s_exp[key];
-                const bool in = ee != INT_MIN && ((s_left[key >> 5] >> (key & 31)) & 1u);
-                const int d = (shift_of ? ee >> 16 : (int)(short)(ee & 0xffff)) - e_step;
-                // 2^d as two float16: exponent field d + 15
-                const uint32_t m = (uint32_t)((d + 15) << 10) * 0x10001u;
-                uint4 x = raw[i];
-                if (!in) x = make_uint4(0, 0, 0, 0);
-                uint32_t h[8];
-                q8_to_f16x4(x.x, h[0], h[1]); q8_to_f16x4(x.y, h[2], h[3]);
-                q8_to_f16x4(x.z, h[4], h[5]); q8_to_f16x4(x.w, h[6], h[7]);
-                if (in) {
+                for (int i = 0; i < LOADS; i++) {
+                    // where there is no key: the first row, which the conversion leaves out
+                    const int r = max(s_plan[p].row[key_off + i * KEY_STEP], 0);
+                    raw[i] = load_early(reinterpret_cast<const uint4*>(store + (int64_t)r * HD));
+                }
+            };
+            int stage = 0;
+            unsigned parity = 1;                               // of the stages' "empty" barriers: free at first
+            bool ok = mbar_wait(&bar_plan_full[0], 0, abort_flag, a.status, 1);
+            if (ok) fetch(0);
+#pragma unroll 1
+            for (int step = 0; ok; step++) {
+                const int p = step % PLANS, p2 = (step + 1) % PLANS;
+                const Note& note = s_note[step % NOTES];
+                const bool last = note.last != 0;
+                // not all keys of the tile are of this step: the multiplier of the others is 0, and their bytes (which may be
+                // NaN) become zeros
+                const bool some = (note.member[0] & note.member[1] & note.member[2] & note.member[3]) != 0xffffffffu;
+                const uint32_t* mul = (values ? s_plan[p].vmul : s_plan[p].kmul) + key_off;
+                ok = mbar_wait(&empty[stage], parity, abort_flag, a.status, 7);
+                if (!ok) break;
+                const unsigned dst = stages + stage * KV_BYTES + place;
+#pragma unroll
+                for (int i = 0; i < LOADS; i++) {
+                    const uint32_t m = mul[i * KEY_STEP];
+                    uint4 x = raw[i];
+                    if (some) {
+                        const uint32_t keep = m ? 0xffffffffu : 0u;
+                        x.x &= keep; x.y &= keep; x.z &= keep; x.w &= keep;
+                    }
+                    uint32_t h[8];
+                    q8_to_f16x4(x.x, h[0], h[1]); q8_to_f16x4(x.y, h[2], h[3]);
+                    q8_to_f16x4(x.z, h[4], h[5]); q8_to_f16x4(x.w, h[6], h[7]);
 #pragma unroll
                     for (int j = 0; j < 8; j++) h[j] = half2_times(h[j], m);
+                    // rows KEY_STEP apart are whole groups of eight apart: the same place in a later group; the other half of the
+                    // piece is the neighbouring chunk, one bit away
+                    const unsigned at = dst + (unsigned)(i * KEY_STEP * 128);
+                    static_assert(KEY_STEP % 8 == 0, "groups of eight rows");
+                    if (odd_first) {
+                        store16(at, h[4], h[5], h[6], h[7]);
+                        store16(at ^ 16u, h[0], h[1], h[2], h[3]);
+                    } else {
+                        store16(at, h[0], h[1], h[2], h[3]);
+                        store16(at ^ 16u, h[4], h[5], h[6], h[7]);
+                    }
                 }
-                const unsigned panel = dst + (unsigned)((piece >> 2) * PANEL);
-                const unsigned at0 = panel + swz(key, (piece & 3) * 2), at1 = panel + swz(key, (piece & 3) * 2 + 1);
-                if (odd_first) {
-                    store16(at1, h[4], h[5], h[6], h[7]);
-                    store16(at0, h[0], h[1], h[2], h[3]);
-                } else {
-                    store16(at0, h[0], h[1], h[2], h[3]);
-                    store16(at1, h[4], h[5], h[6], h[7]);
-                }
-            }
-        };
-        lookup(tile_lo);
-        bool ok = true;
-        int stage = 0, step = 0;
-        unsigned parity = 1;                                   // of the stages' "empty" barriers: free at first
-        for (int tile = tile_lo; ok && tile < tile_hi; tile++) {
-            s_row[tid] = row; s_exp[tid] = exps;
-            named_sync(1, 128);
-#pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int r = s_row[key_off + i * (128 / PIECES)];
-                kraw[i] = vraw[i] = make_uint4(0, 0, 0, 0);
-                if (r >= 0) {
-                    kraw[i] = __ldg(reinterpret_cast<const uint4*>(a.kcache + (int64_t)r * HD + piece * 16));
-                    vraw[i] = __ldg(reinterpret_cast<const uint4*>(a.vcache + (int64_t)r * HD + piece * 16));
-                }
-            }
-            bool left = exps != INT_MIN;                       // this thread's key has not had its step
-            const int mine = exps;
-            lookup(tile + 1);
-            bool done = false;
-            while (ok && !done) {
-                // the first key that is left names the step's exponents; those near enough join it
-                const uint32_t b = __ballot_sync(0xffffffffu, left);
-                if (lane == 0) s_left[warp - 8] = b;
-                named_sync(1, 128);
-                int lead = -1;
-#pragma unroll
-                for (int w = 3; w >= 0; w--)
-                    if (s_left[w]) lead = w * 32 + __ffs(s_left[w]) - 1;
-                const int le = lead >= 0 ? s_exp[lead] : 0, ek = le >> 16, ev = (int)(short)(le & 0xffff);
-                const bool in = left && abs((mine >> 16) - ek) <= E_SPAN && abs((int)(short)(mine & 0xffff) - ev) <= E_SPAN;
-                done = half_all(2, !left || in);               // and everybody has read s_left
-                const uint32_t member = __ballot_sync(0xffffffffu, in);
-                if (lane == 0) s_left[warp - 8] = member;
-                left = left && !in;
-                ok = half_all(1, mbar_wait(&bar_k_empty[stage], parity, abort_flag, a.status, 1));
-                if (!ok) break;
-                Note& note = s_note[step % NOTES];
-                if (lane == 0) note.member[warp - 8] = member;
-                if (tid == 0) { note.key0 = tile * TILE; note.ek = ek; note.ev = ev; note.last = done && tile + 1 == tile_hi; }
-                mbar_arrive(&bar_note[step % NOTES]);
-                convert(kraw, sK + stage * KV_BYTES, 1, ek);
                 fence_async_smem();
-                mbar_arrive(&bar_k_full[stage]);
-                ok = half_all(1, mbar_wait(&bar_v_empty[stage], parity, abort_flag, a.status, 7));
+                mbar_arrive(&full[stage]);
+                mbar_arrive(&bar_plan_empty[p]);
+                if (last) break;
+                ok = mbar_wait(&bar_plan_full[p2], (unsigned)((step + 1) / PLANS) & 1u, abort_flag, a.status, 1);
                 if (!ok) break;
-                convert(vraw, sV + stage * KV_BYTES, 0, ev);
-                fence_async_smem();
-                mbar_arrive(&bar_v_full[stage]);
+                fetch(p2);
                 if (++stage == STAGES) { stage = 0; parity ^= 1u; }
-                step++;
-                named_sync(1, 128);                            // s_left and s_row are read
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFTMAX));
         // ---- softmax: this thread's row is (token, head of the group) of row tile x -----------------------
+        const int gs = a.n_heads / a.n_kv, tpt = a.tokens_per_tile, kvh = (blockIdx.x / a.splits) % a.n_kv, split = blockIdx.x % a.splits;
+        const int tok0 = s_work.tok0, n_tok = s_work.n_tok, pos0 = s_work.pos0, tiles = s_work.tiles;
+        const unsigned tmem = *tmem_at;
         const int x = warp >> 2, r = threadIdx.x & 127;
         const int tt = x * tpt + r / gs, hh = r % gs;
         const bool valid = r < tpt * gs && tt < n_tok;
@@ -368,7 +515,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
         const int w_row = (a.window > 0) ? p_row + 1 - a.window : 0;
         const int64_t at = (int64_t)(tok0 + tt) * a.n_heads + kvh * gs + hh;
         const unsigned lane_base = (unsigned)((warp & 3) * 32) << 16;
-        const unsigned t_s = tmem + lane_base + COL_S + x * TILE, t_o = tmem + lane_base + COL_O + x * HD;
+        const unsigned t_s0 = tmem + lane_base + COL_S, t_o = tmem + lane_base + COL_O + x * HD;
         float m_ref = -INFINITY, l_run = 0.f;
         bool ok = x < tiles && !nothing;
         if (ok) {
@@ -394,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             const bool finite = m < 0x7f800000;
             const float up = finite ? copysignf(q8_pow2(row_shift(m)), a.scale) : 0.f;
             const float factor = finite ? fabsf(a.scale) * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);
-            const unsigned dst = sQ + x * Q_BYTES;
+            const unsigned dst = shared_base() + x * Q_BYTES;
 #pragma unroll
             for (int i = 0; i < HD / 8; i++) {
                 uint32_t h[4];
@@ -408,16 +555,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             fence_async_smem();
             mbar_arrive(&bar_q_full[x]);
             bool last = false;
-            for (int step = 0; ok && !last; step++) {
+            int step = 0, buf = x % SBUFS;
+            unsigned parity = 0;
+            for (; ok && !last; step++) {
                 ok = mbar_wait(&bar_note[step % NOTES], (unsigned)(step / NOTES) & 1u, abort_flag, a.status, 8) &&
-                     mbar_wait(&bar_s_full[x], (unsigned)step & 1u, abort_flag, a.status, 9);
+                     mbar_wait(&bar_s_full[buf], parity, abort_flag, a.status, 9);
                 if (!ok) break;
+                const unsigned t_s = t_s0 + buf * TILE;
                 tc_fence_after();
                 const Note& note = s_note[step % NOTES];
                 last = note.last != 0;
                 // never 0 (a scale of 0, tiny queries): -inf has to stay -inf; NaN stays
                 const float product = factor * q8_pow2(note.ek), f = product < 1.1754944e-38f ? 1.1754944e-38f : product;
-                const float ev = (float)note.ev;
+                const float ev = (float)note.ev, per_sum = q8_pow2(-note.ev);
                 // which of the tile's keys this row sees
                 const int upto = p_row - note.key0 + 1, from = w_row - note.key0;
                 uint32_t seen[4];
@@ -442,7 +592,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
 #pragma unroll
                 for (int c = 0; c < 4; c++)
 #pragma unroll
-                    for (int j = 0; j < 32; j++) mx4[j & 3] = fmaxf(mx4[j & 3], s[c][j]);
+                    for (int j = 0; j < 32; j += 2) mx4[(j >> 1) & 3] = max3(mx4[(j >> 1) & 3], s[c][j], s[c][j + 1]);
                 const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 const float mx = top == -INFINITY ? -INFINITY : fmaf(top, f, ev);
                 const bool move = mx > m_ref + kMoveAt;
@@ -452,7 +602,28 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     m_ref = mx;
                 }
                 const float shift = m_ref == -INFINITY ? ev + kLift : ev - m_ref + kLift;
-                float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+                // the product of this row tile's step before is over (waited for every time: a wait by parity is only sound for
+                // the phase behind the one waited for last)
+                if (step > 0) {
+                    ok = mbar_wait(&bar_pv[x], (unsigned)(step - 1) & 1u, abort_flag, a.status, 10);
+                    if (!ok) break;
+                    if (__any_sync(0xffffffffu, move)) {
+                        // rows of this warp rescale what the products so far have added up (rows that did not move multiply by
+                        // one); the next product waits for these weights
+                        tc_fence_after();
+#pragma unroll
+                        for (int cb = 0; cb < HD / 8; cb++) {
+                            float t[8];
+                            tmem_ld8(t_o + cb * 8, t);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 8; j++) t[j] *= corr;
+                            tmem_st8(t_o + cb * 8, t);
+                        }
+                    }
+                }
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const float2 f2 = make_float2(f, f), shift2 = make_float2(shift, shift);
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     float pk[32];
@@ -460,32 +631,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     for (int c = 0; c < 2; c++)
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
-                            const float p0 = fast_exp2(fmaf(s[half * 2 + c][j], f, shift)), p1 = fast_exp2(fmaf(s[half * 2 + c][j + 1], f, shift));
-                            sum4[j & 3] += p0;
-                            sum4[(j + 1) & 3] += p1;
-                            pk[c * 16 + j / 2] = __uint_as_float(q8_half2(p0, p1));
+                            float2 p = fma2(make_float2(s[half * 2 + c][j], s[half * 2 + c][j + 1]), f2, shift2);
+                            p.x = fast_exp2(p.x);
+                            p.y = fast_exp2(p.y);
+                            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], p);
+                            pk[c * 16 + j / 2] = __uint_as_float(q8_half2(p.x, p.y));
                         }
                     tmem_st32(t_s + half * 32, pk);        // over the first 64 columns of the scores
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&bar_p_full[buf][half]);
                 }
-                l_run = l_run * corr + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) * q8_pow2(-note.ev);
-                if (step > 0 && __any_sync(0xffffffffu, move)) {
-                    // rows of this warp rescale what the products so far have added up (rows that did not move multiply by
-                    // one); the product of the step before is over, the next one waits for these weights
-#pragma unroll
-                    for (int cb = 0; cb < HD / 32; cb++) {
-                        float t[32];
-                        tmem_ld32(t_o + cb * 32, t);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 32; j++) t[j] *= corr;
-                        tmem_st32(t_o + cb * 32, t);
-                    }
-                }
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(&bar_p_full[x]);
+                l_run = l_run * corr + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) * per_sum;
+                buf += tiles;
+                if (buf >= SBUFS) { buf -= SBUFS; parity ^= 1u; }
             }
-            if (ok) ok = mbar_wait(&bar_o_full[x], 0, abort_flag, a.status, 10);
+            if (ok) ok = mbar_wait(&bar_pv[x], (unsigned)(step - 1) & 1u, abort_flag, a.status, 11);
             if (ok) {
                 tc_fence_after();
 #pragma unroll
@@ -522,8 +683,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(TMEM_COLS));
+    if (warp == 16)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(__shfl_sync(0xffffffffu, *tmem_at, 0)), "r"(TMEM_COLS));
 }
 
 }  // namespace
@@ -533,7 +694,7 @@ extern "C" int kllm_attention_q8_tcgen05_head_dim() { return HD; }
 // Requests' portions: rows q_start[s]..q_start[s+1] of request s start at cache position start_pos[s]; bfloat16 rows.  row_tiles:
 // tiles of 128 rows a CTA (1 or 2); splits: parts of the keys, with part_o float32 [n, heads, splits, HD] and part_ml
 // float32 [n, heads, splits, 2] where there are several.  status: a device int that a bounded wait which ran out sets (1, 7:
-// loader, 2-6: issuer, 8-10: softmax).
+// loader, 2-6: issuer, 8-11: softmax, 12: planner).
 extern "C" int kllm_attention_prefill_q8_tcgen05(void* out, float* part_o, float* part_ml, const void* q, int64_t q_stride,
                                                  const void* kcache, const void* vcache, const float* kscale,
                                                  const float* vscale, const int* q_start, const int* start_pos,

@@ -47,6 +47,23 @@ __device__ __forceinline__ void q8_to_f16x4(uint32_t four, uint32_t& lo, uint32_
     asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
         : "=r"(lo), "=r"(hi) : "r"(four));
 }
+// Loads of what the kernel does not write that stay where they are written: the compiler moves plain ones down to their
+// use, past the work that they were to overlap with.
+__device__ __forceinline__ int load_early(const int* p) {
+    int v;
+    asm volatile("ld.global.nc.b32 %0, [%1];\n" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float load_early(const float* p) {
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];\n" : "=f"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 load_early(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 // the nearest e4m3 numbers, ties to even; beyond +-448 they stay at it, NaN is NaN
 __device__ __forceinline__ uint32_t q8_pack2(float lo, float hi) {
     unsigned short r;
