@@ -1042,8 +1042,30 @@ Q8_MAX_PAGE = 4096
 Q8_MAX_GROUP = 64                     # query heads over one kv head
 
 
+_f32, _i32_t = torch.float32, torch.int32
+_q8_functions = {}                    # (entry point, head size) -> it and its library
+
+
+def _q8_function(library: str, name: str, head_dim: int = 0):
+    """(entry point, library) of a library of the cache in 8 bits, remembered."""
+    fn = _q8_functions.get((name, head_dim))
+    if fn is None:
+        lib = load_library(library, {"KLLM_HD": head_dim} if head_dim else None)
+        fn = _q8_functions[name, head_dim] = (getattr(lib, name), lib)
+    return fn
+
+
 def _check_q8(what, kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim):
-    """The stores, scales and table that the kernels of the cache in 8 bits share."""
+    """The stores, scales and table that the kernels of the cache in 8 bits share: one pass over what is usual (these calls
+    are short), then the reason where something is not."""
+    pages, heads, _, size = shape = kcache.shape if kcache.dim() == 4 else (0, 0, 0, 0)
+    cell = (pages, heads)
+    if (heads == n_kv and size == head_dim and n_kv > 0 and n_heads > 0 and n_heads % n_kv == 0 and size in Q8_HEAD_DIMS
+            and kcache.dtype is Q8_DTYPE and vcache.dtype is Q8_DTYPE and vcache.shape == shape and kscale.dtype is _f32
+            and vscale.dtype is _f32 and kscale.shape == cell and vscale.shape == cell and block_table.dtype is _i32_t
+            and block_table.dim() == 2 and kcache.is_contiguous() and vcache.is_contiguous() and kscale.is_contiguous()
+            and vscale.is_contiguous() and block_table.is_contiguous()):
+        return
     if kcache.dtype != Q8_DTYPE or vcache.dtype != Q8_DTYPE or not kcache.is_contiguous() or not vcache.is_contiguous():
         raise KernelError(f"{what}: the caches must be contiguous float8_e4m3fn tensors")
     if kcache.dim() != 4 or kcache.shape[1] != n_kv or kcache.shape[3] != head_dim or vcache.shape != kcache.shape:
@@ -1055,9 +1077,13 @@ def _check_q8(what, kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, 
         raise KernelError(f"{what}: head size {head_dim} is not a multiple of 32 up to 256")
     if n_kv <= 0 or n_heads <= 0 or n_heads % n_kv:
         raise KernelError(f"{what}: {n_heads} heads are not a multiple of {n_kv} kv heads")
-    if block_table.dim() != 2:
-        raise KernelError(f"{what}: the block table must be [requests, pages of a request]")
-    _i32(block_table, "block_table")
+    raise KernelError(f"{what}: the block table must be contiguous int32 [requests, pages of a request]")
+
+
+def _check_q8_ints(what, *tensors):
+    for t in tensors:
+        if t.dtype is not _i32_t or not t.is_contiguous():
+            raise KernelError(f"{what}: positions, requests and starts must be contiguous int32 tensors")
 
 
 def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_sin: Optional[torch.Tensor],
@@ -1080,36 +1106,55 @@ def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     or one behind the table of angles are neither rotated nor stored, those without a page not stored; rows behind the last
     request are left as they are.  No page may belong to two requests of a step."""
     _check_q8("rope_append_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
-    _i32(positions, "positions"); _i32(token_req, "token_req"); _i32(q_start, "q_start")
-    n = q.shape[0]
-    dt = q.dtype
-    dtype_code(dt)
-    if q_out.dtype != dt or k.dtype != dt or v.dtype != dt:
+    _check_q8_ints("rope_append_q8", positions, q_start)
+    dt, (n, width) = q.dtype, q.shape
+    code = dtype_code(dt)
+    if q_out.dtype is not dt or k.dtype is not dt or v.dtype is not dt:
         raise KernelError("rope_append_q8: q, k, v and q_out must have one dtype")
-    Q, K = n_heads * head_dim, n_kv * head_dim
-    if q.shape[1] != Q or q_out.shape != q.shape or k.shape != (n, K) or v.shape != (n, K):
+    rows = (n, n_kv * head_dim)
+    if width != n_heads * head_dim or q_out.shape != q.shape or k.shape != rows or v.shape != rows:
         raise KernelError("rope_append_q8: q and q_out [n, heads * head_dim], k and v [n, kv heads * head_dim]")
-    if q.stride(1) != 1 or q_out.stride(1) != 1 or k.stride(1) != 1 or v.stride(1) != 1:
+    (sq, dq), (so, do), (sk, dk), (sv, dv) = q.stride(), q_out.stride(), k.stride(), v.stride()
+    if dq != 1 or do != 1 or dk != 1 or dv != 1:
         raise KernelError("rope_append_q8: rows must be dense")
-    if kcache.shape[2] > Q8_MAX_PAGE:
-        raise KernelError(f"rope_append_q8: pages of {kcache.shape[2]} tokens, at most {Q8_MAX_PAGE}")
+    pages, _, page_size, _ = kcache.shape
+    if page_size > Q8_MAX_PAGE:
+        raise KernelError(f"rope_append_q8: pages of {page_size} tokens, at most {Q8_MAX_PAGE}")
     R = q_start.numel() - 1
-    if positions.numel() < n or R < 0 or block_table.shape[0] < R or (
-            token_req.numel() < n if token_req is not None else n > R):
+    requests, blocks = block_table.shape
+    if token_req is not None:
+        _check_q8_ints("rope_append_q8", token_req)
+    if positions.numel() < n or R < 0 or requests < R or (token_req.numel() < n if token_req is not None else n > R):
         raise KernelError("rope_append_q8: positions and token_req per token, a table row and a q_start per request "
                           "(token_req None: one token per request)")
     n_pos = rot = 0
     if cos_sin is not None:
         n_pos, rot = cos_sin.shape
-        if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or rot % 2 or rot > head_dim:
+        if cos_sin.dtype is not _f32 or not cos_sin.is_contiguous() or rot % 2 or rot > head_dim:
             raise KernelError("rope_append_q8: cos_sin must be contiguous float32 [positions, even rotary width <= head_dim]")
     _cuda(q_out, q, k, v, cos_sin, positions, token_req, q_start, block_table, kcache, vcache, kscale, vscale)
-    lib = load_library("cache_q8")
-    rc = lib.kllm_rope_append_q8(_p(q_out), q_out.stride(0), _p(q), q.stride(0), _p(k), k.stride(0), _p(v), v.stride(0),
-                                 _p(cos_sin), n_pos, _p(positions), _p(token_req), _p(q_start), R, _p(block_table),
-                                 block_table.shape[1], _p(kcache), _p(vcache), _p(kscale), _p(vscale), kcache.shape[0], n,
-                                 n_heads, n_kv, head_dim, rot, kcache.shape[2], dtype_code(dt), _stream())
+    fn, lib = _q8_function("cache_q8", "kllm_rope_append_q8")
+    rc = fn(q_out.data_ptr(), so, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _p(cos_sin), n_pos, positions.data_ptr(),
+            _p(token_req), q_start.data_ptr(), R, block_table.data_ptr(), blocks, kcache.data_ptr(), vcache.data_ptr(),
+            kscale.data_ptr(), vscale.data_ptr(), pages, n, n_heads, n_kv, head_dim, rot, page_size, code, _stream())
     _check(lib, "cache_q8", rc)
+
+
+@functools.lru_cache(maxsize=4096)
+def _decode_q8_parts(n_tokens, n_kv, group, head_dim, ctx_bound, wide, sms):
+    most = 16 if head_dim <= 128 else 8
+    subs = next(s for s in range(1, group + 1) if group % s == 0 and group // s <= most)
+    base = max(1, n_tokens * n_kv * subs)
+    blocks = max(1, -(-ctx_bound // 128))
+    wave = sms * (4 if head_dim <= 64 else 3 if head_dim <= 128 else 2) // base
+    square = (0.49 if head_dim <= 64 else 0.29) * (2 if wide else 1) * blocks * sms / base
+    cluster = 1
+    while cluster < 8 and 4 * cluster * cluster <= square and 2 * cluster <= min(blocks, wave):
+        cluster *= 2
+    ranges = 1
+    if cluster == 8 and square >= 24 * 24:
+        ranges = max(1, min(int(square ** 0.5) // 8, wave // 8, blocks // 32))
+    return ranges, cluster
 
 
 def decode_q8_parts(n_tokens: int, n_kv: int, group: int, head_dim: int, ctx_bound: int, wide: bool = False) -> tuple:
@@ -1125,27 +1170,16 @@ def decode_q8_parts(n_tokens: int, n_kv: int, group: int, head_dim: int, ctx_bou
     Up to eight parts are one cluster, which joins through distributed shared memory (1.5 us).  More parts are several ranges
     of such clusters, joined by a second kernel (2 us more): 1 x 4 of size 64 at 2048 8: 6.3, 16: 7.4; 1 x 8 of size 128 at
     131072 8: 109, 48: 53."""
-    most = 16 if head_dim <= 128 else 8
-    subs = next(s for s in range(1, group + 1) if group % s == 0 and group // s <= most)
-    base = max(1, n_tokens * n_kv * subs)
-    blocks = max(1, -(-ctx_bound // 128))
-    sms = sm_count()
-    wave = sms * (4 if head_dim <= 64 else 3 if head_dim <= 128 else 2) // base
-    square = (0.49 if head_dim <= 64 else 0.29) * (2 if wide else 1) * blocks * sms / base
-    cluster = 1
-    while cluster < 8 and 4 * cluster * cluster <= square and 2 * cluster <= min(blocks, wave):
-        cluster *= 2
-    ranges = 1
-    if cluster == 8 and square >= 24 * 24:
-        ranges = max(1, min(int(square ** 0.5) // 8, wave // 8, blocks // 32))
-    return ranges, cluster
+    return _decode_q8_parts(n_tokens, n_kv, group, head_dim, ctx_bound, wide, sm_count())
 
 
 def _check_q8_rows(what, out, q, n_heads, head_dim):
-    dtype_code(q.dtype)
-    if out.dtype != q.dtype or q.dim() != 2 or q.shape[1] != n_heads * head_dim or q.stride(1) != 1 or out.shape != q.shape \
-            or not out.is_contiguous():
+    """(dtype's code, rows, row stride)"""
+    dt, (n, width) = q.dtype, q.shape
+    stride, dense = q.stride()
+    if out.dtype is not dt or width != n_heads * head_dim or dense != 1 or out.shape != q.shape or not out.is_contiguous():
         raise KernelError(f"{what}: q [n, heads * head_dim] with dense rows, out contiguous of the same shape and dtype")
+    return dtype_code(dt), n, stride
 
 
 def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
@@ -1158,23 +1192,26 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
     no context is longer; it only decides into how many parts the contexts are cut.  Keys whose table entry names no page
     are not seen; a row that sees none (a negative position, say) becomes zeros."""
     _check_q8("attention_decode_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
-    _check_q8_rows("attention_decode_q8", out, q, n_heads, head_dim)
-    _i32(positions, "positions"); _i32(token_req, "token_req")
-    n, R = q.shape[0], block_table.shape[0]
+    code, n, stride = _check_q8_rows("attention_decode_q8", out, q, n_heads, head_dim)
+    _check_q8_ints("attention_decode_q8", positions)
+    if token_req is not None:
+        _check_q8_ints("attention_decode_q8", token_req)
+    R, blocks = block_table.shape
     if positions.numel() < n or (token_req.numel() < n if token_req is not None else R < n):
         raise KernelError("attention_decode_q8: a position (and a request) per token")
     _cuda(out, q, kcache, vcache, kscale, vscale, positions, token_req, block_table)
-    bound = min(int(ctx_bound), int(window)) if window and window > 0 else int(ctx_bound)
-    ranges, cluster = decode_q8_parts(n, n_kv, n_heads // n_kv, head_dim, bound, q.dtype == torch.float32)
+    bound = min(ctx_bound, window) if window and window > 0 else ctx_bound
+    ranges, cluster = decode_q8_parts(n, n_kv, n_heads // n_kv, head_dim, bound, code == 0)
     part_o = part_ml = None
     if ranges > 1:
-        part_o = torch.empty((n, n_heads, ranges, head_dim), dtype=torch.float32, device=q.device)
-        part_ml = torch.empty((n, n_heads, ranges, 2), dtype=torch.float32, device=q.device)
-    lib = load_library("attention_q8", {"KLLM_HD": head_dim})
-    rc = lib.kllm_attention_decode_q8(_p(out), _p(part_o), _p(part_ml), _p(q), q.stride(0), _p(kcache), _p(vcache), _p(kscale),
-                                      _p(vscale), _p(positions), _p(token_req), _p(block_table), block_table.shape[1],
-                                      kcache.shape[0], n, R, n_heads, n_kv, head_dim, kcache.shape[2], int(window or 0), scale,
-                                      ranges, cluster, dtype_code(q.dtype), _stream())
+        parts = torch.empty((n * n_heads * ranges, head_dim + 2), dtype=torch.float32, device=q.device)
+        part_o = parts.data_ptr()
+        part_ml = part_o + n * n_heads * ranges * head_dim * 4
+    pages, _, page_size, _ = kcache.shape
+    fn, lib = _q8_function("attention_q8", "kllm_attention_decode_q8", head_dim)
+    rc = fn(out.data_ptr(), part_o, part_ml, q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
+            vscale.data_ptr(), positions.data_ptr(), _p(token_req), block_table.data_ptr(), blocks, pages, n, R, n_heads, n_kv,
+            head_dim, page_size, window or 0, scale, ranges, cluster, code, _stream())
     _check(lib, "attention_q8", rc)
     global launches
     if ranges > 1:
@@ -1183,10 +1220,14 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
 
 def prefill_q8_parts(n_tokens: int, n_requests: int, n_kv: int, group: int, ctx_bound: int) -> tuple:
     """(row tiles of a CTA, parts of the keys) of the tcgen05 form of ``attention_prefill_q8``."""
-    sms = sm_count()
+    return _prefill_q8_parts(n_tokens, n_requests, n_kv, group, ctx_bound, sm_count())
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefill_q8_parts(n_tokens, n_requests, n_kv, group, ctx_bound, sms):
     per_tile = 128 // group
     ctas = (n_tokens // (2 * per_tile) + n_requests) * n_kv
-    splits = max(1, min(sms // ctas, -(-int(ctx_bound) // 128) // 4))
+    splits = max(1, min(sms // max(1, ctas), -(-ctx_bound // 128) // 4))
     return 2, splits
 
 
@@ -1198,35 +1239,38 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
     position start_pos[s]; their own keys are in the cache already.  Otherwise as ``attention_decode_q8``; rows that belong
     to no request are left as they are."""
     _check_q8("attention_prefill_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
-    _check_q8_rows("attention_prefill_q8", out, q, n_heads, head_dim)
-    _i32(q_start, "q_start"); _i32(start_pos, "start_pos")
-    R = int(n_requests)
-    if R < 0 or q_start.numel() < R + 1 or start_pos.numel() < R or block_table.shape[0] < R:
+    code, n, stride = _check_q8_rows("attention_prefill_q8", out, q, n_heads, head_dim)
+    _check_q8_ints("attention_prefill_q8", q_start, start_pos)
+    R = n_requests
+    requests, blocks = block_table.shape
+    if R < 0 or q_start.numel() < R + 1 or start_pos.numel() < R or requests < R:
         raise KernelError("attention_prefill_q8: q_start, start_pos and the block table must cover the requests")
     _cuda(out, q, kcache, vcache, kscale, vscale, q_start, start_pos, block_table)
-    n = q.shape[0]
-    if (q.dtype == torch.bfloat16 and head_dim in TCGEN05_HEAD_DIMS and USE_TCGEN05 and n_heads // n_kv <= 128
-            and out.data_ptr() % 16 == 0):
-        row_tiles, splits = prefill_q8_parts(n, R, n_kv, n_heads // n_kv, ctx_bound)
+    pages, _, page_size, _ = kcache.shape
+    group = n_heads // n_kv
+    if code == 1 and head_dim in TCGEN05_HEAD_DIMS and USE_TCGEN05 and group <= 128 and out.data_ptr() % 16 == 0:
+        row_tiles, splits = prefill_q8_parts(n, R, n_kv, group, ctx_bound)
         part_o = part_ml = None
         if splits > 1:
-            part_o = torch.empty((n, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
-            part_ml = torch.empty((n, n_heads, splits, 2), dtype=torch.float32, device=q.device)
-        lib = load_library("attention_q8_tcgen05", {"KLLM_HD": head_dim})
-        rc = lib.kllm_attention_prefill_q8_tcgen05(
-            _p(out), _p(part_o), _p(part_ml), _p(q), q.stride(0), _p(kcache), _p(vcache), _p(kscale), _p(vscale), _p(q_start),
-            _p(start_pos), _p(block_table), block_table.shape[1], kcache.shape[0], n, R, n_heads, n_kv, head_dim, kcache.shape[2],
-            int(window or 0), scale, row_tiles, splits, _p(status_word(q.device)), _stream())
+            parts = torch.empty((n * n_heads * splits, head_dim + 2), dtype=torch.float32, device=q.device)
+            part_o = parts.data_ptr()
+            part_ml = part_o + n * n_heads * splits * head_dim * 4
+        word = _status_words.get(q.device.index)
+        if word is None:
+            word = status_word(q.device)
+        fn, lib = _q8_function("attention_q8_tcgen05", "kllm_attention_prefill_q8_tcgen05", head_dim)
+        rc = fn(out.data_ptr(), part_o, part_ml, q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
+                vscale.data_ptr(), q_start.data_ptr(), start_pos.data_ptr(), block_table.data_ptr(), blocks, pages, n, R, n_heads,
+                n_kv, head_dim, page_size, window or 0, scale, row_tiles, splits, word.data_ptr(), _stream())
         _check(lib, "attention_q8_tcgen05", rc)
         global launches
         if splits > 1:
             launches += 1
         return
-    lib = load_library("attention_q8", {"KLLM_HD": head_dim})
-    rc = lib.kllm_attention_prefill_q8(_p(out), _p(q), q.stride(0), _p(kcache), _p(vcache), _p(kscale), _p(vscale), _p(q_start),
-                                       _p(start_pos), _p(block_table), block_table.shape[1], kcache.shape[0], q.shape[0], R,
-                                       n_heads, n_kv, head_dim, kcache.shape[2], int(window or 0), scale, dtype_code(q.dtype),
-                                       _stream())
+    fn, lib = _q8_function("attention_q8", "kllm_attention_prefill_q8", head_dim)
+    rc = fn(out.data_ptr(), q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(),
+            q_start.data_ptr(), start_pos.data_ptr(), block_table.data_ptr(), blocks, pages, n, R, n_heads, n_kv, head_dim,
+            page_size, window or 0, scale, code, _stream())
     _check(lib, "attention_q8", rc)
 
 
