@@ -9,19 +9,24 @@
 // The rotation is that of rope.cu: rotate_half, float32, angles from a table computed in float64.  A key is rounded once,
 // from the rotated float32 numbers to e4m3.
 //
-// One CTA takes (a few tokens, one kv head): it rotates the query heads of that kv head's group for its tokens, and stores
-// whole runs of rows: the first token of a request's rows in a page (the request's first token of the step, or slot 0)
-// does it for all of them, so that exactly one CTA touches a (page, kv head) and its scale.  Each run is read twice, the
-// second time from the first-level cache: once for the rows' largest magnitudes (integer maxima in shared memory: the order does
-// not matter), once to store.
+// What bounds it: bytes, and for few tokens a chain of dependent loads.  A CTA takes a few tokens and one of two jobs: it
+// rotates some of their query heads, or it stores whole runs of rows of some kv heads: the first token of a request's rows in a
+// page (the request's first token of the step, or slot 0) does it for all of them, so that exactly one CTA touches a (page,
+// kv head) and its scale.  A thread keeps its place in the rows and walks the rows, without a division per unit.  A run is
+// read twice, the second time from the first-level cache: once for the largest magnitudes (integer maxima in shared memory:
+// their order does not matter), once to store.  Rows that are not finite are rare: they are marked on the first way, and only
+// where there are any the maxima are taken again without them.
 #include "q8.cuh"
 
 KLLM_EXPORT_LAST_ERROR(cache_q8)
 
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kMaxPage = 4096;              // two words of shared memory per row of a run
+constexpr int kThreads = 256;
+constexpr int kChunk = 16;                  // tokens a CTA looks after
+constexpr int kMaxHeads = 16;               // kv heads a CTA stores at most
+constexpr int kMaxMarks = 32768;            // rows of a run x kv heads: a byte each
+constexpr int kMaxPage = 4096;
 
 template <typename T, int U> __device__ __forceinline__ void load(const T* p, float (&v)[U]) {
     if constexpr (U == 1) {
@@ -47,7 +52,7 @@ template <typename T, int U> __device__ __forceinline__ void store(T* p, const f
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     }
 }
-template <int U> __device__ __forceinline__ void store8(uint8_t* p, const float (&v)[U], float mul) {
+template <int U> __device__ __forceinline__ void store8(uint8_t* p, const float* v, float mul) {
     if constexpr (U == 1) *p = (uint8_t)(q8_pack2(v[0] * mul, 0.f) & 0xff);
     else *reinterpret_cast<uint32_t*>(p) = q8_pack2(v[0] * mul, v[1] * mul) | (q8_pack2(v[2] * mul, v[3] * mul) << 16);
 }
@@ -55,174 +60,204 @@ template <int U> __device__ __forceinline__ void fill8(uint8_t* p, uint32_t byte
     if constexpr (U == 1) *p = (uint8_t)byte;
     else *reinterpret_cast<uint32_t*>(p) = byte * 0x01010101u;
 }
-template <int U> __device__ __forceinline__ int largest(const float (&v)[U]) {
-    int m = 0;
-#pragma unroll
-    for (int i = 0; i < U; i++) m = max(m, __float_as_int(v[i]) & 0x7fffffff);
-    return m;
-}
 
-// a[], b[]: U numbers of a row at j and U at j + half, turned by the angles of the row's position
-template <typename T, int U>
-__device__ __forceinline__ void turn(const T* row, const float* cs, int j, int half, float (&a)[U], float (&b)[U]) {
-    float c[U], s[U], x[U], y[U];
-    load<T, U>(row + j, x);
-    load<T, U>(row + j + half, y);
-    load<float, U>(cs + j, c);
-    load<float, U>(cs + half + j, s);
+// A unit of a row is 2 U numbers: v[0 .. U) from place `at`, v[U .. 2U) from `at2`.  Units below `pairs` are the two halves of
+// U rotated pairs, the others 2 U neighbours.
+struct Unit {
+    int at, at2;
+};
+template <int U> __device__ __forceinline__ Unit unit_of(int i, int pairs, int half, int rot) {
+    if (i < pairs) return Unit{i * U, i * U + half};
+    const int at = rot + (i - pairs) * 2 * U;
+    return Unit{at, at + U};
+}
+struct Run {                                // rows of one request in one page that this step stores
+    int token, page, slot, rows;
+};
+template <typename T, int U> struct Raw {   // a unit as it is read, with its angles
+    float x[U], y[U], c[U], s[U];
+};
+template <typename T, int U> __device__ __forceinline__ void read_unit(Raw<T, U>& w, const T* row, Unit u, bool turned, const float* cs, int half) {
+    load<T, U>(row + u.at, w.x);
+    load<T, U>(row + u.at2, w.y);
+    if (turned) {
+        load<float, U>(cs + u.at, w.c);
+        load<float, U>(cs + half + u.at, w.s);
+    }
+}
+template <typename T, int U> __device__ __forceinline__ void turn(const Raw<T, U>& w, bool turned, float (&v)[2 * U]) {
 #pragma unroll
     for (int i = 0; i < U; i++) {
-        a[i] = x[i] * c[i] - y[i] * s[i];
-        b[i] = y[i] * c[i] + x[i] * s[i];
+        v[i] = turned ? w.x[i] * w.c[i] - w.y[i] * w.s[i] : w.x[i];
+        v[U + i] = turned ? w.y[i] * w.c[i] + w.x[i] * w.s[i] : w.y[i];
     }
 }
 
-// U numbers at a time: 4 where half the rotary width, strides and addresses allow it, else 1
+// U = 4 where half the rotary width, strides and addresses allow it, else 1
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride, const T* __restrict__ k,
                       int64_t k_stride, const T* __restrict__ v, int64_t v_stride, const float* __restrict__ cos_sin, int n_pos,
                       const int* __restrict__ positions, const int* __restrict__ token_req, const int* __restrict__ q_start,
                       int n_requests, const int* __restrict__ block_table, int max_blocks, uint8_t* __restrict__ kcache,
                       uint8_t* __restrict__ vcache, float* __restrict__ kscale, float* __restrict__ vscale, int n_pages,
-                      int n_tokens, int group, int n_kv, int hd, int rot, int page_size, int chunk) {
-    extern __shared__ int row_max[];          // [2][rows of the run]: the largest magnitude's bits of keys, of values
-    __shared__ int s_max[2];
+                      int n_tokens, int n_heads, int q_heads, int n_kv, int kv_heads, int hd, int rot, int page_size, int chunk) {
+    extern __shared__ uint8_t bad[];          // [rows of the run][kv heads]: an infinity or NaN in the key or the value
+    __shared__ int s_max[kMaxHeads][2], s_pos[kChunk], s_req[kChunk], s_runs, s_any;
+    __shared__ Run s_run[kChunk];
     griddep_wait();
     griddep_launch();
-    const int tid = threadIdx.x, g = blockIdx.y;
+    const int tid = threadIdx.x, threads = blockDim.x, kv_ctas = (n_kv + kv_heads - 1) / kv_heads;
     const int n_all = min(n_tokens, q_start[n_requests]);          // rows behind the last request are left alone
     const int t0 = blockIdx.x * chunk, t1 = min(n_all, t0 + chunk);
-    const int half = rot >> 1;
-    const int pairs = half / U, tail = (hd - rot) / U;             // units of a row
+    if (t0 >= t1) return;
+    if (tid < t1 - t0) {
+        s_pos[tid] = positions[t0 + tid];
+        s_req[tid] = token_req ? token_req[t0 + tid] : t0 + tid;
+    }
+    const int half = rot >> 1, pairs = half / U, per_row = hd / (2 * U);     // units of a row
+    __syncthreads();
 
-    // queries of this kv head's group
-    const int per_head = pairs + (q_out != q ? tail : 0);
-    if (per_head > 0) {
-        for (int u = tid; u < (t1 - t0) * group * per_head; u += kThreads) {
-            const int i = u % per_head, th = u / per_head;
-            const int t = t0 + th / group, h = g * group + th % group;
-            const int p = positions[t];
-            const T* src = q + (int64_t)t * q_stride + (int64_t)h * hd;
-            T* dst = q_out + (int64_t)t * qo_stride + (int64_t)h * hd;
-            if (i < pairs) {
-                if (p < 0 || p >= n_pos) continue;
-                float a[U], b[U];
-                turn<T, U>(src, cos_sin + (int64_t)p * rot, i * U, half, a, b);
-                store<T, U>(dst + i * U, a);
-                store<T, U>(dst + half + i * U, b);
-            } else {
-                float a[U];
-                load<T, U>(src + rot + (i - pairs) * U, a);
-                store<T, U>(dst + rot + (i - pairs) * U, a);
+    if ((int)blockIdx.y >= kv_ctas) {
+        // queries: a CTA's share of the heads, in place only the pairs
+        const int per_head = q_out != q ? per_row : pairs, h0 = ((int)blockIdx.y - kv_ctas) * q_heads;
+        const int cols = min(q_heads, n_heads - h0) * per_head;
+        const int together = max(1, threads / cols);                // tokens at a time
+        for (int c0 = 0; c0 < cols; c0 += threads) {
+            const int first = cols <= threads ? tid / cols : 0, c = cols <= threads ? tid - first * cols : c0 + tid;
+            if (first >= together || c >= cols) continue;
+            const int h = c / per_head, i = c - h * per_head;
+            const Unit unit = unit_of<U>(i, pairs, half, rot);
+            const bool turned = i < pairs;
+            const T* src = q + (int64_t)(h0 + h) * hd;
+            T* dst = q_out + (int64_t)(h0 + h) * hd;
+#pragma unroll 2
+            for (int t = first; t < t1 - t0; t += together) {
+                const int p = s_pos[t];
+                if (turned && (p < 0 || p >= n_pos)) continue;
+                Raw<T, U> w;
+                float x[2 * U];
+                read_unit<T, U>(w, src + (int64_t)(t0 + t) * q_stride, unit, turned, cos_sin + (int64_t)p * rot, half);
+                turn<T, U>(w, turned, x);
+                T* to = dst + (int64_t)(t0 + t) * qo_stride;
+                store<T, U>(to + unit.at, *reinterpret_cast<const float(*)[U]>(x));
+                store<T, U>(to + unit.at2, *reinterpret_cast<const float(*)[U]>(x + U));
             }
         }
+        return;
     }
 
-    // runs of rows that begin among these tokens
-    for (int t = t0; t < t1; t++) {
-        const int req = token_req ? token_req[t] : t;
-        if (req < 0 || req >= n_requests) continue;
-        const int p = positions[t], begin = q_start[req], end = min(q_start[req + 1], n_all);
-        if (p < 0 || (rot > 0 && p >= n_pos)) continue;
-        const int lp = p / page_size, slot = p - lp * page_size;
-        if ((slot != 0 && t != begin) || lp >= max_blocks) continue;
-        const int page = block_table[(int64_t)req * max_blocks + lp];
-        if (page < 0 || page >= n_pages) continue;
-        int rows = min(end - t, page_size - slot);
-        if (rot > 0) rows = min(rows, n_pos - p);
-        if (rows <= 0) continue;
-        int* kmax = row_max;
-        int* vmax = row_max + rows;
-        const int64_t cell = (int64_t)page * n_kv + g;
-        // read before the meetings below: thread 0 stores the new scales behind them
-        const int ke_old = slot ? q8_exponent(kscale[cell]) : Q8_E_MIN, ve_old = slot ? q8_exponent(vscale[cell]) : Q8_E_MIN;
-        __syncthreads();                                          // the run before is done with the maxima
-        for (int r = tid; r < 2 * rows; r += kThreads) row_max[r] = 0;
-        if (tid < 2) s_max[tid] = 0;
-        __syncthreads();
-        const int k_units = pairs + tail, v_units = hd / U, units = k_units + v_units;
-        const T* k0 = k + (int64_t)t * k_stride + (int64_t)g * hd;
-        const T* v0 = v + (int64_t)t * v_stride + (int64_t)g * hd;
-        const float* cs0 = cos_sin + (int64_t)p * rot;
-        for (int u = tid; u < rows * units; u += kThreads) {
-            const int r = u / units, i = u - r * units;
-            float a[U];
-            if (i < pairs) {
-                float b[U];
-                turn<T, U>(k0 + r * k_stride, cs0 + (int64_t)r * rot, i * U, half, a, b);
-                atomicMax(&kmax[r], max(largest<U>(a), largest<U>(b)));
-            } else if (i < k_units) {
-                load<T, U>(k0 + r * k_stride + rot + (i - pairs) * U, a);
-                atomicMax(&kmax[r], largest<U>(a));
-            } else {
-                load<T, U>(v0 + r * v_stride + (i - k_units) * U, a);
-                atomicMax(&vmax[r], largest<U>(a));
+    const int g0 = blockIdx.y * kv_heads, heads = min(kv_heads, n_kv - g0);
+    const int units = 2 * per_row, cols = heads * units;            // a head's key, then its value
+    const int together = threads / cols, first = tid / cols, col = tid - first * cols, h = col / units, i = col - h * units;
+    const bool key = i < per_row, turned = i < pairs, mine = first < together;
+    const Unit unit = key ? unit_of<U>(i, pairs, half, rot) : unit_of<U>(i - per_row, 0, 0, 0);
+    const T* src = (key ? k : v) + (int64_t)(g0 + h) * hd;
+    const int64_t src_stride = key ? k_stride : v_stride;
+    // runs of rows that begin among these tokens: found by a thread per token
+    if (tid < 32) {
+        int page = -1, slot = 0, rows = 0;
+        if (tid < t1 - t0) {
+            const int req = s_req[tid], p = s_pos[tid], t = t0 + tid;
+            if (req >= 0 && req < n_requests && p >= 0 && (rot == 0 || p < n_pos)) {
+                const int lp = p / page_size, begin = q_start[req], end = min(q_start[req + 1], n_all);
+                slot = p - lp * page_size;
+                if ((slot == 0 || t == begin) && lp < max_blocks) page = block_table[(int64_t)req * max_blocks + lp];
+                rows = min(end - t, page_size - slot);
+                if (rot > 0) rows = min(rows, n_pos - p);
             }
         }
+        const bool run = page >= 0 && page < n_pages && rows > 0;
+        const unsigned runs = __ballot_sync(0xffffffffu, run);
+        if (run) s_run[__popc(runs & ((1u << tid) - 1))] = Run{tid, page, slot, rows};
+        if (tid == 0) s_runs = __popc(runs);
+    }
+    __syncthreads();
+    for (int n = 0; n < s_runs; n++) {
+        const int t = t0 + s_run[n].token, p = s_pos[s_run[n].token], page = s_run[n].page, slot = s_run[n].slot, rows = s_run[n].rows;
+        const int64_t cell0 = (int64_t)page * n_kv + g0, cell = cell0 + h;
+        // read before the meetings below: the new scales are stored behind them
+        const int ke_old = slot ? q8_exponent(kscale[cell]) : Q8_E_MIN, ve_old = slot ? q8_exponent(vscale[cell]) : Q8_E_MIN;
+        const T* row0 = src + (int64_t)t * src_stride;
+        const float* cs0 = cos_sin + (int64_t)p * rot;
+        auto read = [&](int r, float (&x)[2 * U]) {
+            Raw<T, U> w;
+            read_unit<T, U>(w, row0 + (int64_t)r * src_stride, unit, turned, cs0 + (int64_t)r * rot, half);
+            turn<T, U>(w, turned, x);
+        };
+        __syncthreads();                                            // the run before is done with the marks and the maxima
+        for (int j = tid; j < rows * heads; j += threads) bad[j] = 0;
+        if (tid < 2 * kMaxHeads) s_max[tid >> 1][tid & 1] = 0;
+        if (tid == 0) s_any = 0;
         __syncthreads();
-        for (int r = tid; r < rows; r += kThreads) {
-            const int a = kmax[r], b = vmax[r];
-            if (max(a, b) >= 0x7f800000) kmax[r] = -1;            // an infinity or NaN in the key or the value
-            else { atomicMax(&s_max[0], a); atomicMax(&s_max[1], b); }
-        }
-        __syncthreads();
-        const int ke = max(ke_old, q8_exponent_for(s_max[0])), ve = max(ve_old, q8_exponent_for(s_max[1]));
-        uint8_t* kp = kcache + cell * page_size * hd;
-        uint8_t* vp = vcache + cell * page_size * hd;
-        // rows that the page holds already
+        int m = 0;
+#pragma unroll 4
+        for (int r = first; mine && r < rows; r += together) {
+            float x[2 * U];
+            read(r, x);
+            int mr = 0;
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-            const int e = w ? ve : ke, e_old = w ? ve_old : ke_old;
-            if (!slot || e == e_old) continue;
-            uint32_t* c = reinterpret_cast<uint32_t*>(w ? vp : kp);
-            const float mul = q8_pow2(max(e_old - e, -126));
-            for (int u = tid; u < slot * hd / 4; u += kThreads) {
-                const uint32_t x = c[u];
-                const uint32_t lo = q8_to_f16x2(x & 0xffffu), hi = q8_to_f16x2(x >> 16);
-                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-                const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                c[u] = q8_pack2(a.x * mul, a.y * mul) | (q8_pack2(b.x * mul, b.y * mul) << 16);
+            for (int j = 0; j < 2 * U; j++) mr = max(mr, __float_as_int(x[j]) & 0x7fffffff);
+            if (mr >= 0x7f800000) { bad[r * heads + h] = 1; s_any = 1; }
+            else m = max(m, mr);
+        }
+        if (mine) atomicMax(&s_max[h][key], m);
+        __syncthreads();
+        const bool any = s_any != 0;
+        if (any) {                                                  // the same for all threads
+            __syncthreads();
+            if (tid < 2 * kMaxHeads) s_max[tid >> 1][tid & 1] = 0;
+            __syncthreads();
+            m = 0;
+            for (int r = first; mine && r < rows; r += together) {
+                if (bad[r * heads + h]) continue;
+                float x[2 * U];
+                read(r, x);
+#pragma unroll
+                for (int j = 0; j < 2 * U; j++) m = max(m, __float_as_int(x[j]) & 0x7fffffff);
+            }
+            if (mine) atomicMax(&s_max[h][key], m);
+            __syncthreads();
+        }
+        const int ke = max(ke_old, q8_exponent_for(s_max[h][1])), ve = max(ve_old, q8_exponent_for(s_max[h][0]));
+        uint8_t* page_rows = (key ? kcache : vcache) + cell * page_size * hd;
+        const int e = key ? ke : ve, e_old = key ? ke_old : ve_old;
+        // rows that the page holds already
+        if (mine && slot && e != e_old) {
+            const float down = q8_pow2(max(e_old - e, -126));
+            for (int r = first; r < slot; r += together) {
+                uint8_t* at[2] = {page_rows + (int64_t)r * hd + unit.at, page_rows + (int64_t)r * hd + unit.at2};
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if constexpr (U == 1) {
+                        const uint32_t lo = q8_to_f16x2(*at[j]);
+                        *at[j] = (uint8_t)(q8_pack2(__half22float2(*reinterpret_cast<const __half2*>(&lo)).x * down, 0.f) & 0xff);
+                    } else {
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(at[j]);
+                        uint32_t lo, hi;
+                        q8_to_f16x4(x, lo, hi);
+                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                        *reinterpret_cast<uint32_t*>(at[j]) = q8_pack2(a.x * down, a.y * down) | (q8_pack2(b.x * down, b.y * down) << 16);
+                    }
+                }
             }
         }
         // the new rows
-        const float kmul = q8_pow2(-ke), vmul = q8_pow2(-ve);
-        kp += (int64_t)slot * hd;
-        vp += (int64_t)slot * hd;
-        for (int u = tid; u < rows * units; u += kThreads) {
-            const int r = u / units, i = u - r * units;
-            const bool bad = kmax[r] < 0;
-            float a[U];
-            if (i < pairs) {
-                uint8_t* dst = kp + (int64_t)r * hd + i * U;
-                if (bad) {
-                    fill8<U>(dst, 0x7f);
-                    fill8<U>(dst + half, 0x7f);
-                } else {
-                    float b[U];
-                    turn<T, U>(k0 + r * k_stride, cs0 + (int64_t)r * rot, i * U, half, a, b);
-                    store8<U>(dst, a, kmul);
-                    store8<U>(dst + half, b, kmul);
-                }
-            } else if (i < k_units) {
-                const int d = rot + (i - pairs) * U;
-                if (bad) {
-                    fill8<U>(kp + (int64_t)r * hd + d, 0x7f);
-                } else {
-                    load<T, U>(k0 + r * k_stride + d, a);
-                    store8<U>(kp + (int64_t)r * hd + d, a, kmul);
-                }
-            } else {
-                const int d = (i - k_units) * U;
-                if (bad) {
-                    fill8<U>(vp + (int64_t)r * hd + d, 0);
-                } else {
-                    load<T, U>(v0 + r * v_stride + d, a);
-                    store8<U>(vp + (int64_t)r * hd + d, a, vmul);
-                }
+        const float mul = q8_pow2(-e);
+#pragma unroll 4
+        for (int r = first; mine && r < rows; r += together) {
+            uint8_t* dst = page_rows + (int64_t)(slot + r) * hd;
+            if (any && bad[r * heads + h]) {
+                fill8<U>(dst + unit.at, key ? 0x7f : 0);
+                fill8<U>(dst + unit.at2, key ? 0x7f : 0);
+                continue;
             }
+            float x[2 * U];
+            read(r, x);
+            store8<U>(dst + unit.at, x, mul);
+            store8<U>(dst + unit.at2, x + U, mul);
         }
-        if (tid == 0) {
+        if (first == 0 && i == 0) {
             kscale[cell] = q8_pow2(ke);
             vscale[cell] = q8_pow2(ve);
         }
@@ -230,8 +265,8 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
 }
 
 template <typename T, int U, typename... A>
-void launch(dim3 grid, size_t smem, cudaStream_t s, A... a) {
-    kllm_launch((rope_append_q8_kernel<T, U>), grid, dim3(kThreads), smem, s, a...);
+void launch(dim3 grid, int threads, size_t smem, cudaStream_t s, A... a) {
+    kllm_launch((rope_append_q8_kernel<T, U>), grid, dim3(threads), smem, s, a...);
 }
 
 }  // namespace
@@ -254,19 +289,34 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     if (n_kv > 65535) KLLM_FAIL("append (8 bits): %d kv heads, at most 65535", n_kv);
     if (dtype != KLLM_F32 && dtype != KLLM_BF16) KLLM_FAIL("append (8 bits): element type %d", dtype);
     const int es = dtype == KLLM_F32 ? 4 : 2;
-    // one CTA a token where every request brings one, else 16 tokens a CTA
-    const int chunk = n_tokens <= n_requests ? 1 : 16;
-    const dim3 grid((n_tokens + chunk - 1) / chunk, n_kv);
-    const size_t smem = (size_t)2 * 4 * (page_size < n_tokens ? page_size : n_tokens);
     const bool four = rot % 8 == 0 && !((qo_stride | q_stride | k_stride | v_stride) & 3) &&
                       !(((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & (4 * es - 1)) &&
                       !((uintptr_t)cos_sin & 15) && !(((uintptr_t)kcache | (uintptr_t)vcache) & 3);
+    // A CTA a token where every request brings one, else one for sixteen.  kv heads a CTA: as many as its threads cover, as long
+    // as there are runs enough for two CTAs an SM.
+    const int chunk = n_tokens <= n_requests ? 1 : kChunk;
+    const int units = four ? hd / 4 : hd;      // of a head's key and value
+    const int run = page_size < n_tokens ? page_size : n_tokens;
+    const int64_t runs = chunk == 1 ? n_tokens : (int64_t)n_tokens / page_size + n_requests;
+    int kv_heads = kThreads / units < kMaxHeads ? kThreads / units : kMaxHeads;
+    if (kv_heads > runs * n_kv / 296) kv_heads = (int)(runs * n_kv / 296);
+    if (kv_heads > kMaxMarks / run) kv_heads = kMaxMarks / run;
+    if (kv_heads < 1) kv_heads = 1;
+    if (kv_heads > n_kv) kv_heads = n_kv;
+    // threads for the longest run, as many query heads a CTA as they cover
+    int threads = 64;
+    while (threads < kv_heads * units || (threads < kThreads && threads < (chunk == 1 ? 1 : run) * kv_heads * units)) threads *= 2;
+    const int q_heads = threads / (units / 2);
+    const int kv_ctas = (n_kv + kv_heads - 1) / kv_heads, q_ctas = rot > 0 || q_out != q ? (n_heads + q_heads - 1) / q_heads : 0;
+    if (kv_ctas + q_ctas > 65535) KLLM_FAIL("append (8 bits): %d heads over %d kv heads", n_heads, n_kv);
+    const dim3 grid((n_tokens + chunk - 1) / chunk, kv_ctas + q_ctas);
+    const size_t smem = (size_t)run * kv_heads;
     if (((uintptr_t)kcache | (uintptr_t)vcache) & 3) KLLM_FAIL("append (8 bits): the caches must be 4-byte aligned");
     const cudaStream_t s = (cudaStream_t)stream;
 #define KLLM_GO(T, U)                                                                                                        \
-    launch<T, U>(grid, smem, s, (T*)q_out, qo_stride, (const T*)q, q_stride, (const T*)k, k_stride, (const T*)v, v_stride,  \
+    launch<T, U>(grid, threads, smem, s, (T*)q_out, qo_stride, (const T*)q, q_stride, (const T*)k, k_stride, (const T*)v, v_stride,  \
                  cos_sin, n_pos, positions, token_req, q_start, n_requests, block_table, max_blocks, (uint8_t*)kcache,      \
-                 (uint8_t*)vcache, kscale, vscale, n_pages, n_tokens, n_heads / n_kv, n_kv, hd, rot, page_size, chunk)
+                 (uint8_t*)vcache, kscale, vscale, n_pages, n_tokens, n_heads, q_heads, n_kv, kv_heads, hd, rot, page_size, chunk)
     if (dtype == KLLM_F32) {
         if (four) KLLM_GO(float, 4); else KLLM_GO(float, 1);
     } else {
