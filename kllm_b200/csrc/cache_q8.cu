@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 16;                  // tokens a CTA looks after
+constexpr int kBatch = 4;                   // query heads whose numbers a thread requests together
 constexpr int kMaxHeads = 16;               // kv heads a CTA stores at most
 constexpr int kMaxMarks = 32768;            // rows of a run x kv heads: a byte each
 constexpr int kMaxPage = 4096;
@@ -95,7 +96,7 @@ template <typename T, int U> __device__ __forceinline__ void turn(const Raw<T, U
 
 // U = 4 where half the rotary width, strides and addresses allow it, else 1
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
 rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride, const T* __restrict__ k,
                       int64_t k_stride, const T* __restrict__ v, int64_t v_stride, const float* __restrict__ cos_sin, int n_pos,
                       const int* __restrict__ positions, const int* __restrict__ token_req, const int* __restrict__ q_start,
@@ -119,29 +120,44 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
     __syncthreads();
 
     if ((int)blockIdx.y >= kv_ctas) {
-        // queries: a CTA's share of the heads, in place only the pairs
-        const int per_head = q_out != q ? per_row : pairs, h0 = ((int)blockIdx.y - kv_ctas) * q_heads;
-        const int cols = min(q_heads, n_heads - h0) * per_head;
-        const int together = max(1, threads / cols);                // tokens at a time
-        for (int c0 = 0; c0 < cols; c0 += threads) {
-            const int first = cols <= threads ? tid / cols : 0, c = cols <= threads ? tid - first * cols : c0 + tid;
-            if (first >= together || c >= cols) continue;
-            const int h = c / per_head, i = c - h * per_head;
+        // queries: a CTA's share of the heads, in place only the pairs.  A thread keeps (token, place in the head), for which it
+        // reads the angles once, and walks the heads.
+        const int per_head = q_out != q ? per_row : pairs, h0 = ((int)blockIdx.y - kv_ctas) * q_heads, h1 = min(h0 + q_heads, n_heads);
+        const int places = chunk * per_head, together = max(1, threads / places);        // heads at a time
+        for (int c0 = 0; c0 < places; c0 += threads) {
+            const int first = places <= threads ? tid / places : 0, c = places <= threads ? tid - first * places : c0 + tid;
+            const int t = c / per_head, i = c - t * per_head;
+            if (first >= together || t >= t1 - t0) continue;
             const Unit unit = unit_of<U>(i, pairs, half, rot);
             const bool turned = i < pairs;
-            const T* src = q + (int64_t)(h0 + h) * hd;
-            T* dst = q_out + (int64_t)(h0 + h) * hd;
-#pragma unroll 2
-            for (int t = first; t < t1 - t0; t += together) {
-                const int p = s_pos[t];
-                if (turned && (p < 0 || p >= n_pos)) continue;
-                Raw<T, U> w;
-                float x[2 * U];
-                read_unit<T, U>(w, src + (int64_t)(t0 + t) * q_stride, unit, turned, cos_sin + (int64_t)p * rot, half);
-                turn<T, U>(w, turned, x);
-                T* to = dst + (int64_t)(t0 + t) * qo_stride;
-                store<T, U>(to + unit.at, *reinterpret_cast<const float(*)[U]>(x));
-                store<T, U>(to + unit.at2, *reinterpret_cast<const float(*)[U]>(x + U));
+            const int p = s_pos[t];
+            if (turned && (p < 0 || p >= n_pos)) continue;
+            Raw<T, U> w;
+            if (turned) {
+                load<float, U>(cos_sin + (int64_t)p * rot + unit.at, w.c);
+                load<float, U>(cos_sin + (int64_t)p * rot + half + unit.at, w.s);
+            }
+            const T* src = q + (int64_t)(t0 + t) * q_stride;
+            T* dst = q_out + (int64_t)(t0 + t) * qo_stride;
+            for (int h = h0 + first; h < h1; h += kBatch * together) {
+                float x[kBatch][U], y[kBatch][U];
+#pragma unroll
+                for (int j = 0; j < kBatch; j++)
+                    if (h + j * together < h1) {
+                        load<T, U>(src + (int64_t)(h + j * together) * hd + unit.at, x[j]);
+                        load<T, U>(src + (int64_t)(h + j * together) * hd + unit.at2, y[j]);
+                    }
+#pragma unroll
+                for (int j = 0; j < kBatch; j++)
+                    if (h + j * together < h1) {
+                        float z[2 * U];
+#pragma unroll
+                        for (int l = 0; l < U; l++) { w.x[l] = x[j][l]; w.y[l] = y[j][l]; }
+                        turn<T, U>(w, turned, z);
+                        T* to = dst + (int64_t)(h + j * together) * hd;
+                        store<T, U>(to + unit.at, *reinterpret_cast<const float(*)[U]>(z));
+                        store<T, U>(to + unit.at2, *reinterpret_cast<const float(*)[U]>(z + U));
+                    }
             }
         }
         return;
@@ -303,13 +319,16 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     if (kv_heads > kMaxMarks / run) kv_heads = kMaxMarks / run;
     if (kv_heads < 1) kv_heads = 1;
     if (kv_heads > n_kv) kv_heads = n_kv;
-    // threads for the longest run, as many query heads a CTA as they cover
+    // threads for the longest run
     int threads = 64;
     while (threads < kv_heads * units || (threads < kThreads && threads < (chunk == 1 ? 1 : run) * kv_heads * units)) threads *= 2;
-    const int q_heads = threads / (units / 2);
+    // query heads a CTA: a batch for every thread, as long as that leaves two CTAs an SM
+    const int chunks = (n_tokens + chunk - 1) / chunk;
+    int q_heads = kBatch * (threads / (chunk * (units / 2)) > 0 ? threads / (chunk * (units / 2)) : 1);
+    while (q_heads > 1 && (int64_t)chunks * ((n_heads + q_heads - 1) / q_heads) < 296) q_heads /= 2;
     const int kv_ctas = (n_kv + kv_heads - 1) / kv_heads, q_ctas = rot > 0 || q_out != q ? (n_heads + q_heads - 1) / q_heads : 0;
     if (kv_ctas + q_ctas > 65535) KLLM_FAIL("append (8 bits): %d heads over %d kv heads", n_heads, n_kv);
-    const dim3 grid((n_tokens + chunk - 1) / chunk, kv_ctas + q_ctas);
+    const dim3 grid(chunks, kv_ctas + q_ctas);
     const size_t smem = (size_t)run * kv_heads;
     if (((uintptr_t)kcache | (uintptr_t)vcache) & 3) KLLM_FAIL("append (8 bits): the caches must be 4-byte aligned");
     const cudaStream_t s = (cudaStream_t)stream;
