@@ -57,6 +57,7 @@ constexpr int Q_BYTES = PANELS * PANEL;    // per row tile
 constexpr int KV_BYTES = PANELS * PANEL;   // keys or values of a tile
 constexpr int STAGES = HD == 64 ? 3 : 2;
 constexpr int SBUFS = HD == 64 ? 3 : 2;    // score buffers in TMEM, 128 columns each: taken in turn by the row tiles' steps
+constexpr int PARTS = SBUFS == 2 ? 2 : 1;   // parts in which a job's weights are handed over: where the next scores wait for its product
 constexpr int PLANS = 4;                   // steps that the planner is ahead of the loader
 constexpr int NOTES = 16;                  // steps described at a time; see Note
 constexpr int SMEM_BYTES = 1024 + 2 * Q_BYTES + STAGES * 2 * KV_BYTES;
@@ -182,7 +183,7 @@ struct Args {
 __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const Args a) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t bar_k_full[STAGES], bar_k_empty[STAGES], bar_v_full[STAGES], bar_v_empty[STAGES];
-    __shared__ __align__(8) uint64_t bar_q_full[2], bar_s_full[SBUFS], bar_p_full[SBUFS][2], bar_pv[2], bar_note[NOTES];
+    __shared__ __align__(8) uint64_t bar_q_full[2], bar_s_full[SBUFS], bar_p_full[SBUFS][PARTS], bar_pv[2], bar_note[NOTES];
     __shared__ __align__(8) uint64_t bar_plan_full[PLANS], bar_plan_empty[PLANS];
     __shared__ Note s_note[NOTES];
     __shared__ Plan s_plan[PLANS];
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
         }
         for (int i = 0; i < SBUFS; i++) {
             mbar_init(&bar_s_full[i], 1);
-            mbar_init(&bar_p_full[i][0], ROWS); mbar_init(&bar_p_full[i][1], ROWS);
+            for (int j = 0; j < PARTS; j++) mbar_init(&bar_p_full[i][j], ROWS);
         }
         for (int i = 0; i < 2; i++) { mbar_init(&bar_q_full[i], ROWS); mbar_init(&bar_pv[i], 1); }
         for (int i = 0; i < NOTES; i++) mbar_init(&bar_note[i], 32);
@@ -267,14 +268,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             const uint32_t q_lo0 = desc_lo(sQ, 16), k_lo0 = desc_lo(sK, 16), v_lo0 = desc_lo(sV, PANEL);
             int s_step = 0, s_x = 0, s_buf = 0, ks = 0;        // the next scores: step, row tile, buffer; stage of its keys
             unsigned kp = 0;
-            bool s_last = false, s_done = false;
+            int last_step = INT_MAX;                           // known once its scores are issued
+            bool s_done = false;
             auto next_scores = [&]() -> bool {
                 if (s_done) return true;
                 if (s_x == 0) {
-                    if (!mbar_wait_warp(&bar_note[s_step % NOTES], (unsigned)(s_step / NOTES) & 1u, abort_flag, a.status, 6) ||
-                        !mbar_wait_warp(&bar_k_full[ks], kp, abort_flag, a.status, 3))
-                        return false;
-                    s_last = s_note[s_step % NOTES].last != 0;
+                    if (!mbar_wait_warp(&bar_k_full[ks], kp, abort_flag, a.status, 3)) return false;
+                    // the loader that announces the keys has seen the planner's note
+                    if (s_note[s_step % NOTES].last) last_step = s_step;
                 }
                 if (s_step == 0 && !mbar_wait_warp(&bar_q_full[s_x], 0, abort_flag, a.status, 2)) return false;
                 fence_async_smem();
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 if (++s_x == tiles) {
                     s_x = 0;
                     s_step++;
-                    s_done = s_last;
+                    s_done = s_step > last_step;
                     if (++ks == STAGES) { ks = 0; kp ^= 1u; }
                 }
                 return true;
@@ -304,21 +305,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             int step = 0, x = 0, buf = 0, vs = 0;              // of the next product
             unsigned pp = 0, vp = 0;
             while (ok) {
-                const bool last = s_note[step % NOTES].last != 0;
                 if (x == 0) ok = mbar_wait_warp(&bar_v_full[vs], vp, abort_flag, a.status, 4);
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    // half of the weights are in tensor memory, and the output is rescaled
-                    ok = ok && mbar_wait_warp(&bar_p_full[buf][half], pp, abort_flag, a.status, 5);
+                for (int part = 0; part < PARTS; part++) {
+                    // these weights are in tensor memory, and the output is rescaled
+                    ok = ok && mbar_wait_warp(&bar_p_full[buf][part], pp, abort_flag, a.status, 5);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint32_t v_lo = v_lo0 + (uint32_t)(vs * (KV_BYTES >> 4));
 #pragma unroll
-                        for (int kk = half * (TILE / 32); kk < (half + 1) * (TILE / 32); kk++)
+                        for (int kk = part * (TILE / 16 / PARTS); kk < (part + 1) * (TILE / 16 / PARTS); kk++)
                             umma_tmem_a_words(tmem + COL_O + x * HD, tmem + COL_S + buf * TILE + (unsigned)(kk * 8),
                                               v_lo + (uint32_t)(kk * (2048 >> 4)), IDESC_O, step > 0 || kk > 0);
-                        if (half == 1) {
+                        if (part == PARTS - 1) {
                             umma_commit(&bar_pv[x]);
                             if (x == tiles - 1) umma_commit(&bar_v_empty[vs]);
                         }
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     __syncwarp();
                 }
                 ok = ok && next_scores();
-                if (!ok || (last && x == tiles - 1)) break;
+                if (!ok || (step == last_step && x == tiles - 1)) break;
                 if (++buf == SBUFS) { buf = 0; pp ^= 1u; }
                 if (++x == tiles) {
                     x = 0;
@@ -638,9 +638,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                             pk[c * 16 + j / 2] = __uint_as_float(q8_half2(p.x, p.y));
                         }
                     tmem_st32(t_s + half * 32, pk);        // over the first 64 columns of the scores
-                    tmem_st_wait();
-                    tc_fence_before();
-                    mbar_arrive(&bar_p_full[buf][half]);
+                    if (PARTS == 2 || half == 1) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(&bar_p_full[buf][PARTS == 2 ? half : 0]);
+                    }
                 }
                 l_run = l_run * corr + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) * per_sum;
                 buf += tiles;
@@ -694,7 +696,7 @@ extern "C" int kllm_attention_q8_tcgen05_head_dim() { return HD; }
 // Requests' portions: rows q_start[s]..q_start[s+1] of request s start at cache position start_pos[s]; bfloat16 rows.  row_tiles:
 // tiles of 128 rows a CTA (1 or 2); splits: parts of the keys, with part_o float32 [n, heads, splits, HD] and part_ml
 // float32 [n, heads, splits, 2] where there are several.  status: a device int that a bounded wait which ran out sets (1, 7:
-// loader, 2-6: issuer, 8-11: softmax, 12: planner).
+// loader, 2-5: issuer, 8-11: softmax, 12: planner).
 extern "C" int kllm_attention_prefill_q8_tcgen05(void* out, float* part_o, float* part_ml, const void* q, int64_t q_stride,
                                                  const void* kcache, const void* vcache, const float* kscale,
                                                  const float* vscale, const int* q_start, const int* start_pos,
