@@ -152,6 +152,41 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// mbar_wait and mbar_arrive of tc5_common.cuh by 32-bit shared addresses: a generic pointer is two registers, and the roles
+// here have none to spare
+__device__ __forceinline__ bool try_at(unsigned bar, unsigned parity) {
+    unsigned ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool wait_at(unsigned bar, unsigned parity, unsigned abort_at, int* status, int where) {
+    if (try_at(bar, parity)) return true;
+    const long long t0 = clock64();
+    unsigned spins = 0;
+    while (!try_at(bar, parity)) {
+        if ((++spins & 255u) == 0) {
+            int gone;
+            asm volatile("ld.volatile.shared.b32 %0, [%1];\n" : "=r"(gone) : "r"(abort_at) : "memory");
+            if (gone) return false;
+            if (clock64() - t0 > kCycleLimit) {
+                asm volatile("st.volatile.shared.b32 [%0], %1;\n" ::"r"(abort_at), "r"(1) : "memory");
+                if (status) atomicCAS(status, 0, where);
+                return false;
+            }
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool wait_warp_at(unsigned bar, unsigned parity, unsigned abort_at, int* status, int where) {
+    return __all_sync(0xffffffffu, wait_at(bar, parity, abort_at, status, where));
+}
+__device__ __forceinline__ void arrive_at(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ uint32_t word_at(unsigned addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 // bits 0 .. n - 1
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
@@ -250,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    volatile int* abort_flag = &s_abort;
+    const unsigned abort_at = smem_u32(&s_abort);
     volatile unsigned* tmem_at = &s_tmem;
     const bool nothing = s_work.tile_lo >= s_work.tile_hi;
     // swizzled tiles want 1024-byte alignment
@@ -273,11 +308,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             auto next_scores = [&]() -> bool {
                 if (s_done) return true;
                 if (s_x == 0) {
-                    if (!mbar_wait_warp(&bar_k_full[ks], kp, abort_flag, a.status, 3)) return false;
+                    if (!wait_warp_at(smem_u32(&bar_k_full[ks]), kp, abort_at, a.status, 3)) return false;
                     // the loader that announces the keys has seen the planner's note
                     if (s_note[s_step % NOTES].last) last_step = s_step;
                 }
-                if (s_step == 0 && !mbar_wait_warp(&bar_q_full[s_x], 0, abort_flag, a.status, 2)) return false;
+                if (s_step == 0 && !wait_warp_at(smem_u32(&bar_q_full[s_x]), 0, abort_at, a.status, 2)) return false;
                 fence_async_smem();
                 tc_fence_after();
                 if (elect_one()) {
@@ -305,11 +340,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             int step = 0, x = 0, buf = 0, vs = 0;              // of the next product
             unsigned pp = 0, vp = 0;
             while (ok) {
-                if (x == 0) ok = mbar_wait_warp(&bar_v_full[vs], vp, abort_flag, a.status, 4);
+                if (x == 0) ok = wait_warp_at(smem_u32(&bar_v_full[vs]), vp, abort_at, a.status, 4);
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
                     // these weights are in tensor memory, and the output is rescaled
-                    ok = ok && mbar_wait_warp(&bar_p_full[buf][part], pp, abort_flag, a.status, 5);
+                    ok = ok && wait_warp_at(smem_u32(&bar_p_full[buf][part]), pp, abort_at, a.status, 5);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
@@ -412,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
 #pragma unroll
                     for (int d = 1; d < 8; d <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, d);
                     const int p = step % PLANS;
-                    ok = mbar_wait_warp(&bar_plan_empty[p], ((unsigned)(step / PLANS) & 1u) ^ 1u, abort_flag, a.status, 12);
+                    ok = wait_warp_at(smem_u32(&bar_plan_empty[p]), ((unsigned)(step / PLANS) & 1u) ^ 1u, abort_at, a.status, 12);
                     if (!ok) break;
                     Note& note = s_note[step % NOTES];
                     if ((lane & 7) == 0) note.member[lane >> 3] = word;
@@ -420,8 +455,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     *reinterpret_cast<int4*>(&s_plan[p].row[lane * 4]) = make_int4(at[0], at[1], at[2], at[3]);
                     *reinterpret_cast<uint4*>(&s_plan[p].kmul[lane * 4]) = make_uint4(kmul[0], kmul[1], kmul[2], kmul[3]);
                     *reinterpret_cast<uint4*>(&s_plan[p].vmul[lane * 4]) = make_uint4(vmul[0], vmul[1], vmul[2], vmul[3]);
-                    mbar_arrive(&bar_note[step % NOTES]);
-                    mbar_arrive(&bar_plan_full[p]);
+                    arrive_at(smem_u32(&bar_note[step % NOTES]));
+                    arrive_at(smem_u32(&bar_plan_full[p]));
                     step++;
                 }
             }
@@ -435,25 +470,26 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             const int tid = threadIdx.x & 127;
             const unsigned stages = shared_base() + 2 * Q_BYTES + (values ? STAGES * KV_BYTES : 0);
             const uint8_t* store = values ? a.vcache : a.kcache;
-            uint64_t* full = values ? bar_v_full : bar_k_full;
-            uint64_t* empty = values ? bar_v_empty : bar_k_empty;
+            const unsigned full = smem_u32(values ? bar_v_full : bar_k_full), empty = smem_u32(values ? bar_v_empty : bar_k_empty);
             // a thread's pieces are of keys KEY_STEP apart
             const int piece = tid % PIECES, key_off = tid / PIECES;
             const bool odd_first = PIECES == 8 && piece >= 4;  // the panels of a row at a time on different banks
             const unsigned place = (unsigned)((piece >> 2) * PANEL) + swz(key_off, (piece & 3) * 2 + (odd_first ? 1 : 0));
             store += piece * 16;
+            const unsigned rows_at = smem_u32(s_plan[0].row) + key_off * 4;
+            const unsigned mul_at = smem_u32(values ? s_plan[0].vmul : s_plan[0].kmul) + key_off * 4;
             uint4 raw[LOADS];
             auto fetch = [&](int p) {
 #pragma unroll
                 for (int i = 0; i < LOADS; i++) {
                     // where there is no key: the first row, which the conversion leaves out
-                    const int r = max(s_plan[p].row[key_off + i * KEY_STEP], 0);
+                    const int r = max((int)word_at(rows_at + p * (unsigned)sizeof(Plan) + i * KEY_STEP * 4), 0);
                     raw[i] = load_early(reinterpret_cast<const uint4*>(store + (int64_t)r * HD));
                 }
             };
             int stage = 0;
             unsigned parity = 1;                               // of the stages' "empty" barriers: free at first
-            bool ok = mbar_wait(&bar_plan_full[0], 0, abort_flag, a.status, 1);
+            bool ok = wait_at(smem_u32(&bar_plan_full[0]), 0, abort_at, a.status, 1);
             if (ok) fetch(0);
 #pragma unroll 1
             for (int step = 0; ok; step++) {
@@ -463,13 +499,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 // not all keys of the tile are of this step: the multiplier of the others is 0, and their bytes (which may be
                 // NaN) become zeros
                 const bool some = (note.member[0] & note.member[1] & note.member[2] & note.member[3]) != 0xffffffffu;
-                const uint32_t* mul = (values ? s_plan[p].vmul : s_plan[p].kmul) + key_off;
-                ok = mbar_wait(&empty[stage], parity, abort_flag, a.status, 7);
+                ok = wait_at(empty + stage * 8, parity, abort_at, a.status, 7);
                 if (!ok) break;
                 const unsigned dst = stages + stage * KV_BYTES + place;
 #pragma unroll
                 for (int i = 0; i < LOADS; i++) {
-                    const uint32_t m = mul[i * KEY_STEP];
+                    const uint32_t m = word_at(mul_at + p * (unsigned)sizeof(Plan) + i * KEY_STEP * 4);
                     uint4 x = raw[i];
                     if (some) {
                         const uint32_t keep = m ? 0xffffffffu : 0u;
@@ -493,10 +528,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     }
                 }
                 fence_async_smem();
-                mbar_arrive(&full[stage]);
-                mbar_arrive(&bar_plan_empty[p]);
+                arrive_at(full + stage * 8);
+                arrive_at(smem_u32(&bar_plan_empty[p]));
                 if (last) break;
-                ok = mbar_wait(&bar_plan_full[p2], (unsigned)((step + 1) / PLANS) & 1u, abort_flag, a.status, 1);
+                ok = wait_at(smem_u32(&bar_plan_full[p2]), (unsigned)((step + 1) / PLANS) & 1u, abort_at, a.status, 1);
                 if (!ok) break;
                 fetch(p2);
                 if (++stage == STAGES) { stage = 0; parity ^= 1u; }
@@ -553,13 +588,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 store16(dst + (unsigned)((i >> 3) * PANEL) + swz(r, i & 7), h[0], h[1], h[2], h[3]);
             }
             fence_async_smem();
-            mbar_arrive(&bar_q_full[x]);
+            arrive_at(smem_u32(&bar_q_full[x]));
             bool last = false;
             int step = 0, buf = x % SBUFS;
             unsigned parity = 0;
             for (; ok && !last; step++) {
-                ok = mbar_wait(&bar_note[step % NOTES], (unsigned)(step / NOTES) & 1u, abort_flag, a.status, 8) &&
-                     mbar_wait(&bar_s_full[buf], parity, abort_flag, a.status, 9);
+                ok = wait_at(smem_u32(&bar_note[step % NOTES]), (unsigned)(step / NOTES) & 1u, abort_at, a.status, 8) &&
+                     wait_at(smem_u32(&bar_s_full[buf]), parity, abort_at, a.status, 9);
                 if (!ok) break;
                 const unsigned t_s = t_s0 + buf * TILE;
                 tc_fence_after();
@@ -605,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 // the product of this row tile's step before is over (waited for every time: a wait by parity is only sound for
                 // the phase behind the one waited for last)
                 if (step > 0) {
-                    ok = mbar_wait(&bar_pv[x], (unsigned)(step - 1) & 1u, abort_flag, a.status, 10);
+                    ok = wait_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 10);
                     if (!ok) break;
                     if (__any_sync(0xffffffffu, move)) {
                         // rows of this warp rescale what the products so far have added up (rows that did not move multiply by
@@ -641,14 +676,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     if (PARTS == 2 || half == 1) {
                         tmem_st_wait();
                         tc_fence_before();
-                        mbar_arrive(&bar_p_full[buf][PARTS == 2 ? half : 0]);
+                        arrive_at(smem_u32(&bar_p_full[buf][PARTS == 2 ? half : 0]));
                     }
                 }
                 l_run = l_run * corr + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) * per_sum;
                 buf += tiles;
                 if (buf >= SBUFS) { buf -= SBUFS; parity ^= 1u; }
             }
-            if (ok) ok = mbar_wait(&bar_pv[x], (unsigned)(step - 1) & 1u, abort_flag, a.status, 11);
+            if (ok) ok = wait_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 11);
             if (ok) {
                 tc_fence_after();
 #pragma unroll
