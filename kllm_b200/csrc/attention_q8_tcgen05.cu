@@ -65,7 +65,7 @@ static_assert(SMEM_BYTES <= 226 * 1024, "shared memory");
 constexpr unsigned COL_S = 0, COL_O = SBUFS * TILE;      // scores / weights, outputs of the row tiles (HD columns each)
 constexpr int TMEM_COLS = 512;
 static_assert(SBUFS * TILE + 2 * HD <= TMEM_COLS, "tensor memory");
-constexpr int REGS_SOFTMAX = 160, REGS_LOADER = 56, REGS_ISSUER = 48;
+constexpr int REGS_SOFTMAX = 168, REGS_LOADER = 48, REGS_ISSUER = 48;
 // setmaxnreg moves registers inside the CTA's own allocation (threads x registers at launch, multiples of 8)
 static_assert(2 * REGS_SOFTMAX + 2 * REGS_LOADER + REGS_ISSUER <= THREADS / 128 * (65536 / THREADS / 8 * 8), "setmaxnreg budget");
 static_assert(PLANS + STAGES < NOTES, "notes");
@@ -637,11 +637,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     m_ref = mx;
                 }
                 const float shift = m_ref == -INFINITY ? ev + kLift : ev - m_ref + kLift;
-                // the product of this row tile's step before is over (waited for every time: a wait by parity is only sound for
-                // the phase behind the one waited for last)
+                // The product of this row tile's step before has to be over.  With two score buffers and two row tiles it was
+                // issued before these scores, and is; otherwise it is waited for, every time (a wait by parity is only sound for
+                // the phase behind the one waited for last).
                 if (step > 0) {
-                    ok = wait_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 10);
-                    if (!ok) break;
+                    if (SBUFS != 2 || tiles != 2) {
+                        ok = wait_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 10);
+                        if (!ok) break;
+                    }
                     if (__any_sync(0xffffffffu, move)) {
                         // rows of this warp rescale what the products so far have added up (rows that did not move multiply by
                         // one); the next product waits for these weights

@@ -1218,17 +1218,32 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
         launches += 1       # the kernel that joins the ranges
 
 
-def prefill_q8_parts(n_tokens: int, n_requests: int, n_kv: int, group: int, ctx_bound: int) -> tuple:
-    """(row tiles of a CTA, parts of the keys) of the tcgen05 form of ``attention_prefill_q8``."""
-    return _prefill_q8_parts(n_tokens, n_requests, n_kv, group, ctx_bound, sm_count())
+def prefill_q8_parts(n_tokens: int, n_requests: int, n_kv: int, group: int, ctx_bound: int, head_dim: int = 128) -> tuple:
+    """(row tiles of a CTA, parts of the keys) of the tcgen05 form of ``attention_prefill_q8``: the pair whose time, by this
+    account, is least.  Measured at head size 128 (64): a CTA takes about 5 us to begin and end and, for every 128 keys, 1.6
+    (1.4) us with one tile of 128 rows and 2.3 (1.8) with two; an SM holds one CTA; several parts cost about 4 us and their
+    unscaled rows written and read once.  Microseconds, 32 heads, tiles x parts: 512 tokens behind 7680 over 8 kv heads of 128
+    1x1: 109, 2x1: 153, 2x2: 106, 2x4: 121; 64 behind 8000 1x1: 105, 1x8: 28, 1x16: 40; 300 alone 1x1: 13.3, 2x1: 17.4; 2048
+    alone over 4 of 64 1x1: 64, 2x1: 40."""
+    return _prefill_q8_parts(n_tokens, n_requests, n_kv, group, ctx_bound, head_dim, sm_count())
 
 
 @functools.lru_cache(maxsize=4096)
-def _prefill_q8_parts(n_tokens, n_requests, n_kv, group, ctx_bound, sms):
-    per_tile = 128 // group
-    ctas = (n_tokens // (2 * per_tile) + n_requests) * n_kv
-    splits = max(1, min(sms // max(1, ctas), -(-ctx_bound // 128) // 4))
-    return 2, splits
+def _prefill_q8_parts(n_tokens, n_requests, n_kv, group, ctx_bound, head_dim, sms):
+    new = -(-n_tokens // max(1, n_requests))
+    longest = max(1, -(-ctx_bound // 128))
+    usual = max(1.0, (ctx_bound - new / 2) / 128)
+    best = None
+    for row_tiles, per_tile in ((2, 2.3 if head_dim == 128 else 1.8), (1, 1.6 if head_dim == 128 else 1.4)):
+        ctas = max(1, n_requests) * -(-new // (row_tiles * (128 // group))) * n_kv
+        for splits in range(1, max(1, min(16, longest // 2)) + 1):
+            waves = ctas / sms if splits == 1 else -(-ctas * splits // sms)      # parts are alike; row tiles are causal, long ones first
+            us = max(5 + -(-longest // splits) * per_tile, waves * (5 + usual / splits * per_tile))
+            if splits > 1:
+                us += 4 + n_tokens * group * n_kv * splits * head_dim * 8 / 5e6
+            if best is None or us < best[0]:
+                best = (us, row_tiles, splits)
+    return best[1:]
 
 
 def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
@@ -1249,7 +1264,8 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
     pages, _, page_size, _ = kcache.shape
     group = n_heads // n_kv
     if code == 1 and head_dim in TCGEN05_HEAD_DIMS and USE_TCGEN05 and group <= 128 and out.data_ptr() % 16 == 0:
-        row_tiles, splits = prefill_q8_parts(n, R, n_kv, group, ctx_bound)
+        bound = min(ctx_bound, window + 256 // group) if window and window > 0 else ctx_bound
+        row_tiles, splits = prefill_q8_parts(n, R, n_kv, group, bound, head_dim)
         part_o = part_ml = None
         if splits > 1:
             parts = torch.empty((n * n_heads * splits, head_dim + 2), dtype=torch.float32, device=q.device)

@@ -122,6 +122,16 @@ def test_parts_of_a_context(tokens, n_kv, group, hd, ctx, monkeypatch):
     assert ranges * cluster <= max(1, blocks), "a part for every 128 keys at most"
 
 
+@pytest.mark.parametrize("tokens,requests", [(1, 1), (9, 9), (300, 1), (2048, 1), (700, 12), (100000, 3)])
+@pytest.mark.parametrize("n_kv,group,hd", [(4, 8, 64), (8, 4, 128), (32, 1, 128), (1, 128, 64)])
+@pytest.mark.parametrize("ctx", [0, 1, 128, 257, 8192, 2 ** 31 - 1])
+def test_parts_of_portions(tokens, requests, n_kv, group, hd, ctx, monkeypatch):
+    monkeypatch.setattr(kernels, "sm_count", lambda: 148)
+    row_tiles, splits = kernels.prefill_q8_parts(tokens, requests, n_kv, group, max(ctx, tokens // requests), hd)
+    assert row_tiles in (1, 2) and 1 <= splits <= 16
+    assert splits == 1 or splits * 2 * 128 <= max(ctx, tokens) + 128, "two tiles of keys a part at least"
+
+
 # ---- the manager and the options -----------------------------------------------------------------------------------------
 
 def test_manager_keeps_pages_in_eight_bits():
