@@ -333,7 +333,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         copies_wait<2 * DEC_STAGES - 1>();                            // this tile's keys and scales
         __syncwarp();
         const unsigned k_at = ring + stage * 2 * DEC_TILE, v_at = k_at + DEC_TILE;
-        float s[DEC_MT][NG][4];
+        float s[DEC_MT][NG][4], part[DEC_MT][NG][4];
 #pragma unroll
         for (int mt = 0; mt < DEC_MT; mt++)
 #pragma unroll
@@ -360,6 +360,13 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                     q8_to_f16x4(kr[mt][0][w], ka[mt][0], ka[mt][2]);
                     q8_to_f16x4(kr[mt][1][w], ka[mt][1], ka[mt][3]);
                 }
+                // The tensor core cuts its sums; beside float32 queries 32 products at a time are added to a sum in registers
+                // (one sum over 256 dims was 2.7 times as far from 64 bits as float32 arithmetic).
+                float (&to)[DEC_MT][NG][4] = NQ > 1 ? part : s;
+                if (NQ > 1 && kk % 2 == 0) {
+#pragma unroll
+                    for (int i = 0; i < DEC_MT * NG * 4; i++) (&part[0][0][0])[i] = 0.f;
+                }
 #pragma unroll
                 for (int j = NQ - 1; j >= 0; j--)                   // the smallest part first
 #pragma unroll
@@ -367,8 +374,12 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                         const int at = (kk * NQ + j) * NG + ng;
                         const uint2 b = Q_IN_REGS ? qr[Q_IN_REGS ? at : 0] : sq[at * 32 + lane];
 #pragma unroll
-                        for (int mt = 0; mt < DEC_MT; mt++) mma16816(s[mt][ng], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
+                        for (int mt = 0; mt < DEC_MT; mt++) mma16816(to[mt][ng], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
                     }
+                if (NQ > 1 && kk % 2 == 1) {
+#pragma unroll
+                    for (int i = 0; i < DEC_MT * NG * 4; i++) (&s[0][0][0])[i] += (&part[0][0][0])[i];
+                }
             }
         }
         __syncwarp();                                                 // everybody has read this tile's keys
