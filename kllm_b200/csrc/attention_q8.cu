@@ -821,6 +821,7 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
                 for (int n = 0; n < HD / 8; n++) { o[n][2 * i] *= corr; o[n][2 * i + 1] *= corr; }
             }
         }
+        float l_tile[2] = {0.f, 0.f};
         const float ref[2] = {m_ref[0] == -INFINITY ? 0.f : m_ref[0] - kLift, m_ref[1] == -INFINITY ? 0.f : m_ref[1] - kLift};
 #pragma unroll
         for (int n = 0; n < PRE_KEYS / 8; n++)
@@ -831,12 +832,14 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
                 for (int i = 0; i < 2; i++) {
                     float& x = s[n][2 * i + j];
                     x = fast_exp2(x - ref[i]);
-                    l_run[i] = fmaf(x, inv, l_run[i]);
+                    l_tile[i] = fmaf(x, inv, l_tile[i]);
                 }
             }
+        l_run[0] += l_tile[0];
+        l_run[1] += l_tile[1];
+        uint32_t pa[PRE_KEYS / 16][NP][4];
 #pragma unroll
-        for (int kk = 0; kk < PRE_KEYS / 16; kk++) {
-            uint32_t pa[NP][4];
+        for (int kk = 0; kk < PRE_KEYS / 16; kk++)
 #pragma unroll
             for (int x = 0; x < 4; x++) {                 // a0: row g, keys 2t; a1: row g + 8; a2, a3: keys + 8
                 const int n = 2 * kk + (x >> 1), i = x & 1;
@@ -846,17 +849,31 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
 #pragma unroll
                 for (int j = 0; j < NP; j++) {
                     const __half2 hh = __halves2half2(h0[j], h1[j]);
-                    pa[j][x] = *reinterpret_cast<const uint32_t*>(&hh);
+                    pa[kk][j][x] = *reinterpret_cast<const uint32_t*>(&hh);
                 }
             }
+        // The tensor core cuts its sums: beside float32 queries a tile's keys are added to a sum in registers (one sum over
+        // 4000 keys was four times as far from 64 bits as float32 arithmetic).
 #pragma unroll
-            for (int n = 0; n < HD / 16; n++) {
+        for (int n = 0; n < HD / 16; n++) {
+            float part[2][4] = {};
+            float (&to0)[4] = NP > 1 ? part[0] : o[2 * n];
+            float (&to1)[4] = NP > 1 ? part[1] : o[2 * n + 1];
+#pragma unroll
+            for (int kk = 0; kk < PRE_KEYS / 16; kk++) {
                 uint32_t b[4];
                 ldmatrix4t(sv_u + vb_off + (unsigned)(kk * 16 * PRE_LD * 2) + n * 32, b);
 #pragma unroll
                 for (int j = NP - 1; j >= 0; j--) {
-                    mma16816(o[2 * n], pa[j][0], pa[j][1], pa[j][2], pa[j][3], b[0], b[1]);
-                    mma16816(o[2 * n + 1], pa[j][0], pa[j][1], pa[j][2], pa[j][3], b[2], b[3]);
+                    mma16816(to0, pa[kk][j][0], pa[kk][j][1], pa[kk][j][2], pa[kk][j][3], b[0], b[1]);
+                    mma16816(to1, pa[kk][j][0], pa[kk][j][1], pa[kk][j][2], pa[kk][j][3], b[2], b[3]);
+                }
+            }
+            if constexpr (NP > 1) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    o[2 * n][j] += part[0][j];
+                    o[2 * n + 1][j] += part[1][j];
                 }
             }
         }
