@@ -188,12 +188,12 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     const int head0 = kvh * (a.n_heads / a.n_kv) + sub * a.heads_per_cta, nh = a.heads_per_cta;
     const int req = a.token_req ? a.token_req[token] : token;
     const int p = (req >= 0 && req < a.n_requests) ? a.positions[token] : -1;
-    const int hi = p + 1, lo = (a.window > 0 && hi > a.window) ? hi - a.window : 0;
+    const int lo = (a.window > 0 && p >= a.window) ? p - a.window + 1 : 0, hi = keys_end((int64_t)p + 1, a.max_blocks, a.page_size);
 
     // this warp's tiles: the token's tiles [first, last) in one part per CTA, a part's tiles in turn over the warps
     const int parts = gridDim.x, part = blockIdx.x;
     const int first = lo / DEC_KT, last = (hi + DEC_KT - 1) / DEC_KT;      // tiles start at multiples of their size
-    const int per = (last - first + parts - 1) / parts;
+    const int per = (max(last - first, 0) + parts - 1) / parts;
     const int tile_lo = first + part * per, tile_hi = min(last, tile_lo + per);
 
     const int* table = a.block_table + (int64_t)(req < 0 ? 0 : req) * a.max_blocks;
@@ -210,7 +210,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + Shape::Q_BYTES + warp * DEC_RING;
     const unsigned meta = ring + DEC_STAGES * 2 * DEC_TILE;
     // Copies of 16 bytes, COPIES a lane and tile.  Sixteen keys of one page, all seen, lie one behind the other: their
-    // copies differ by constants (765 instructions a tile of 32 keys at head size 128 with a look-up per row, !!! with this).
+    // copies differ by constants, where a look-up per row costs a shuffle, a comparison and a 64-bit product each.
     constexpr int COPIES = DEC_KT * PIECES / 32;
     const bool blocks = a.page_size % 16 == 0;
     int rows[COPIES];                     // of the tile that is being requested; -1: not seen.  In blocks: the first two, a row each
@@ -651,15 +651,10 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
     griddep_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
     const int kvh = blockIdx.x % a.n_kv, gs = a.n_heads / a.n_kv;
-    if (tid == 0) {
-        int tile = (gridDim.x - 1 - blockIdx.x) / a.n_kv, req = -1, tok0 = 0;       // longest key ranges first
-        for (int s = 0; s < a.n_requests; s++) {
-            const int n = a.q_start[s + 1] - a.q_start[s];
-            const int nt = (n + a.tokens_per_tile - 1) / a.tokens_per_tile;
-            if (tile < nt) { req = s; tok0 = a.q_start[s] + tile * a.tokens_per_tile; break; }
-            tile -= nt;
-        }
-        s_req = req; s_tok0 = tok0;
+    if (warp == 0) {
+        int req = -1, tok0 = 0;                           // longest key ranges first
+        if (!find_portion(a.q_start, a.n_requests, a.tokens_per_tile, (gridDim.x - 1 - blockIdx.x) / a.n_kv, req, tok0)) req = -1;
+        if (lane == 0) { s_req = req; s_tok0 = tok0; }
     }
     __syncthreads();
     const int req = s_req, tok0 = s_tok0;
@@ -667,8 +662,8 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
     const int n_tok = min(min(a.tokens_per_tile, a.q_start[req + 1] - tok0), a.n_tokens - tok0);
     if (n_tok <= 0) return;
     const int pos0 = a.start_pos[req] + (tok0 - a.q_start[req]);
-    const int lo = (a.window > 0 && pos0 + 1 > a.window) ? pos0 + 1 - a.window : 0;
-    const int hi = pos0 + n_tok;
+    const int lo = (a.window > 0 && pos0 >= a.window) ? pos0 - a.window + 1 : 0;
+    const int hi = keys_end((int64_t)pos0 + n_tok, a.max_blocks, a.page_size);
     const int* table = a.block_table + (int64_t)req * a.max_blocks;
 
     // queries into shared memory as float16 parts; a quarter warp's lanes share a row's pieces
@@ -805,7 +800,7 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
                 for (int i = 0; i < 2; i++) {
                     float& x = s[n][2 * i + j];
                     x = fmaf(x * mul, factor[i], ev);
-                    if (key > p_row[i] || (a.window > 0 && key + a.window <= p_row[i]) || ev == -INFINITY) x = -INFINITY;
+                    if (key > p_row[i] || (a.window > 0 && p_row[i] - key >= a.window) || ev == -INFINITY) x = -INFINITY;
                     mx[i] = fmaxf(mx[i], x);
                 }
             }
@@ -907,8 +902,9 @@ template <typename T> int launch_prefill(const PrefillArgs& a, cudaStream_t stre
         snprintf(g_kllm_err, sizeof(g_kllm_err), "attention (8 bits): %zu bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
         return (int)e;
     }
-    const int tiles = a.n_tokens / a.tokens_per_tile + a.n_requests;
-    kllm_launch((attn_prefill_q8_kernel<T>), dim3((unsigned)tiles * a.n_kv), dim3(PRE_THREADS), smem, stream, a);
+    const int64_t ctas = ((int64_t)a.n_tokens / a.tokens_per_tile + a.n_requests) * a.n_kv;
+    if (ctas > 0x7fffffffLL) KLLM_FAIL("attention (8 bits): %lld CTAs", (long long)ctas);
+    kllm_launch((attn_prefill_q8_kernel<T>), dim3((unsigned)ctas), dim3(PRE_THREADS), smem, stream, a);
     KLLM_LAUNCH_STATUS();
 }
 

@@ -225,32 +225,30 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
     static_assert(alignof(Plan) == 16 && sizeof(Plan) % 16 == 0, "four words at a time");
     __shared__ unsigned s_tmem;
     __shared__ volatile Work s_work;
+    __shared__ int2 s_place;
     __shared__ int s_abort;
     const int warp = warp_index(), lane = threadIdx.x & 31;
     griddep_wait();
     griddep_launch();
-    if (threadIdx.x == 0) {
+    if (warp == 0) {
         // CTAs start in the order of blockIdx.x: longest key ranges first, all kv heads and parts of a range side by side
-        const int per_cta = a.tokens_per_tile * a.row_tiles, split = blockIdx.x % a.splits;
-        int tile = (gridDim.x - 1 - blockIdx.x) / (a.n_kv * a.splits), req = -1, tok0 = 0, first_row = 0, end = 0;
-        for (int s = 0; s < a.n_requests; s++) {
-            const int n = a.q_start[s + 1] - a.q_start[s];
-            const int nt = (n + per_cta - 1) / per_cta;
-            if (tile < nt) {
-                req = s;
-                first_row = a.q_start[s];
-                tok0 = first_row + tile * per_cta;
-                end = min(a.q_start[s + 1], a.n_tokens);
-                break;
-            }
-            tile -= nt;
-        }
+        const int per_cta = a.tokens_per_tile * a.row_tiles;
+        int req = -1, tok0 = 0;
+        if (!find_portion(a.q_start, a.n_requests, per_cta, (gridDim.x - 1 - blockIdx.x) / (a.n_kv * a.splits), req, tok0)) req = -1;
+        if (lane == 0) s_place = make_int2(req, tok0);
+        __syncwarp();
+    }
+    if (threadIdx.x == 0) {
+        const int per_cta = a.tokens_per_tile * a.row_tiles, split = blockIdx.x % a.splits, tok0 = s_place.y;
+        int req = s_place.x;
+        const int first_row = req >= 0 ? a.q_start[req] : 0, end = req >= 0 ? min(a.q_start[req + 1], a.n_tokens) : 0;
         if (req >= 0 && end <= tok0) req = -1;
         s_work.req = req;
         if (req >= 0) {
             const int n_tok = min(per_cta, end - tok0), pos0 = a.start_pos[req] + (tok0 - first_row);
-            const int lo = (a.window > 0 && pos0 + 1 > a.window) ? pos0 + 1 - a.window : 0;
-            const int hi = max(pos0 + n_tok, 1);               // one tile at least: every role takes at least one step
+            const int hi = max(keys_end((int64_t)pos0 + n_tok, a.max_blocks, a.page_size), 1);
+            // one tile at least: every role takes at least one step (a window behind the table's end sees nothing in it)
+            const int lo = min((a.window > 0 && pos0 >= a.window) ? pos0 - a.window + 1 : 0, hi - 1);
             // this part's tiles of keys; a part without any leaves zeros
             const int first = lo / TILE, all = (hi + TILE - 1) / TILE - first, per = (all + a.splits - 1) / a.splits;
             s_work.tok0 = tok0;

@@ -7,8 +7,8 @@
 // The range leaves float32 room for what is multiplied with it: weights times 2^(-e) stay finite and, between any two
 // pages, above 2^-126 unless they differ by 2^30 besides.
 //
-// Every e4m3 number is a float16 number (and e4m3 x e4m3-scaled sums are not needed): the attention kernels hand keys and
-// values to the tensor cores as float16, exactly, with one conversion per two numbers, and float32 accumulators.
+// Every e4m3 number is a float16 number: the attention kernels hand keys and values to the tensor cores as float16, exactly,
+// with one conversion per two numbers, and float32 accumulators.
 //
 // A key row that holds NaN marks a token whose key or value was not finite when it was stored; its values are stored as
 // zeros.  Value rows therefore never hold NaN, and a weight of 0 removes a masked token whatever it held.
@@ -110,6 +110,38 @@ template <typename T> __device__ __forceinline__ void store_row4(T* dst, const f
     } else {
         *reinterpret_cast<float4*>(dst) = y;
     }
+}
+
+// A request's portion and its rows' tile: the tile'th of the tiles of `per` rows into which the requests' portions
+// q_start[s] .. q_start[s + 1] are cut one after another.  By a whole warp, a request a lane (400 requests of 2
+// tokens behind 100: 101 us, with a walk by one thread 322).  False: there are fewer tiles.
+__device__ __forceinline__ bool find_portion(const int* q_start, int n_requests, int per, int tile, int& req, int& tok0) {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < n_requests; s0 += 32) {
+        const int s = s0 + lane, begin = s < n_requests ? q_start[s] : 0, rows = s < n_requests ? q_start[s + 1] - begin : 0;
+        const int mine = rows > 0 ? (rows + per - 1) / per : 0;
+        int upto = mine;                                     // tiles of this group of requests up to the lane's own
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int before = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += before;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, tile < upto);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            req = s0 + l;
+            tok0 = __shfl_sync(0xffffffffu, begin + (tile - (upto - mine)) * per, l);
+            return true;
+        }
+        tile -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+// The end of the keys that a table of max_blocks pages can name, at most hi: a position behind the table costs no walk there.
+__device__ __forceinline__ int keys_end(int64_t hi, int max_blocks, int page_size) {
+    const int64_t end = (int64_t)max_blocks * page_size;
+    return (int)(hi < end ? hi : end);
 }
 
 // joins the ranges of a (token, head) in order

@@ -1080,6 +1080,17 @@ def _check_q8(what, kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, 
     raise KernelError(f"{what}: the block table must be contiguous int32 [requests, pages of a request]")
 
 
+def _q8_device(what, *tensors):
+    """All operands on one CUDA device, and that the current one: the launch goes to the current device's stream."""
+    device = torch._C._cuda_getDevice() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            _cuda(*tensors)
+            raise KernelError(f"{what}: operands on more than one device, or on another than the current one")
+    if device < 0:
+        _cuda(*tensors)
+
+
 def _check_q8_ints(what, *tensors):
     for t in tensors:
         if t.dtype is not _i32_t or not t.is_contiguous():
@@ -1103,10 +1114,12 @@ def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
 
     Rows ``q_start[s] .. q_start[s + 1]`` are request s's, at consecutive ``positions``; ``token_req`` None: every request
     brings one token.  ``cos_sin``: float32 [positions, rotary width], None: no rotation.  Tokens with a negative position
-    or one behind the table of angles are neither rotated nor stored, those without a page not stored; rows behind the last
-    request are left as they are.  No page may belong to two requests of a step."""
+    or one behind the table of angles are neither rotated nor stored (the rotated part of their rows of ``q_out`` is left as it
+    is), those without a page not stored; rows behind the last request are left as they are.  No page may belong to two requests of a step."""
     _check_q8("rope_append_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
     _check_q8_ints("rope_append_q8", positions, q_start)
+    if q.dim() != 2:
+        raise KernelError("rope_append_q8: q and q_out [n, heads * head_dim], k and v [n, kv heads * head_dim]")
     dt, (n, width) = q.dtype, q.shape
     code = dtype_code(dt)
     if q_out.dtype is not dt or k.dtype is not dt or v.dtype is not dt:
@@ -1129,10 +1142,10 @@ def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
                           "(token_req None: one token per request)")
     n_pos = rot = 0
     if cos_sin is not None:
-        n_pos, rot = cos_sin.shape
+        n_pos, rot = cos_sin.shape if cos_sin.dim() == 2 else (0, 1)
         if cos_sin.dtype is not _f32 or not cos_sin.is_contiguous() or rot % 2 or rot > head_dim:
             raise KernelError("rope_append_q8: cos_sin must be contiguous float32 [positions, even rotary width <= head_dim]")
-    _cuda(q_out, q, k, v, cos_sin, positions, token_req, q_start, block_table, kcache, vcache, kscale, vscale)
+    _q8_device("rope_append_q8", q_out, q, k, v, cos_sin, positions, token_req, q_start, block_table, kcache, vcache, kscale, vscale)
     fn, lib = _q8_function("cache_q8", "kllm_rope_append_q8")
     rc = fn(q_out.data_ptr(), so, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _p(cos_sin), n_pos, positions.data_ptr(),
             _p(token_req), q_start.data_ptr(), R, block_table.data_ptr(), blocks, kcache.data_ptr(), vcache.data_ptr(),
@@ -1173,10 +1186,15 @@ def decode_q8_parts(n_tokens: int, n_kv: int, group: int, head_dim: int, ctx_bou
     return _decode_q8_parts(n_tokens, n_kv, group, head_dim, ctx_bound, wide, sm_count())
 
 
+def _q8_window(window) -> int:
+    """0: none.  A window of 2^31 - 1 tokens or more leaves out nothing that a cache can hold."""
+    return min(window, 2 ** 31 - 1) if window and window > 0 else 0
+
+
 def _check_q8_rows(what, out, q, n_heads, head_dim):
     """(dtype's code, rows, row stride)"""
-    dt, (n, width) = q.dtype, q.shape
-    stride, dense = q.stride()
+    dt, (n, width) = q.dtype, q.shape if q.dim() == 2 else (0, 0)
+    stride, dense = q.stride() if width else (0, 0)
     if out.dtype is not dt or width != n_heads * head_dim or dense != 1 or out.shape != q.shape or not out.is_contiguous():
         raise KernelError(f"{what}: q [n, heads * head_dim] with dense rows, out contiguous of the same shape and dtype")
     return dtype_code(dt), n, stride
@@ -1190,7 +1208,7 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
     leaves them): row t, at ``positions[t]`` of request ``token_req[t]`` (None: request t), sees its request's keys up to
     its own place (``window`` W > 0: the last W of them).  bfloat16 or float32 ``q`` and ``out`` [n, H*hd].  ``ctx_bound``:
     no context is longer; it only decides into how many parts the contexts are cut.  Keys whose table entry names no page
-    are not seen; a row that sees none (a negative position, say) becomes zeros."""
+    are not seen; a row that sees none (a negative position, say) becomes zeros.  At most 65535 rows a call."""
     _check_q8("attention_decode_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
     code, n, stride = _check_q8_rows("attention_decode_q8", out, q, n_heads, head_dim)
     _check_q8_ints("attention_decode_q8", positions)
@@ -1199,8 +1217,9 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
     R, blocks = block_table.shape
     if positions.numel() < n or (token_req.numel() < n if token_req is not None else R < n):
         raise KernelError("attention_decode_q8: a position (and a request) per token")
-    _cuda(out, q, kcache, vcache, kscale, vscale, positions, token_req, block_table)
-    bound = min(ctx_bound, window) if window and window > 0 else ctx_bound
+    _q8_device("attention_decode_q8", out, q, kcache, vcache, kscale, vscale, positions, token_req, block_table)
+    window = _q8_window(window)
+    bound = min(ctx_bound, window) if window else ctx_bound
     ranges, cluster = decode_q8_parts(n, n_kv, n_heads // n_kv, head_dim, bound, code == 0)
     part_o = part_ml = None
     if ranges > 1:
@@ -1211,7 +1230,7 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
     fn, lib = _q8_function("attention_q8", "kllm_attention_decode_q8", head_dim)
     rc = fn(out.data_ptr(), part_o, part_ml, q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
             vscale.data_ptr(), positions.data_ptr(), _p(token_req), block_table.data_ptr(), blocks, pages, n, R, n_heads, n_kv,
-            head_dim, page_size, window or 0, scale, ranges, cluster, code, _stream())
+            head_dim, page_size, window, scale, ranges, cluster, code, _stream())
     _check(lib, "attention_q8", rc)
     global launches
     if ranges > 1:
@@ -1260,11 +1279,12 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
     requests, blocks = block_table.shape
     if R < 0 or q_start.numel() < R + 1 or start_pos.numel() < R or requests < R:
         raise KernelError("attention_prefill_q8: q_start, start_pos and the block table must cover the requests")
-    _cuda(out, q, kcache, vcache, kscale, vscale, q_start, start_pos, block_table)
+    _q8_device("attention_prefill_q8", out, q, kcache, vcache, kscale, vscale, q_start, start_pos, block_table)
     pages, _, page_size, _ = kcache.shape
     group = n_heads // n_kv
+    window = _q8_window(window)
     if code == 1 and head_dim in TCGEN05_HEAD_DIMS and USE_TCGEN05 and group <= 128 and out.data_ptr() % 16 == 0:
-        bound = min(ctx_bound, window + 256 // group) if window and window > 0 else ctx_bound
+        bound = min(ctx_bound, window + 256 // group) if window else ctx_bound
         row_tiles, splits = prefill_q8_parts(n, R, n_kv, group, bound, head_dim)
         part_o = part_ml = None
         if splits > 1:
@@ -1277,7 +1297,7 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
         fn, lib = _q8_function("attention_q8_tcgen05", "kllm_attention_prefill_q8_tcgen05", head_dim)
         rc = fn(out.data_ptr(), part_o, part_ml, q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
                 vscale.data_ptr(), q_start.data_ptr(), start_pos.data_ptr(), block_table.data_ptr(), blocks, pages, n, R, n_heads,
-                n_kv, head_dim, page_size, window or 0, scale, row_tiles, splits, word.data_ptr(), _stream())
+                n_kv, head_dim, page_size, window, scale, row_tiles, splits, word.data_ptr(), _stream())
         _check(lib, "attention_q8_tcgen05", rc)
         global launches
         if splits > 1:
@@ -1286,7 +1306,7 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
     fn, lib = _q8_function("attention_q8", "kllm_attention_prefill_q8", head_dim)
     rc = fn(out.data_ptr(), q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(),
             q_start.data_ptr(), start_pos.data_ptr(), block_table.data_ptr(), blocks, pages, n, R, n_heads, n_kv, head_dim,
-            page_size, window or 0, scale, code, _stream())
+            page_size, window, scale, code, _stream())
     _check(lib, "attention_q8", rc)
 
 

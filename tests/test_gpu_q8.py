@@ -525,3 +525,163 @@ def test_refuses_what_the_kernels_do_not_take():
     c.k = off
     with pytest.raises(KernelError, match="aligned"):
         decode(c, queries(1, 4, 64, "bf16", 1), ints(10), 4, 1, 64)
+
+
+# ---- calls at the edges of what the faces allow -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 40 + 5])
+def test_windows_beyond_every_context(dtype, window):
+    H, G, hd = 8, 2, 64
+    c = Cache([90, 0], [20, 33], G, hd, 16, seed=21)
+    rows = queries(53, H, hd, dtype, 22)
+    assert torch.equal(prefill(c, rows, [90, 0], [20, 33], H, G, hd, window), prefill(c, rows, [90, 0], [20, 33], H, G, hd))
+    pos = ints(109, 32)
+    assert torch.equal(decode(c, rows[:2], pos, H, G, hd, window), decode(c, rows[:2], pos, H, G, hd))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("far", [2 ** 20, 2 ** 30, 2 ** 31 - 200])
+def test_positions_far_behind_the_table(dtype, far):
+    """A row sees what the table names of the keys before it, which is all of it, and walks no further."""
+    H, G, hd = 8, 2, 64
+    c = Cache([47], [1], G, hd, 16, seed=23)
+    rows = queries(3, H, hd, dtype, 24)
+    portion = prefill(c, rows, [far], [3], H, G, hd)
+    single = decode(c, rows, ints(far, far + 1, far + 2), H, G, hd, req=ints(0, 0, 0))
+    for i in range(3):
+        for got in (portion, single):
+            check(got[i:i + 1], rows[i:i + 1], c, [47], [1], H, G, hd)
+    assert not prefill(c, rows, [far], [3], H, G, hd, window=20).any()
+    assert not decode(c, rows, ints(far, far + 1, far + 2), H, G, hd, window=20, req=ints(0, 0, 0)).any()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 96])
+def test_many_portions(dtype, hd):
+    """More requests than a warp has lanes, some without rows, in tiles that end anywhere."""
+    H, G, R = 4, 2, 171
+    lens = [(7 * i) % 5 if i % 11 else 0 for i in range(R)]
+    lens[40], lens[170] = 150, 90
+    starts = [(13 * i) % 37 for i in range(R)]
+    c = Cache(starts, lens, G, hd, 16, seed=25)
+    rows = queries(sum(lens), H, hd, dtype, 26)
+    check(prefill(c, rows, starts, lens, H, G, hd), rows, c, starts, lens, H, G, hd)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_calls_without_rows(dtype):
+    from kllm_b200 import kernels
+    H, G, hd = 4, 2, 64
+    c = Cache([10], [1], G, hd, 16, seed=27)
+    none = torch.zeros(0, H * hd, dtype=DT[dtype], device="cuda")
+    flat = torch.zeros(0, dtype=torch.int32, device="cuda")
+    decode(c, none, flat, H, G, hd, bound=1)
+    kernels.attention_prefill_q8(none, none, c.k, c.v, c.ks, c.vs, ints(0, 0), ints(10), c.dev_table, 1, H, G, hd, 0, 0.1, 0)
+    rows = queries(3, H, hd, dtype, 28)
+    out = torch.full_like(rows, 7.0).contiguous()
+    kernels.attention_prefill_q8(out, rows, c.k, c.v, c.ks, c.vs, ints(0), flat, c.dev_table[:0], 0, H, G, hd, 0, 0.1, 0)
+    assert bool((out == 7.0).all())
+    before = [t.clone() for t in (c.k.view(torch.uint8), c.ks)]
+    kv = torch.zeros(0, G * hd, dtype=DT[dtype], device="cuda")
+    kernels.rope_append_q8(none, none, kv, kv, None, flat, flat, ints(0, 0), c.dev_table, c.k, c.v, c.ks, c.vs, H, G, hd)
+    torch.cuda.synchronize()
+    assert torch.equal(before[0], c.k.view(torch.uint8)) and torch.equal(before[1].nan_to_num(3.0), c.ks.nan_to_num(3.0))
+
+
+def test_two_graphs_that_share_their_workspace():
+    """Contexts in several ranges and portions in several parts take room for their parts: two graphs of one memory pool are
+    replayed in turn, on a stream of their own, beside eager calls."""
+    from kllm_b200 import kernels
+    H, G, hd = 32, 8, 128
+    c = Cache([8000], [64], G, hd, 64, seed=29)
+    one = Cache([20010], [1], 1, hd, 16, seed=30)
+    assert kernels.decode_q8_parts(1, 1, 4, hd, 20011)[0] > 1 and kernels.prefill_q8_parts(64, 1, G, H // G, 8064, hd)[1] > 1
+    rows, row = queries(64, H, hd, "bf16", 31), queries(1, 4, hd, "bf16", 32)
+    q_start, start, pos = ints(0, 64), ints(8000), ints(20010)
+    outs = [torch.zeros(64, H * hd, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 4 * hd, dtype=torch.bfloat16, device="cuda")]
+
+    def portion(out):
+        kernels.attention_prefill_q8(out, rows, c.k, c.v, c.ks, c.vs, q_start, start, c.dev_table, 1, H, G, hd, 0, 0.08, 8064)
+
+    def single(out):
+        kernels.attention_decode_q8(out, row, one.k, one.v, one.ks, one.vs, pos, None, one.dev_table, 4, 1, hd, 0, 0.08, 20011)
+    eager = [torch.zeros_like(t) for t in outs]
+    portion(eager[0]), single(eager[1])
+    torch.cuda.synchronize()
+    graphs, pool = [], torch.cuda.graph_pool_handle()
+    for call, out in zip((portion, single), outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            call(out)
+    side, again = torch.cuda.Stream(), [torch.zeros_like(t) for t in outs]
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for t in outs + again:
+            t.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+            graphs[1].replay()
+        portion(again[0]), single(again[1])
+        torch.cuda.current_stream().wait_stream(side)
+        for got, eag, want in zip(outs, again, eager):
+            assert torch.equal(got, want) and torch.equal(eag, want)
+
+
+def test_stores_of_more_than_32_bits():
+    """Pages whose bytes lie beyond 2^32 of a store: what is appended there is read from there."""
+    from kllm_b200 import kernels
+    H, G, hd, ps = 8, 8, 128, 64
+    pages = (2 ** 32) // (G * ps * hd) + 40
+    small = Cache([100], [30], G, hd, ps, seed=33)
+    far = torch.tensor([[pages - 1, pages - 7, pages - 30]], dtype=torch.int32)
+    k, v = (torch.zeros(pages, G, ps, hd, dtype=torch.uint8, device="cuda").view(plain.E4M3) for _ in range(2))
+    ks, vs = (torch.ones(pages, G, device="cuda") for _ in range(2))
+    x = [queries(130, G, hd, "bf16", 34 + i) for i in range(2)]
+    pos = torch.arange(130, dtype=torch.int32, device="cuda")
+    rows, turned = queries(130, H, hd, "bf16", 36), torch.zeros(130, H * hd, dtype=torch.bfloat16, device="cuda")
+    outs = []
+    for kc, vc, kss, vss, table in ((small.k, small.v, small.ks, small.vs, small.dev_table), (k, v, ks, vs, far.cuda())):
+        kernels.rope_append_q8(turned, rows, x[0], x[1], table_of_angles(130, hd), pos, torch.zeros_like(pos), ints(0, 130), table, kc, vc,
+                               kss, vss, H, G, hd)
+        for dt in DT.values():
+            q = turned.to(dt)
+            out, one = torch.zeros_like(q), torch.zeros_like(q[:1])
+            kernels.attention_prefill_q8(out, q, kc, vc, kss, vss, ints(0, 130), ints(0), table, 1, H, G, hd, 0, 0.09, 130)
+            kernels.attention_decode_q8(one, q[129:], kc, vc, kss, vss, ints(129), None, table, H, G, hd, 0, 0.09, 130)
+            outs.append((kc.view(torch.uint8)[table[0].long()], vc.view(torch.uint8)[table[0].long()], out, one))
+    for near, there in zip(outs[:2], outs[2:]):
+        assert bool(there[2].any())
+        for i, (a, b) in enumerate(zip(near, there)):
+            if i < 2:          # the last page's slots behind the 130th are not written
+                a, b = (t.transpose(1, 2).reshape(3 * ps, G, hd)[:130] for t in (a, b))
+            assert torch.equal(a, b)
+    assert not bool(k.view(torch.uint8)[:pages - 40].any()) and not bool(v.view(torch.uint8)[:pages - 40].any())
+
+
+def test_refuses_another_device_and_too_many_rows(monkeypatch):
+    from kllm_b200 import kernels
+    from kllm_b200.kernels import KernelError
+    H, G, hd = 4, 1, 64
+    c = Cache([10], [1], G, hd, 16, seed=37)
+    rows, kv = queries(1, H, hd, "bf16", 38), queries(1, G, hd, "bf16", 39)
+    calls = [lambda: decode(c, rows, ints(10), H, G, hd), lambda: prefill(c, rows, [10], [1], H, G, hd),
+             lambda: kernels.rope_append_q8(rows, rows, kv, kv, None, ints(10), None, ints(0, 1), c.dev_table, c.k, c.v, c.ks, c.vs, H, G, hd)]
+    many = torch.zeros(65536, H * hd, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(KernelError, match="at most 65535"):
+        decode(c, many, torch.zeros(65536, dtype=torch.int32, device="cuda"), H, G, hd, req=torch.zeros(65536, dtype=torch.int32, device="cuda"))
+    held = c.vs
+    c.vs = held.cpu()
+    for call in calls:
+        with pytest.raises(KernelError, match="not on a CUDA device"):
+            call()
+    c.vs = held
+    here = torch.cuda.current_device()
+    with monkeypatch.context() as m:
+        m.setattr(torch._C, "_cuda_getDevice", lambda: here + 1)
+        for call in calls:
+            with pytest.raises(KernelError, match="another than the current one"):
+                call()
+    for call in calls:
+        call()

@@ -201,3 +201,24 @@ def test_options_name_it():
     assert Options().fill().cache_dtype == "" and Options(cache_dtype="float8_e4m3fn").fill().cache_dtype == "float8_e4m3fn"
     with pytest.raises(ValueError, match="cache dtype"):
         Options(cache_dtype="int8").fill()
+
+
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("shape", [(-1,), (1, N, -1)])
+def test_queries_that_are_no_matrix(call, shape):
+    o = operands()
+    o.update(q=o["q"].view(*shape), out=o["out"].view(*shape))
+    with pytest.raises(KernelError, match="n, heads"):
+        CALLS[call](o)
+
+
+def test_angles_that_are_no_matrix():
+    o = operands()
+    o.update(cos_sin=o["cos_sin"].view(-1))
+    with pytest.raises(KernelError, match="cos_sin"):
+        append(o)
+
+
+@pytest.mark.parametrize("window,kept", [(None, 0), (0, 0), (-3, 0), (7, 7), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (2 ** 40 + 5, 2 ** 31 - 1)])
+def test_windows_fit_the_kernels_integers(window, kept):
+    assert kernels._q8_window(window) == kept
