@@ -646,22 +646,21 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
     __shared__ float s_mul[PRE_KEYS], s_ev[PRE_KEYS], s_inv[PRE_KEYS];   // per key: 2^ek, ev (-inf: not there), 2^-ev
     __shared__ int s_row[PRE_KEYS];
     __shared__ float s_factor[PRE_ROWS];
-    __shared__ int s_req, s_tok0;
+    __shared__ Portion s_portion;
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
     const int kvh = blockIdx.x % a.n_kv, gs = a.n_heads / a.n_kv;
     if (warp == 0) {
-        int req = -1, tok0 = 0;                           // longest key ranges first
-        if (!find_portion(a.q_start, a.n_requests, a.tokens_per_tile, (gridDim.x - 1 - blockIdx.x) / a.n_kv, req, tok0)) req = -1;
-        if (lane == 0) { s_req = req; s_tok0 = tok0; }
+        Portion p;                                        // longest key ranges first
+        if (!find_portion(a.q_start, a.start_pos, a.n_requests, a.tokens_per_tile, (gridDim.x - 1 - blockIdx.x) / a.n_kv, p)) p.req = -1;
+        if (lane == 0) s_portion = p;
     }
     __syncthreads();
-    const int req = s_req, tok0 = s_tok0;
+    const int req = s_portion.req, tok0 = s_portion.tok0, pos0 = s_portion.pos0;
     if (req < 0) return;                                  // the grid is an upper bound on the tiles
-    const int n_tok = min(min(a.tokens_per_tile, a.q_start[req + 1] - tok0), a.n_tokens - tok0);
+    const int n_tok = min(min(a.tokens_per_tile, s_portion.end - tok0), a.n_tokens - tok0);
     if (n_tok <= 0) return;
-    const int pos0 = a.start_pos[req] + (tok0 - a.q_start[req]);
     const int lo = (a.window > 0 && pos0 >= a.window) ? pos0 - a.window + 1 : 0;
     const int hi = keys_end((int64_t)pos0 + n_tok, a.max_blocks, a.page_size);
     const int* table = a.block_table + (int64_t)req * a.max_blocks;

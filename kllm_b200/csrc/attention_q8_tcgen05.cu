@@ -72,6 +72,7 @@ static_assert(PLANS + STAGES < NOTES, "notes");
 constexpr int PIECES = HD / 16;            // 16-byte pieces of a stored row
 constexpr int LOADS = TILE * PIECES / LOADERS;           // pieces of the keys (of the values) a loader thread carries
 constexpr int KEY_STEP = LOADERS / PIECES;               // its pieces' keys are so far apart
+constexpr int ROW_LANES = HD / 8, ROWS_AT_ONCE = 32 / ROW_LANES;   // rows of 16-bit numbers as a warp reads and writes them
 constexpr int E_SPAN = 7;                  // how far a key's exponents may be from its step's
 
 // What the planner says of a step to everybody.  The note of step t is written once the values of step t - PLANS are converted,
@@ -128,6 +129,11 @@ __device__ __forceinline__ void tmem_st8(unsigned taddr, const float (&v)[8]) {
 }
 __device__ __forceinline__ void store16(unsigned addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared16(unsigned addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 __device__ __forceinline__ uint32_t half2_times(uint32_t x, uint32_t m) {
     uint32_t r;
@@ -225,27 +231,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
     static_assert(alignof(Plan) == 16 && sizeof(Plan) % 16 == 0, "four words at a time");
     __shared__ unsigned s_tmem;
     __shared__ volatile Work s_work;
-    __shared__ int2 s_place;
     __shared__ int s_abort;
     const int warp = warp_index(), lane = threadIdx.x & 31;
     griddep_wait();
     griddep_launch();
     if (warp == 0) {
         // CTAs start in the order of blockIdx.x: longest key ranges first, all kv heads and parts of a range side by side
-        const int per_cta = a.tokens_per_tile * a.row_tiles;
-        int req = -1, tok0 = 0;
-        if (!find_portion(a.q_start, a.n_requests, per_cta, (gridDim.x - 1 - blockIdx.x) / (a.n_kv * a.splits), req, tok0)) req = -1;
-        if (lane == 0) s_place = make_int2(req, tok0);
-        __syncwarp();
-    }
-    if (threadIdx.x == 0) {
-        const int per_cta = a.tokens_per_tile * a.row_tiles, split = blockIdx.x % a.splits, tok0 = s_place.y;
-        int req = s_place.x;
-        const int first_row = req >= 0 ? a.q_start[req] : 0, end = req >= 0 ? min(a.q_start[req + 1], a.n_tokens) : 0;
-        if (req >= 0 && end <= tok0) req = -1;
-        s_work.req = req;
-        if (req >= 0) {
-            const int n_tok = min(per_cta, end - tok0), pos0 = a.start_pos[req] + (tok0 - first_row);
+        const int per_cta = a.tokens_per_tile * a.row_tiles, split = blockIdx.x % a.splits;
+        Portion p;
+        if (!find_portion(a.q_start, a.start_pos, a.n_requests, per_cta, (gridDim.x - 1 - blockIdx.x) / (a.n_kv * a.splits), p)) p.req = -1;
+        const int tok0 = p.tok0, pos0 = p.pos0, n_tok = p.req >= 0 ? min(per_cta, min(p.end, a.n_tokens) - tok0) : 0;
+        if (lane == 0) s_work.req = n_tok > 0 ? p.req : -1;
+        if (lane == 0 && n_tok > 0) {
             const int hi = max(keys_end((int64_t)pos0 + n_tok, a.max_blocks, a.page_size), 1);
             // one tile at least: every role takes at least one step (a window behind the table's end sees nothing in it)
             const int lo = min((a.window > 0 && pos0 >= a.window) ? pos0 - a.window + 1 : 0, hi - 1);
@@ -260,6 +257,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             s_work.tile_lo = first + min(all, split * per);
             s_work.tile_hi = first + min(all, (split + 1) * per);
         }
+    }
+    if (threadIdx.x == 32) {
         s_abort = 0;
         for (int i = 0; i < STAGES; i++) {
             mbar_init(&bar_k_full[i], LOADERS); mbar_init(&bar_k_empty[i], 1);
@@ -274,8 +273,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
         for (int i = 0; i < PLANS; i++) { mbar_init(&bar_plan_full[i], 32); mbar_init(&bar_plan_empty[i], 2 * LOADERS); }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    __syncthreads();
-    if (s_work.req < 0) return;                // the grid is an upper bound on the tiles
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -283,8 +280,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const unsigned abort_at = smem_u32(&s_abort);
     volatile unsigned* tmem_at = &s_tmem;
+    if (s_work.req < 0) {                      // the grid is an upper bound on the tiles
+        if (warp == 16)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(__shfl_sync(0xffffffffu, *tmem_at, 0)), "r"(TMEM_COLS));
+        return;
+    }
+    const unsigned abort_at = smem_u32(&s_abort);
     const bool nothing = s_work.tile_lo >= s_work.tile_hi;
     // swizzled tiles want 1024-byte alignment
     auto shared_base = [&]() { return (smem_u32(smem_raw) + 1023u) & ~1023u; };
@@ -553,38 +555,49 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
         bool ok = x < tiles && !nothing;
         if (ok) {
             // the row's queries: float16, its power of two in the factor, the scale's sign in the numbers
-            const bf16* q = a.q + (int64_t)(tok0 + tt) * a.q_stride + (int64_t)(kvh * gs + hh) * HD;
-            uint32_t w[HD / 2];
-            int m = 0;
+            // A warp reads its 32 rows together, ROW_LANES lanes a row (a thread per row took 10400 cycles at head size 128, and
+            // the loaders' first tile waited behind it).
+            const int64_t own = (int64_t)(tok0 + (valid ? tt : 0)) * a.q_stride + (int64_t)(kvh * gs + (valid ? hh : 0)) * HD;
+            const int piece = lane % ROW_LANES;
+            uint4 w[ROW_LANES];
+            bool there[ROW_LANES];
 #pragma unroll
-            for (int i = 0; i < HD / 8; i++) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (valid) {
-                    if (a.q_by_eight) {
-                        v = *reinterpret_cast<const uint4*>(q + i * 8);
-                    } else {
-                        const unsigned short* h = reinterpret_cast<const unsigned short*>(q + i * 8);
-                        v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
-                    }
+            for (int i = 0; i < ROW_LANES; i++) {
+                const int from = i * ROWS_AT_ONCE + lane / ROW_LANES;
+                const bf16* src = a.q + __shfl_sync(0xffffffffu, own, from) + piece * 8;
+                there[i] = __shfl_sync(0xffffffffu, valid, from);
+                if (a.q_by_eight) {
+                    w[i] = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
+                    w[i] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
                 }
-                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-#pragma unroll
-                for (int j = 0; j < 4; j++) m = max(m, max((int)(w[4 * i + j] & 0x7fffu) << 16, (int)(w[4 * i + j] & 0x7fff0000u)));
             }
-            const bool finite = m < 0x7f800000;
-            const float up = finite ? copysignf(q8_pow2(row_shift(m)), a.scale) : 0.f;
-            const float factor = finite ? fabsf(a.scale) * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);
             const unsigned dst = shared_base() + x * Q_BYTES;
+            int m = 0;                                                       // of this thread's row
 #pragma unroll
-            for (int i = 0; i < HD / 8; i++) {
-                uint32_t h[4];
+            for (int i = 0; i < ROW_LANES; i++) {
+                uint32_t h[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                int mr = 0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t two = finite ? w[4 * i + j] : 0u;
+                    if (!there[i]) h[j] = 0;
+                    mr = max(mr, max((int)(h[j] & 0x7fffu) << 16, (int)(h[j] & 0x7fff0000u)));
+                }
+#pragma unroll
+                for (int d = 1; d < ROW_LANES; d <<= 1) mr = max(mr, __shfl_xor_sync(0xffffffffu, mr, d));
+                const int given = __shfl_sync(0xffffffffu, mr, (lane % ROWS_AT_ONCE) * ROW_LANES);
+                if (lane / ROWS_AT_ONCE == i) m = given;
+                const bool finite = mr < 0x7f800000;
+                const float up = finite ? copysignf(q8_pow2(row_shift(mr)), a.scale) : 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t two = finite ? h[j] : 0u;
                     h[j] = q8_half2(__uint_as_float(two << 16) * up, __uint_as_float(two & 0xffff0000u) * up);
                 }
-                store16(dst + (unsigned)((i >> 3) * PANEL) + swz(r, i & 7), h[0], h[1], h[2], h[3]);
+                store16(dst + (unsigned)((piece >> 3) * PANEL) + swz((warp & 3) * 32 + i * ROWS_AT_ONCE + lane / ROW_LANES, piece & 7), h[0], h[1], h[2], h[3]);
             }
+            const float factor = m < 0x7f800000 ? fabsf(a.scale) * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);
             fence_async_smem();
             arrive_at(smem_u32(&bar_q_full[x]));
             bool last = false;
@@ -593,6 +606,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             for (; ok && !last; step++) {
                 ok = wait_at(smem_u32(&bar_note[step % NOTES]), (unsigned)(step / NOTES) & 1u, abort_at, a.status, 8) &&
                      wait_at(smem_u32(&bar_s_full[buf]), parity, abort_at, a.status, 9);
+                ok = __all_sync(0xffffffffu, ok);             // a warp leaves together, if it does
                 if (!ok) break;
                 const unsigned t_s = t_s0 + buf * TILE;
                 tc_fence_after();
@@ -640,7 +654,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 // the phase behind the one waited for last).
                 if (step > 0) {
                     if (SBUFS != 2 || tiles != 2) {
-                        ok = wait_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 10);
+                        ok = wait_warp_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 10);
                         if (!ok) break;
                     }
                     if (__any_sync(0xffffffffu, move)) {
@@ -684,32 +698,53 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 buf += tiles;
                 if (buf >= SBUFS) { buf -= SBUFS; parity ^= 1u; }
             }
-            if (ok) ok = wait_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 11);
+            if (ok) ok = wait_warp_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 11);
             if (ok) {
                 tc_fence_after();
-#pragma unroll
-                for (int cb = 0; cb < HD / 32; cb++) {
-                    float t[32];
-                    tmem_ld32(t_o + cb * 32, t);
-                    tmem_ld_wait();
-                    if (!valid) continue;
+                // The rows go through the queries' place in shared memory (their products are through), a warp's 32 by itself, so that
+                // neighbouring lanes store neighbouring bytes: 16-byte pieces of a row's 2 HD bytes, XORed with the row as the
+                // queries were.  Float32 parts take two passes.
+                const unsigned rows_at = shared_base() + x * Q_BYTES + (warp & 3) * 32 * (HD * 2);
+                const float inv = a.splits > 1 ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
+                const int passes = a.splits > 1 ? 2 : 1;
+                unsigned char* const rows_out = a.splits > 1 ? reinterpret_cast<unsigned char*>(a.part_o) : reinterpret_cast<unsigned char*>(a.out);
+                const int64_t own = a.splits > 1 ? (at * a.splits + split) * (HD * 4) : at * (HD * 2);
+#pragma unroll 1
+                for (int pass = 0; pass < passes; pass++) {
                     if (a.splits == 1) {
-                        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
 #pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            uint4 pk;
-                            pk.x = pack_bf16(t[8 * c] * inv, t[8 * c + 1] * inv);
-                            pk.y = pack_bf16(t[8 * c + 2] * inv, t[8 * c + 3] * inv);
-                            pk.z = pack_bf16(t[8 * c + 4] * inv, t[8 * c + 5] * inv);
-                            pk.w = pack_bf16(t[8 * c + 6] * inv, t[8 * c + 7] * inv);
-                            *reinterpret_cast<uint4*>(a.out + at * HD + cb * 32 + 8 * c) = pk;
+                        for (int cb = 0; cb < HD / 32; cb++) {
+                            float t[32];
+                            tmem_ld32(t_o + cb * 32, t);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                store16(rows_at + lane * (HD * 2) + (((cb * 4 + c) ^ (lane & 7)) << 4),
+                                        pack_bf16(t[8 * c] * inv, t[8 * c + 1] * inv), pack_bf16(t[8 * c + 2] * inv, t[8 * c + 3] * inv),
+                                        pack_bf16(t[8 * c + 4] * inv, t[8 * c + 5] * inv), pack_bf16(t[8 * c + 6] * inv, t[8 * c + 7] * inv));
                         }
                     } else {
-                        float* part = a.part_o + (at * a.splits + split) * HD + cb * 32;
 #pragma unroll
-                        for (int c = 0; c < 8; c++)
-                            *reinterpret_cast<float4*>(part + 4 * c) = make_float4(t[4 * c], t[4 * c + 1], t[4 * c + 2], t[4 * c + 3]);
+                        for (int cb = 0; cb < HD / 64; cb++) {
+                            float t[32];
+                            tmem_ld32(t_o + pass * (HD / 2) + cb * 32, t);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int c = 0; c < 8; c++)
+                                store16(rows_at + lane * (HD * 2) + (((cb * 8 + c) ^ (lane & 7)) << 4), __float_as_uint(t[4 * c]),
+                                        __float_as_uint(t[4 * c + 1]), __float_as_uint(t[4 * c + 2]), __float_as_uint(t[4 * c + 3]));
+                        }
                     }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < ROW_LANES; i++) {
+                        const int row = i * ROWS_AT_ONCE + lane / ROW_LANES, piece = lane % ROW_LANES;
+                        const int64_t to = __shfl_sync(0xffffffffu, own, row);
+                        const bool there = __shfl_sync(0xffffffffu, valid, row);
+                        const uint4 v = load_shared16(rows_at + row * (HD * 2) + ((piece ^ (row & 7)) << 4));
+                        if (there) *reinterpret_cast<uint4*>(rows_out + to + pass * (HD * 2) + piece * 16) = v;
+                    }
+                    __syncwarp();
                 }
             }
         } else if (valid && nothing) {

@@ -112,28 +112,46 @@ template <typename T> __device__ __forceinline__ void store_row4(T* dst, const f
     }
 }
 
-// A request's portion and its rows' tile: the tile'th of the tiles of `per` rows into which the requests' portions
-// q_start[s] .. q_start[s + 1] are cut one after another.  By a whole warp, a request a lane (400 requests of 2
-// tokens behind 100: 101 us, with a walk by one thread 322).  False: there are fewer tiles.
-__device__ __forceinline__ bool find_portion(const int* q_start, int n_requests, int per, int tile, int& req, int& tok0) {
+// The tile'th of the tiles of `per` rows into which the requests' portions, rows q_start[s] .. q_start[s + 1], are cut.  Where the
+// requests are no more than lanes, their portions come one after another in the order of their contexts' ends, the longest
+// last (kernels start with the last tile: what takes long begins first), else as they stand.
+struct Portion {
+    int req, tok0, end, pos0;            // request, the tile's first row, the portion's end, the first row's position
+};
+// By a whole warp, a request a lane (400 requests of 2 tokens behind 100: 101 us, with a walk by one thread 322).  False: there are
+// fewer tiles.
+__device__ __forceinline__ bool find_portion(const int* q_start, const int* start_pos, int n_requests, int per, int tile, Portion& p) {
     const int lane = threadIdx.x & 31;
     for (int s0 = 0; s0 < n_requests; s0 += 32) {
-        const int s = s0 + lane, begin = s < n_requests ? q_start[s] : 0, rows = s < n_requests ? q_start[s + 1] - begin : 0;
-        const int mine = rows > 0 ? (rows + per - 1) / per : 0;
-        int upto = mine;                                     // tiles of this group of requests up to the lane's own
+        const int s = s0 + lane;
+        const bool there = s < n_requests;
+        const int begin = there ? q_start[s] : 0, end = there ? q_start[s + 1] : 0, start = there ? start_pos[s] : 0;
+        const int rows = end - begin, mine = rows > 0 ? (rows + per - 1) / per : 0;
+        int upto = mine;                                     // tiles up to the lane's last
+        if (n_requests <= 32) {
+            upto = 0;
+            const int ctx = start + rows;
+            for (int j = 0; j < n_requests; j++) {
+                const int other = __shfl_sync(0xffffffffu, ctx, j), tiles = __shfl_sync(0xffffffffu, mine, j);
+                if (other < ctx || (other == ctx && j <= lane)) upto += tiles;
+            }
+        } else {
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int before = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += before;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int before = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += before;
+            }
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, tile < upto);
+        const unsigned hit = __ballot_sync(0xffffffffu, tile < upto && tile >= upto - mine);
         if (hit) {
-            const int l = __ffs(hit) - 1;
-            req = s0 + l;
-            tok0 = __shfl_sync(0xffffffffu, begin + (tile - (upto - mine)) * per, l);
+            const int l = __ffs(hit) - 1, into = (tile - (upto - mine)) * per;
+            p.req = s0 + l;
+            p.tok0 = __shfl_sync(0xffffffffu, begin + into, l);
+            p.end = __shfl_sync(0xffffffffu, end, l);
+            p.pos0 = __shfl_sync(0xffffffffu, start + into, l);
             return true;
         }
-        tile -= __shfl_sync(0xffffffffu, upto, 31);
+        tile -= __reduce_add_sync(0xffffffffu, mine);
     }
     return false;
 }
