@@ -130,6 +130,16 @@ __device__ __forceinline__ void tmem_st8(unsigned taddr, const float (&v)[8]) {
 __device__ __forceinline__ void store16(unsigned addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// 16 bytes, or as many zeros
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 __device__ __forceinline__ uint4 load_shared16(unsigned addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -555,49 +565,51 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
         bool ok = x < tiles && !nothing;
         if (ok) {
             // the row's queries: float16, its power of two in the factor, the scale's sign in the numbers
-            // A warp reads its 32 rows together, ROW_LANES lanes a row (a thread per row took 10400 cycles at head size 128, and
-            // the loaders' first tile waited behind it).
-            const int64_t own = (int64_t)(tok0 + (valid ? tt : 0)) * a.q_stride + (int64_t)(kvh * gs + (valid ? hh : 0)) * HD;
+            // A warp brings its 32 rows as they are into their places, ROW_LANES lanes a row; then a thread turns its row into float16
+            // where it lies.  In short loops: this runs once a CTA, and what is unrolled waits for its instructions to be
+            // fetched (16 loads and their shuffles 2200 cycles, the rest 3900 at head size 128).
+            const unsigned rows_at = shared_base() + x * Q_BYTES;
+            const int64_t own = valid ? (int64_t)(tok0 + tt) * a.q_stride + (int64_t)(kvh * gs + hh) * HD : -1;
             const int piece = lane % ROW_LANES;
-            uint4 w[ROW_LANES];
-            bool there[ROW_LANES];
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < ROW_LANES; i++) {
                 const int from = i * ROWS_AT_ONCE + lane / ROW_LANES;
-                const bf16* src = a.q + __shfl_sync(0xffffffffu, own, from) + piece * 8;
-                there[i] = __shfl_sync(0xffffffffu, valid, from);
+                const int64_t off = __shfl_sync(0xffffffffu, own, from);
+                const unsigned to = rows_at + (unsigned)((piece >> 3) * PANEL) + swz((warp & 3) * 32 + from, piece & 7);
+                const bf16* src = a.q + (off < 0 ? 0 : off) + piece * 8;
                 if (a.q_by_eight) {
-                    w[i] = *reinterpret_cast<const uint4*>(src);
+                    copy16(to, src, off >= 0);
                 } else {
                     const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
-                    w[i] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (off >= 0) v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+                    store16(to, v.x, v.y, v.z, v.w);
                 }
             }
-            const unsigned dst = shared_base() + x * Q_BYTES;
-            int m = 0;                                                       // of this thread's row
-#pragma unroll
-            for (int i = 0; i < ROW_LANES; i++) {
-                uint32_t h[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                int mr = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (!there[i]) h[j] = 0;
-                    mr = max(mr, max((int)(h[j] & 0x7fffu) << 16, (int)(h[j] & 0x7fff0000u)));
-                }
-#pragma unroll
-                for (int d = 1; d < ROW_LANES; d <<= 1) mr = max(mr, __shfl_xor_sync(0xffffffffu, mr, d));
-                const int given = __shfl_sync(0xffffffffu, mr, (lane % ROWS_AT_ONCE) * ROW_LANES);
-                if (lane / ROWS_AT_ONCE == i) m = given;
-                const bool finite = mr < 0x7f800000;
-                const float up = finite ? copysignf(q8_pow2(row_shift(mr)), a.scale) : 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t two = finite ? h[j] : 0u;
-                    h[j] = q8_half2(__uint_as_float(two << 16) * up, __uint_as_float(two & 0xffff0000u) * up);
-                }
-                store16(dst + (unsigned)((piece >> 3) * PANEL) + swz((warp & 3) * 32 + i * ROWS_AT_ONCE + lane / ROW_LANES, piece & 7), h[0], h[1], h[2], h[3]);
+            copies_wait();
+            __syncwarp();
+            uint32_t two = 0;                                                // the row's largest magnitudes at even and odd places
+#pragma unroll 4
+            for (int c = 0; c < HD / 8; c++) {
+                const uint4 v = load_shared16(rows_at + (unsigned)((c >> 3) * PANEL) + swz(r, c & 7));
+                two = max_u16x2(two, max_u16x2(max_u16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), max_u16x2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
             }
-            const float factor = m < 0x7f800000 ? fabsf(a.scale) * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);
+            const int m = (int)max(two << 16, two & 0xffff0000u);
+            const bool finite = m < 0x7f800000;
+            const float up = finite ? copysignf(q8_pow2(row_shift(m)), a.scale) : 0.f;
+#pragma unroll 2
+            for (int c = 0; c < HD / 8; c++) {
+                const unsigned to = rows_at + (unsigned)((c >> 3) * PANEL) + swz(r, c & 7);
+                const uint4 v = load_shared16(to);
+                uint32_t h[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (!finite) h[j] = 0;
+                    h[j] = q8_half2(__uint_as_float(h[j] << 16) * up, __uint_as_float(h[j] & 0xffff0000u) * up);
+                }
+                store16(to, h[0], h[1], h[2], h[3]);
+            }
+            const float factor = finite ? fabsf(a.scale) * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);
             fence_async_smem();
             arrive_at(smem_u32(&bar_q_full[x]));
             bool last = false;
@@ -712,7 +724,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
 #pragma unroll 1
                 for (int pass = 0; pass < passes; pass++) {
                     if (a.splits == 1) {
-#pragma unroll
+#pragma unroll 1
                         for (int cb = 0; cb < HD / 32; cb++) {
                             float t[32];
                             tmem_ld32(t_o + cb * 32, t);
@@ -724,7 +736,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                                         pack_bf16(t[8 * c + 4] * inv, t[8 * c + 5] * inv), pack_bf16(t[8 * c + 6] * inv, t[8 * c + 7] * inv));
                         }
                     } else {
-#pragma unroll
+#pragma unroll 1
                         for (int cb = 0; cb < HD / 64; cb++) {
                             float t[32];
                             tmem_ld32(t_o + pass * (HD / 2) + cb * 32, t);
@@ -736,7 +748,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                         }
                     }
                     __syncwarp();
-#pragma unroll
+#pragma unroll 2
                     for (int i = 0; i < ROW_LANES; i++) {
                         const int row = i * ROWS_AT_ONCE + lane / ROW_LANES, piece = lane % ROW_LANES;
                         const int64_t to = __shfl_sync(0xffffffffu, own, row);
