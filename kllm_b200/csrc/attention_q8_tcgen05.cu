@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             const unsigned rows_at = shared_base() + x * Q_BYTES;
             const int64_t own = valid ? (int64_t)(tok0 + tt) * a.q_stride + (int64_t)(kvh * gs + hh) * HD : -1;
             const int piece = lane % ROW_LANES;
-#pragma unroll 1
+#pragma unroll 4
             for (int i = 0; i < ROW_LANES; i++) {
                 const int from = i * ROWS_AT_ONCE + lane / ROW_LANES;
                 const int64_t off = __shfl_sync(0xffffffffu, own, from);
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             const int m = (int)max(two << 16, two & 0xffff0000u);
             const bool finite = m < 0x7f800000;
             const float up = finite ? copysignf(q8_pow2(row_shift(m)), a.scale) : 0.f;
-#pragma unroll 2
+#pragma unroll 4
             for (int c = 0; c < HD / 8; c++) {
                 const unsigned to = rows_at + (unsigned)((c >> 3) * PANEL) + swz(r, c & 7);
                 const uint4 v = load_shared16(to);
