@@ -596,8 +596,7 @@ int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t s
         return (int)e;
     }
     if (a.ranges > 1) {
-        kllm_launch((q8_join_kernel<T, HD>), dim3(n_tokens * a.n_heads), dim3(HD / 4), 0, stream, (T*)a.out, (const float*)a.part_o,
-                    (const float*)a.part_ml, a.ranges, a.n_heads, (const int*)nullptr, 0);
+        launch_join<T, HD>(a.out, a.part_o, a.part_ml, a.ranges, a.n_heads, (int64_t)n_tokens * a.n_heads, nullptr, 0, stream);
     }
     KLLM_LAUNCH_STATUS();
 }

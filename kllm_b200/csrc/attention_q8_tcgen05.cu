@@ -812,8 +812,7 @@ extern "C" int kllm_attention_prefill_q8_tcgen05(void* out, float* part_o, float
     if (ctas > 0x7fffffffLL) KLLM_FAIL("attention (8 bits, tcgen05): %lld CTAs", (long long)ctas);
     kllm_launch((attn_prefill_q8_tc5_kernel), dim3((unsigned)ctas), dim3(THREADS), SMEM_BYTES, (cudaStream_t)stream, a);
     if (splits > 1) {
-        kllm_launch((q8_join_kernel<bf16, HD>), dim3((unsigned)(n_tokens * n_heads)), dim3(HD / 4), 0, (cudaStream_t)stream, (bf16*)out,
-                    (const float*)part_o, (const float*)part_ml, splits, n_heads, q_start, n_requests);
+        launch_join<bf16, HD>(out, part_o, part_ml, splits, n_heads, (int64_t)n_tokens * n_heads, q_start, n_requests, (cudaStream_t)stream);
     }
     KLLM_LAUNCH_STATUS();
 }

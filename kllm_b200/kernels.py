@@ -1242,8 +1242,8 @@ def prefill_q8_parts(n_tokens: int, n_requests: int, n_kv: int, group: int, ctx_
     account, is least.  Measured at head size 128 (64): a CTA takes about 5 us to begin and end and, for every 128 keys, 1.6
     (1.4) us with one tile of 128 rows and 2.3 (1.8) with two; an SM holds one CTA; several parts cost about 4 us and their
     unscaled rows written and read once.  Microseconds, 32 heads, tiles x parts: 512 tokens behind 7680 over 8 kv heads of 128
-    1x1: 109, 2x1: 153, 2x2: 106, 2x4: 121; 64 behind 8000 1x1: 105, 1x8: 28, 1x16: 40; 300 alone 1x1: 13.3, 2x1: 17.4; 2048
-    alone over 4 of 64 1x1: 64, 2x1: 40."""
+    1x1: 108, 2x1: 148, 2x2: 88, 2x4: 100; 64 behind 8000 1x1: 105, 1x3: 45, 1x9: 29; 300 alone 1x1: 12.3, 2x1: 15.1; 2048
+    alone over 4 of 64 1x1: 64, 2x1: 39."""
     return _prefill_q8_parts(n_tokens, n_requests, n_kv, group, ctx_bound, head_dim, sm_count())
 
 
