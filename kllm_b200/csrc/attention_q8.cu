@@ -62,6 +62,12 @@ template <int N> __device__ __forceinline__ void split(float x, __half (&p)[N]) 
 // to the pairs that the operand wants, and the weights, whose layout is (key, head), become the B operand by an 8 x 8
 // transposition in registers (movmatrix).  Row r of a tile is key r ^ (r >> 1 & 1) of it, and the 16-byte pieces of key j lie
 // at piece ^ swizzle(j): with both, neither kind of read meets a bank twice at head sizes 64 and 128.
+//
+// Measured, back to back, bfloat16 (% of a copy's 6.45 TB/s): 64 requests of 846 to 4095 keys, 32 heads over 8 of 128, pages of 16: 67.6 us (74 %);
+// one of 131072 keys 53.8 us (77 %); 8 of 2048 keys, 32 over 4 of 64: 8.4 us; one: 6.2 us, a chain of launch, table, tiles and
+// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 18.9 us (35 %), bound by the products' parts (three for queries, two for
+// weights).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
+// 64 (16 of a CTA pair an SM as before): 64 x 2048 keys 18.7 us against 19.6, 128 x 1000 23.0 against 18.8.
 
 constexpr int DEC_KT = HD <= 128 ? 32 : 16;              // keys of a warp's tile
 constexpr int DEC_MT = DEC_KT / 16;
@@ -607,6 +613,11 @@ int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t s
 // in tiles of 64.  A tile is converted to float16 once, on its way into shared memory, and read from there by all warps
 // as operands (ldmatrix); the next tile's bytes are in registers meanwhile.  Weights go from the first product's result to
 // the second's operand in registers.
+//
+// This form serves float32 and the head sizes that attention_q8_tcgen05.cu does not; its products are bound by mma.sync and by the
+// chain of a warp's 16 rows.  Measured, one prompt alone, back to back: float32, 2048 tokens of 32 heads over 4 of 64 164 us (105 TFLOP/s
+// counted once; the parts make three products and two of every one), over 8 of 128 294 us (117); 333 tokens 21.6 us (six tiles one
+// behind the other); bfloat16, 2048 tokens of 24 heads over 8 of 96 111 us (174), 16 over 8 of 256 223 us (154).
 
 constexpr int PRE_ROWS = 64, PRE_KEYS = 64, PRE_THREADS = 128;
 constexpr int PRE_LD = HD + 8;                            // halves of a row in shared memory: eight rows on eight bank groups

@@ -29,6 +29,13 @@
 // accumulator is read, rescaled and written back between two products).  Few row tiles behind a long context are cut
 // over the keys: every part leaves its unscaled rows, references and sums, which a second kernel joins in order.
 //
+// Measured, back to back: one prompt of 8192 tokens, 32 heads over 4 of 64: 416 us (661 TFLOP/s), over 8 of 128: 558 us (985, 59 % of a
+// library product's 1671); 2048 tokens: 39 and 53 us; 512 behind 7680 over 8 of 128: 88 us.  A step of two row tiles takes 4300 cycles at
+// head size 128 (3300 at 64), of which the tensor core is busy for 2048 (1024) and the exponentials for 2048: a row tile's own chain of
+// scores, maximum, exponentials (1700, at 16 a cycle 1024 alone) and product bounds it, with two softmax warps a scheduler to
+// interleave.  Slower: two threads a row (8192 tokens, head size 64: 525 us against 419), a cubic for some of the exponentials (446 to
+// 518), loads of scores overlapped with their maximum (428), weights handed over whole at head size 128 (652 against 620).
+//
 // Every wait on an mbarrier is bounded by a cycle count: a wait that runs out raises a flag in shared memory and sets the
 // status word, every role leaves its loop, and the CTA frees its TMEM and returns.
 #include "q8.cuh"
