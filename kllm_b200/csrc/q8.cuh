@@ -130,7 +130,7 @@ __device__ __forceinline__ bool find_portion(const int* q_start, const int* star
     for (int s0 = 0; s0 < n_requests; s0 += 32) {
         const int s = s0 + lane;
         const bool there = s < n_requests;
-        const int begin = there ? q_start[s] : 0, end = there ? q_start[s + 1] : 0, start = there ? start_pos[s] : 0;
+        const int begin = there ? max(q_start[s], 0) : 0, end = there ? q_start[s + 1] : 0, start = there ? start_pos[s] : 0;
         const int rows = end - begin, mine = rows > 0 ? (rows + per - 1) / per : 0;
         int upto = mine;                                     // tiles up to the lane's last
         if (n_requests <= 32) {
@@ -161,9 +161,10 @@ __device__ __forceinline__ bool find_portion(const int* q_start, const int* star
     return false;
 }
 
-// The end of the keys that a table of max_blocks pages can name, at most hi: a position behind the table costs no walk there.
+// The end of the keys that a table of max_blocks pages can name, at most hi: a position behind the table costs no walk there.  A few
+// tiles below 2^31, so that the places of the tiles that are looked up ahead are numbers too.
 __device__ __forceinline__ int keys_end(int64_t hi, int max_blocks, int page_size) {
-    const int64_t end = (int64_t)max_blocks * page_size;
+    const int64_t table = (int64_t)max_blocks * page_size, end = table < 0x7ffff000 ? table : 0x7ffff000;
     return (int)(hi < end ? hi : end);
 }
 

@@ -1270,8 +1270,8 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
                          n_requests: int, n_heads: int, n_kv: int, head_dim: int, window: int, scale: float,
                          ctx_bound: int) -> None:
     """Attention of portions over a cache in 8 bits: request s brings rows q_start[s]..q_start[s+1] that start at cache
-    position start_pos[s]; their own keys are in the cache already.  Otherwise as ``attention_decode_q8``; rows that belong
-    to no request are left as they are."""
+    position start_pos[s]; their own keys are in the cache already.  Otherwise as ``attention_decode_q8``, with at most 64 heads
+    over a kv head (128 in bfloat16 at head sizes 64 and 128); rows that belong to no request are left as they are."""
     _check_q8("attention_prefill_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
     code, n, stride = _check_q8_rows("attention_prefill_q8", out, q, n_heads, head_dim)
     _check_q8_ints("attention_prefill_q8", q_start, start_pos)

@@ -685,3 +685,21 @@ def test_refuses_another_device_and_too_many_rows(monkeypatch):
                 call()
     for call in calls:
         call()
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_starts_outside_the_rows(dtype):
+    """Portions that begin before the first row or end behind the last read and write nothing there."""
+    from kllm_b200 import kernels
+    H, G, hd = 4, 2, 64
+    c = Cache([20, 20, 20], [40, 40, 40], G, hd, 16, seed=41)
+    rows = queries(12, H, hd, dtype, 42)
+    room = torch.full((36, H * hd), 7.0, dtype=rows.dtype, device="cuda")
+    out = room[12:24]
+    kernels.attention_prefill_q8(out, rows, c.k, c.v, c.ks, c.vs, ints(-9, 4, 8, 900), ints(20, 20, 20), c.dev_table, 3, H, G, hd, 0, 0.1, 60)
+    assert bool((room[:12] == 7.0).all()) and bool((room[24:] == 7.0).all()) and bool((out != 7.0).any(dim=1).all())
+    kept = [t.view(torch.uint8).clone() for t in (c.k, c.v)]
+    kv = queries(12, G, hd, dtype, 43)
+    pos = ints(*[3] * 12)
+    kernels.rope_append_q8(rows, rows, kv, kv, None, pos, ints(*[0] * 12), ints(5, -3), c.dev_table, c.k, c.v, c.ks, c.vs, H, G, hd)
+    assert torch.equal(kept[0], c.k.view(torch.uint8)) and torch.equal(kept[1], c.v.view(torch.uint8))
