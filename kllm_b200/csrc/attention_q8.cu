@@ -159,6 +159,11 @@ __device__ __forceinline__ unsigned cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
 }
+// ... for the end of a kernel: orders no memory, where the release above waits for the rows just stored (2400 cycles of a call of 10700).  What
+// was read from the others has arrived: it was stored.
+__device__ __forceinline__ void cluster_leave() {
+    asm volatile("barrier.cluster.arrive.relaxed;\nbarrier.cluster.wait;\n" ::: "memory");
+}
 __device__ __forceinline__ unsigned peer_addr(const void* p, unsigned rank) {
     unsigned b;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(b) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
@@ -570,7 +575,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.ranges + range) * 2) = make_float2(m, l);
         }
     }
-    if (C > 1) cluster_sync();           // nobody leaves while another still reads its shared memory
+    if (C > 1) cluster_leave();          // nobody leaves while another still reads its shared memory
 }
 
 template <typename T, int NG>
