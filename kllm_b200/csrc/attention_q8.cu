@@ -51,6 +51,15 @@ template <int N> __device__ __forceinline__ void split(float x, __half (&p)[N]) 
     }
 }
 
+// part i, 0 behind the last
+template <int N> __device__ __forceinline__ __half pick(const __half (&p)[N], int i) {
+    __half x = __ushort_as_half(0);
+#pragma unroll
+    for (int j = 0; j < N; j++)
+        if (i == j) x = p[j];
+    return x;
+}
+
 // ---- single tokens ---------------------------------------------------------------------------------------------------
 //
 // What bounds it: bytes.  Every warp walks its own tiles of keys, which it requests ahead into a ring of its own in shared
@@ -64,9 +73,8 @@ template <int N> __device__ __forceinline__ void split(float x, __half (&p)[N]) 
 // at piece ^ swizzle(j): with both, neither kind of read meets a bank twice at head sizes 64 and 128.
 //
 // Measured, back to back, bfloat16 (% of a copy's 6.45 TB/s): 64 requests of 846 to 4095 keys, 32 heads over 8 of 128, pages of 16: 67.6 us (74 %);
-// one of 131072 keys 53.8 us (77 %); 8 of 2048 keys, 32 over 4 of 64: 8.4 us; one: 6.2 us, a chain of launch, table, tiles and
-// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 18.9 us (35 %), bound by the products' parts (three for queries, two for
-// weights).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
+// one of 131072 keys 53.8 us (77 %); 8 of 2048 keys, 32 over 4 of 64: 8.2 us; one: 5.9 us, a chain of launch, table, tiles and
+// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 16.8 us (40 %; with the parts as products of their own 18.9).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
 // 64 (16 of a CTA pair an SM as before): 64 x 2048 keys 18.7 us against 19.6, 128 x 1000 23.0 against 18.8.
 
 constexpr int DEC_KT = HD <= 128 ? 32 : 16;              // keys of a warp's tile
@@ -86,8 +94,11 @@ __device__ __forceinline__ int dec_swizzle(int key) {
 }
 __device__ __forceinline__ int dec_key(int row) { return row ^ ((row >> 1) & 1); }
 
-template <typename T, int NG> struct DecodeShape {
-    static constexpr int NQ = Parts<T>::Q;
+// SPREAD: where a CTA has one or two heads of float32 queries, the parts of a head's queries, and of its weights, are columns
+// of the N side (part p of head h is column 2 p + h) instead of products of their own: a third of the first product's
+// instructions and half of the second's (32 heads of 128, 8 x 2048 keys: 35.0 us against 40.7).
+template <typename T, int NG, bool SPREAD> struct DecodeShape {
+    static constexpr int NQ = SPREAD ? 1 : Parts<T>::Q;
     static constexpr int QREGS = HD / 16 * 2 * NQ * NG;
     static constexpr bool Q_IN_REGS = QREGS <= 32;
     static constexpr int Q_BYTES = Q_IN_REGS ? 0 : HD / 16 * NQ * NG * 32 * 8;
@@ -181,12 +192,13 @@ __device__ __forceinline__ float4 peer_load4(const void* p, unsigned rank) {
 }
 // grid: (ranges * cluster, kv heads * subgroups of heads, tokens), clusters along x; a cluster's CTAs take neighbouring
 // parts of a range and join through distributed shared memory
-template <typename T, int NG>
-__global__ void __launch_bounds__(DEC_WARPS * 32, (DecodeShape<T, NG>::CTAS))
+template <typename T, int NG, bool SPREAD>
+__global__ void __launch_bounds__(DEC_WARPS * 32, (DecodeShape<T, NG, SPREAD>::CTAS))
 attn_decode_q8_kernel(const DecodeArgs a) {
-    constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P, NH = 8 * NG;
-    constexpr bool Q_IN_REGS = DecodeShape<T, NG>::Q_IN_REGS;
-    using Shape = DecodeShape<T, NG>;
+    using Shape = DecodeShape<T, NG, SPREAD>;
+    constexpr int NQ = Shape::NQ, NP = SPREAD ? 1 : Parts<T>::P, NH = 8 * NG;
+    constexpr bool Q_IN_REGS = Shape::Q_IN_REGS, WIDE = Parts<T>::Q > 1;
+    static_assert(!SPREAD || (WIDE && NG == 1 && Parts<T>::Q <= 4 && Parts<T>::P <= 4), "four parts of two heads are eight columns");
     extern __shared__ __align__(128) unsigned char smem[];
     uint2* sq = reinterpret_cast<uint2*>(smem);                       // the queries as operands: [kk][part][ng][lane]
     float* so = reinterpret_cast<float*>(smem + Shape::Q_BYTES);      // [warps][NH][HD], then the CTA's sum [NH][HD]
@@ -299,7 +311,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     float factor[NG][2], m_ref[NG][2], l_run[NG][2];
 #pragma unroll
     for (int ng = 0; ng < NG; ng++) {
-        const int h = ng * 8 + g8;
+        const int h = SPREAD ? g8 & 1 : ng * 8 + g8;
         float x[HD / 16][4];
         int m = 0;
 #pragma unroll
@@ -316,7 +328,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         const float f = finite ? a.scale * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);   // NaN: the row is
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            factor[ng][i] = __shfl_sync(0xffffffffu, f, (2 * t4 + i) * 4);
+            factor[ng][i] = __shfl_sync(0xffffffffu, f, (SPREAD ? i : 2 * t4 + i) * 4);
             m_ref[ng][i] = -INFINITY;
             l_run[ng][i] = 0.f;
         }
@@ -324,7 +336,15 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         for (int kk = 0; kk < HD / 16; kk++) {
             __half parts[4][NQ];
 #pragma unroll
-            for (int i = 0; i < 4; i++) split<NQ>(finite ? x[kk][i] * up : 0.f, parts[i]);
+            for (int i = 0; i < 4; i++) {
+                if constexpr (SPREAD) {
+                    __half all[Parts<T>::Q];
+                    split<Parts<T>::Q>(finite ? x[kk][i] * up : 0.f, all);
+                    parts[i][0] = pick(all, g8 >> 1);
+                } else {
+                    split<NQ>(finite ? x[kk][i] * up : 0.f, parts[i]);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < NQ; j++) {
                 const __half2 w0 = __halves2half2(parts[0][j], parts[1][j]), w1 = __halves2half2(parts[2][j], parts[3][j]);
@@ -373,8 +393,8 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                 }
                 // The tensor core cuts its sums; beside float32 queries 32 products at a time are added to a sum in registers
                 // (one sum over 256 dims was 2.7 times as far from 64 bits as float32 arithmetic).
-                float (&to)[DEC_MT][NG][4] = NQ > 1 ? part : s;
-                if (NQ > 1 && kk % 2 == 0) {
+                float (&to)[DEC_MT][NG][4] = WIDE ? part : s;
+                if (WIDE && kk % 2 == 0) {
 #pragma unroll
                     for (int i = 0; i < DEC_MT * NG * 4; i++) (&part[0][0][0])[i] = 0.f;
                 }
@@ -387,7 +407,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
 #pragma unroll
                         for (int mt = 0; mt < DEC_MT; mt++) mma16816(to[mt][ng], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
                     }
-                if (NQ > 1 && kk % 2 == 1) {
+                if (WIDE && kk % 2 == 1) {
 #pragma unroll
                     for (int i = 0; i < DEC_MT * NG * 4; i++) (&s[0][0][0])[i] += (&part[0][0][0])[i];
                 }
@@ -395,6 +415,14 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         }
         __syncwarp();                                                 // everybody has read this tile's keys
         request_k(stage, meta_slot == 0 ? DEC_STAGES : meta_slot - 1, page_now, slot_now);
+        if constexpr (SPREAD) {                       // the parts of a score: every lane of a row has both heads' then
+#pragma unroll
+            for (int i = 0; i < DEC_MT * 4; i++) {
+                float& x = (&s[0][0][0])[i];
+                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+            }
+        }
         // scores, in units of log2, with the values' exponents
         bool grown = false;
         float inv[DEC_MT][2];                       // 2^-ev of the lane's keys
@@ -453,8 +481,16 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                         l_run[ng][j] = fmaf(w[j], inv[mt][i], l_run[ng][j]);
                     }
                     __half h0[NP], h1[NP];
-                    split<NP>(w[0], h0);
-                    split<NP>(w[1], h1);
+                    if constexpr (SPREAD) {
+                        __half all[2][Parts<T>::P];
+                        split<Parts<T>::P>(w[0], all[0]);
+                        split<Parts<T>::P>(w[1], all[1]);
+                        h0[0] = pick(all[0], t4);
+                        h1[0] = pick(all[1], t4);
+                    } else {
+                        split<NP>(w[0], h0);
+                        split<NP>(w[1], h1);
+                    }
 #pragma unroll
                     for (int k = 0; k < NP; k++) {
                         const __half2 hh = __halves2half2(h0[k], h1[k]);
@@ -510,13 +546,17 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         for (int j = 0; j < 2; j++) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l_run[ng][j] += __shfl_xor_sync(0xffffffffu, l_run[ng][j], d);
-            const int h = ng * 8 + 2 * t4 + j;
-            if (g8 == 0) { s_ml[warp][h][0] = m_ref[ng][j]; s_ml[warp][h][1] = l_run[ng][j]; }
+            const int h = SPREAD ? j : ng * 8 + 2 * t4 + j;
+            if (g8 == 0 && (!SPREAD || t4 == 0)) { s_ml[warp][h][0] = m_ref[ng][j]; s_ml[warp][h][1] = l_run[ng][j]; }
 #pragma unroll
             for (int i = 0; i < HD / 16; i++) {
                 // dims of rows g and g + 8 of step i: neighbours g * HD / 8 + 2 i, + 1
                 float2 v = make_float2(o[i][ng][j], o[i][ng][2 + j]);
-                *reinterpret_cast<float2*>(so + ((warp * NH + h) * HD + g8 * (HD / 8) + 2 * i)) = v;
+                if constexpr (SPREAD) {
+                    v.x += __shfl_xor_sync(0xffffffffu, v.x, 1);
+                    v.y += __shfl_xor_sync(0xffffffffu, v.y, 1);
+                }
+                if (!SPREAD || t4 == 0) *reinterpret_cast<float2*>(so + ((warp * NH + h) * HD + g8 * (HD / 8) + 2 * i)) = v;
             }
         }
     __syncthreads();
@@ -578,11 +618,11 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     if (C > 1) cluster_leave();          // nobody leaves while another still reads its shared memory
 }
 
-template <typename T, int NG>
+template <typename T, int NG, bool SPREAD = false>
 int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t stream) {
-    constexpr size_t smem = DecodeShape<T, NG>::SMEM;
+    constexpr size_t smem = DecodeShape<T, NG, SPREAD>::SMEM;
     static_assert(smem <= 227 * 1024, "shared memory");
-    auto kernel = attn_decode_q8_kernel<T, NG>;
+    auto kernel = attn_decode_q8_kernel<T, NG, SPREAD>;
     static std::atomic<uint64_t> opened{0};                           // devices on which the kernel may have its shared memory
     cudaError_t e = smem > 48 * 1024 ? open_shared_memory((const void*)kernel, (int)smem, opened) : cudaSuccess;
     if (e == cudaSuccess) {
@@ -968,6 +1008,7 @@ extern "C" int kllm_attention_decode_q8(void* out, float* part_o, float* part_ml
         if (a.heads_per_cta > 8)
             return dtype == KLLM_F32 ? launch_decode<float, 2>(a, n_tokens, cluster, s) : launch_decode<bf16, 2>(a, n_tokens, cluster, s);
     }
+    if (dtype == KLLM_F32 && a.heads_per_cta <= 2) return launch_decode<float, 1, true>(a, n_tokens, cluster, s);
     return dtype == KLLM_F32 ? launch_decode<float, 1>(a, n_tokens, cluster, s) : launch_decode<bf16, 1>(a, n_tokens, cluster, s);
 }
 
