@@ -30,7 +30,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 16;                  // tokens a CTA looks after
 constexpr int kBatch = 4;                   // query heads whose numbers a thread requests together
-constexpr int kMaxHeads = 16;               // kv heads a CTA stores at most
+constexpr int kMaxHeads = 4;                // kv heads a CTA stores at most
+constexpr int kMaxRunBytes = 65536;         // what a CTA reads of a run, where several kv heads are more
 constexpr int kMaxMarks = 32768;            // rows of a run x kv heads: a byte each
 constexpr int kMaxPage = 4096;
 
@@ -313,8 +314,11 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     const bool four = rot % 8 == 0 && !((qo_stride | q_stride | k_stride | v_stride) & 3) &&
                       !(((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & (4 * es - 1)) &&
                       !((uintptr_t)cos_sin & 15) && !(((uintptr_t)kcache | (uintptr_t)vcache) & 3);
-    // A CTA a token where every request brings one, else one for sixteen.  kv heads a CTA: as many as its threads cover, as long
-    // as there are runs enough for two CTAs an SM.
+    // A CTA a token where every request brings one, else one for sixteen.  kv heads a CTA: as many as its threads cover, at most
+    // four, as long as there are runs enough for two CTAs an SM and the run stays in the first-level cache beside those of the SM's
+    // other CTAs until it is read again.  Microseconds for 3842 tokens in 9 portions with 1, 2, 4, 8 heads of 128 a CTA: float32, 32 kv
+    // heads, pages of 16 (16 KB a head) 88, 73, 70, 79, pages of 64 76, 77, 81, 119; bfloat16, 8 kv heads, pages of 16 34, 29, 27, 31; 4 x 2048
+    // tokens, pages of 64 69, 64, 68, 68.
     const int chunk = n_tokens <= n_requests ? 1 : kChunk;
     const int units = four ? hd / 4 : hd;      // of a head's key and value
     const int run = page_size < n_tokens ? page_size : n_tokens;
@@ -322,6 +326,8 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     int kv_heads = kThreads / units < kMaxHeads ? kThreads / units : kMaxHeads;
     if (kv_heads > runs * n_kv / 296) kv_heads = (int)(runs * n_kv / 296);
     if (kv_heads > kMaxMarks / run) kv_heads = kMaxMarks / run;
+    const int64_t head_bytes = (int64_t)(chunk == 1 ? 1 : run) * 2 * hd * es;
+    if (kv_heads > kMaxRunBytes / head_bytes) kv_heads = (int)(kMaxRunBytes / head_bytes);
     if (kv_heads < 1) kv_heads = 1;
     if (kv_heads > n_kv) kv_heads = n_kv;
     // threads for the longest run
