@@ -17,10 +17,10 @@
 // their order does not matter), once to store.  Rows that are not finite are rare: they are marked on the first way, and only
 // where there are any the maxima are taken again without them.
 //
-// Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.5 us, 2048 tokens 8.3 us (20 MB, 2.5 TB/s; copies at
-// 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 79 us (285 MB, 3.6 TB/s,
-// 56 % of a copy).  The last waits for its loads (10.7 of 16 cycles between two instructions of a warp) at the 32 warps an SM that 64 registers
-// leave.  A run's numbers kept in registers between the two ways, and more loads in flight at more registers, were both slower.
+// Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.5 us, 2048 tokens 8.6 us (20 MB, 2.4 TB/s; copies at
+// 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 70.5 us (285 MB, 4.0 TB/s,
+// 63 % of a copy), in bfloat16 55.6.  These wait for their loads (10 of 16 cycles between two instructions of a warp) at the 32 warps an SM that
+// 64 registers leave.  A run's numbers kept in registers between the two ways, and more loads in flight at more registers, were both slower.
 #include "q8.cuh"
 
 KLLM_EXPORT_LAST_ERROR(cache_q8)
@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 16;                  // tokens a CTA looks after
-constexpr int kBatch = 4;                   // query heads whose numbers a thread requests together
+template <int U> constexpr int kBatch = U == 8 ? 2 : 4;   // query heads whose numbers a thread requests together
 constexpr int kMaxHeads = 4;                // kv heads a CTA stores at most
 constexpr int kMaxRunBytes = 65536;         // what a CTA reads of a run, where several kv heads are more
 constexpr int kMaxMarks = 32768;            // rows of a run x kv heads: a byte each
@@ -38,6 +38,15 @@ constexpr int kMaxPage = 4096;
 template <typename T, int U> __device__ __forceinline__ void load(const T* p, float (&v)[U]) {
     if constexpr (U == 1) {
         v[0] = to_f32(*p);
+    } else if constexpr (U == 8 && sizeof(T) == 2) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(h[i] << 16); v[2 * i + 1] = __uint_as_float(h[i] & 0xffff0000u); }
+    } else if constexpr (U == 8) {
+        const float4 w = *reinterpret_cast<const float4*>(p), x = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+        v[4] = x.x; v[5] = x.y; v[6] = x.z; v[7] = x.w;
     } else if constexpr (sizeof(T) == 2) {
         const uint2 w = *reinterpret_cast<const uint2*>(p);
         v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u);
@@ -50,6 +59,15 @@ template <typename T, int U> __device__ __forceinline__ void load(const T* p, fl
 template <typename T, int U> __device__ __forceinline__ void store(T* p, const float (&v)[U]) {
     if constexpr (U == 1) {
         *p = from_f32<T>(v[0]);
+    } else if constexpr (U == 8) {
+        static_assert(sizeof(T) == 2, "16 bytes");
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            h[i] = *reinterpret_cast<const uint32_t*>(&a);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
     } else if constexpr (sizeof(T) == 2) {
         __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
         uint2 w;
@@ -60,11 +78,14 @@ template <typename T, int U> __device__ __forceinline__ void store(T* p, const f
     }
 }
 template <int U> __device__ __forceinline__ void store8(uint8_t* p, const float* v, float mul) {
+    auto four = [&](int i) { return q8_pack2(v[i] * mul, v[i + 1] * mul) | (q8_pack2(v[i + 2] * mul, v[i + 3] * mul) << 16); };
     if constexpr (U == 1) *p = (uint8_t)(q8_pack2(v[0] * mul, 0.f) & 0xff);
-    else *reinterpret_cast<uint32_t*>(p) = q8_pack2(v[0] * mul, v[1] * mul) | (q8_pack2(v[2] * mul, v[3] * mul) << 16);
+    else if constexpr (U == 8) *reinterpret_cast<uint2*>(p) = make_uint2(four(0), four(4));
+    else *reinterpret_cast<uint32_t*>(p) = four(0);
 }
 template <int U> __device__ __forceinline__ void fill8(uint8_t* p, uint32_t byte) {
     if constexpr (U == 1) *p = (uint8_t)byte;
+    else if constexpr (U == 8) *reinterpret_cast<uint2*>(p) = make_uint2(byte * 0x01010101u, byte * 0x01010101u);
     else *reinterpret_cast<uint32_t*>(p) = byte * 0x01010101u;
 }
 
@@ -100,7 +121,7 @@ template <typename T, int U> __device__ __forceinline__ void turn(const Raw<T, U
     }
 }
 
-// U = 4 where half the rotary width, strides and addresses allow it, else 1
+// U = 8 (bfloat16) or 4 where half the rotary width, strides and addresses allow it, else 1: what a thread reads at a time is 16 bytes
 template <typename T, int U>
 __global__ void __launch_bounds__(kThreads, 4)
 rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride, const T* __restrict__ k,
@@ -145,16 +166,16 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
             }
             const T* src = q + (int64_t)(t0 + t) * q_stride;
             T* dst = q_out + (int64_t)(t0 + t) * qo_stride;
-            for (int h = h0 + first; h < h1; h += kBatch * together) {
-                float x[kBatch][U], y[kBatch][U];
+            for (int h = h0 + first; h < h1; h += kBatch<U> * together) {
+                float x[kBatch<U>][U], y[kBatch<U>][U];
 #pragma unroll
-                for (int j = 0; j < kBatch; j++)
+                for (int j = 0; j < kBatch<U>; j++)
                     if (h + j * together < h1) {
                         load<T, U>(src + (int64_t)(h + j * together) * hd + unit.at, x[j]);
                         load<T, U>(src + (int64_t)(h + j * together) * hd + unit.at2, y[j]);
                     }
 #pragma unroll
-                for (int j = 0; j < kBatch; j++)
+                for (int j = 0; j < kBatch<U>; j++)
                     if (h + j * together < h1) {
                         float z[2 * U];
 #pragma unroll
@@ -213,7 +234,7 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
         if (tid == 0) s_any = 0;
         __syncthreads();
         int m = 0;
-#pragma unroll 4
+#pragma unroll (U == 8 ? 2 : 4)
         for (int r = first; mine && r < rows; r += together) {
             float x[2 * U];
             read(r, x);
@@ -255,18 +276,21 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
                         const uint32_t lo = q8_to_f16x2(*at[j]);
                         *at[j] = (uint8_t)(q8_pack2(__half22float2(*reinterpret_cast<const __half2*>(&lo)).x * down, 0.f) & 0xff);
                     } else {
-                        const uint32_t x = *reinterpret_cast<const uint32_t*>(at[j]);
-                        uint32_t lo, hi;
-                        q8_to_f16x4(x, lo, hi);
-                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                        *reinterpret_cast<uint32_t*>(at[j]) = q8_pack2(a.x * down, a.y * down) | (q8_pack2(b.x * down, b.y * down) << 16);
+#pragma unroll
+                        for (int l = 0; l < U; l += 4) {
+                            uint32_t* p4 = reinterpret_cast<uint32_t*>(at[j] + l);
+                            uint32_t lo, hi;
+                            q8_to_f16x4(*p4, lo, hi);
+                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                            *p4 = q8_pack2(a.x * down, a.y * down) | (q8_pack2(b.x * down, b.y * down) << 16);
+                        }
                     }
                 }
             }
         }
         // the new rows
         const float mul = q8_pow2(-e);
-#pragma unroll 4
+#pragma unroll (U == 8 ? 2 : 4)
         for (int r = first; mine && r < rows; r += together) {
             uint8_t* dst = page_rows + (int64_t)(slot + r) * hd;
             if (any && bad[r * heads + h]) {
@@ -311,16 +335,23 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     if (n_kv > 65535) KLLM_FAIL("append (8 bits): %d kv heads, at most 65535", n_kv);
     if (dtype != KLLM_F32 && dtype != KLLM_BF16) KLLM_FAIL("append (8 bits): element type %d", dtype);
     const int es = dtype == KLLM_F32 ? 4 : 2;
+    // Eight numbers at a time cost registers (spills) that calls of a few microseconds notice and larger ones do not: 8 tokens of 32 + 2 * 4 heads
+    // of 64 4.3 us against 3.8 with four, 2048 (5 M numbers) 8.9 against 8.7, 3000 of 24 + 2 * 8 of 96 (12 M) 16.9 against 17.4, 3842 of
+    // 32 + 2 * 32 of 128 (47 M) 55.6 against 65.4.
+    const bool many = (int64_t)n_tokens * (n_heads + 2 * n_kv) * hd >= 1 << 23;
+    const bool eight = many && dtype == KLLM_BF16 && rot % 16 == 0 && !((qo_stride | q_stride | k_stride | v_stride) & 7) &&
+                       !(((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cos_sin) & 15) &&
+                       !(((uintptr_t)kcache | (uintptr_t)vcache) & 7);
     const bool four = rot % 8 == 0 && !((qo_stride | q_stride | k_stride | v_stride) & 3) &&
                       !(((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & (4 * es - 1)) &&
                       !((uintptr_t)cos_sin & 15) && !(((uintptr_t)kcache | (uintptr_t)vcache) & 3);
     // A CTA a token where every request brings one, else one for sixteen.  kv heads a CTA: as many as its threads cover, at most
     // four, as long as there are runs enough for two CTAs an SM and the run stays in the first-level cache beside those of the SM's
     // other CTAs until it is read again.  Microseconds for 3842 tokens in 9 portions with 1, 2, 4, 8 heads of 128 a CTA: float32, 32 kv
-    // heads, pages of 16 (16 KB a head) 88, 73, 70, 79, pages of 64 76, 77, 81, 119; bfloat16, 8 kv heads, pages of 16 34, 29, 27, 31; 4 x 2048
-    // tokens, pages of 64 69, 64, 68, 68.
+    // heads, pages of 16 (16 KB a head) 88, 73, 70, 79, pages of 64 76, 77, 81, 119; bfloat16 (four numbers at a time), 8 kv heads, pages of 16
+    // 34, 29, 27, 31; 4 x 2048 tokens, pages of 64 69, 64, 68, 68.
     const int chunk = n_tokens <= n_requests ? 1 : kChunk;
-    const int units = four ? hd / 4 : hd;      // of a head's key and value
+    const int units = eight ? hd / 8 : four ? hd / 4 : hd;      // of a head's key and value
     const int run = page_size < n_tokens ? page_size : n_tokens;
     const int64_t runs = chunk == 1 ? n_tokens : (int64_t)n_tokens / page_size + n_requests;
     int kv_heads = kThreads / units < kMaxHeads ? kThreads / units : kMaxHeads;
@@ -335,7 +366,7 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     while (threads < kv_heads * units || (threads < kThreads && threads < (chunk == 1 ? 1 : run) * kv_heads * units)) threads *= 2;
     // query heads a CTA: a batch for every thread, as long as that leaves two CTAs an SM
     const int chunks = (n_tokens + chunk - 1) / chunk;
-    int q_heads = kBatch * (threads / (chunk * (units / 2)) > 0 ? threads / (chunk * (units / 2)) : 1);
+    int q_heads = (eight ? kBatch<8> : kBatch<4>) * (threads / (chunk * (units / 2)) > 0 ? threads / (chunk * (units / 2)) : 1);
     while (q_heads > 1 && (int64_t)chunks * ((n_heads + q_heads - 1) / q_heads) < 296) q_heads /= 2;
     const int kv_ctas = (n_kv + kv_heads - 1) / kv_heads, q_ctas = rot > 0 || q_out != q ? (n_heads + q_heads - 1) / q_heads : 0;
     if (kv_ctas + q_ctas > 65535) KLLM_FAIL("append (8 bits): %d heads over %d kv heads", n_heads, n_kv);
@@ -350,7 +381,7 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     if (dtype == KLLM_F32) {
         if (four) KLLM_GO(float, 4); else KLLM_GO(float, 1);
     } else {
-        if (four) KLLM_GO(bf16, 4); else KLLM_GO(bf16, 1);
+        if (eight) KLLM_GO(bf16, 8); else if (four) KLLM_GO(bf16, 4); else KLLM_GO(bf16, 1);
     }
 #undef KLLM_GO
     KLLM_LAUNCH_STATUS();

@@ -703,3 +703,25 @@ def test_starts_outside_the_rows(dtype):
     pos = ints(*[3] * 12)
     kernels.rope_append_q8(rows, rows, kv, kv, None, pos, ints(*[0] * 12), ints(5, -3), c.dev_table, c.k, c.v, c.ks, c.vs, H, G, hd)
     assert torch.equal(kept[0], c.k.view(torch.uint8)) and torch.equal(kept[1], c.v.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,G,hd,rot,page,starts,lens", [
+    (64, 32, 256, 256, 16, [0, 5, 31], [200, 52, 20]), (64, 64, 96, 48, 24, [7, 0], [300, 180]), (64, 64, 128, 0, 64, [70, 3, 0], [1, 240, 130]),
+    (64, 64, 96, 40, 24, [7, 0], [300, 180])])
+def test_append_many_numbers(dtype, H, G, hd, rot, page, starts, lens):
+    """Calls of 2^23 numbers and more, which bfloat16 takes eight at a time where the rotary width is a multiple of 16."""
+    n = sum(lens)
+    assert n * (H + 2 * G) * hd >= 2 ** 23
+    c = Cache(starts, lens, G, hd, page, seed=page + hd, fill=False)
+    q, k, v = queries(n, H, hd, dtype, 1), queries(n, G, hd, dtype, 2, loud=5.0), queries(n, G, hd, dtype, 3)
+    k[4, 7], k[9, hd + 3], v[12, 5], v[30, hd + 60], k[n - 1, 31] = math.inf, math.nan, -math.inf, math.nan, math.nan
+    cs = table_of_angles(400, rot) if rot else None
+    before = dict(key=(c.k.clone(), c.ks.clone()), value=(c.v.clone(), c.vs.clone()))
+    q_out, pos = run_append(c, q, k, v, cs, starts, lens, H, G, hd)
+    check_append(c, before, q_out, q, k, v, cs, pos, starts, lens, H, G, hd)
+    kept = [t.clone() for t in (c.k.view(torch.uint8), c.v.view(torch.uint8), c.ks, c.vs)]
+    q2, _ = run_append(c, q, k, v, cs, starts, lens, H, G, hd, in_place=True)
+    assert torch.equal(q2, q_out)
+    for a, b in zip(kept, (c.k.view(torch.uint8), c.v.view(torch.uint8), c.ks, c.vs)):
+        assert torch.equal(a.float().nan_to_num(-1.0), b.float().nan_to_num(-1.0))
