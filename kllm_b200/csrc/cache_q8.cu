@@ -6,8 +6,8 @@
 //     e = max(e_old, the smallest e' with max |x_r| <= 448 * 2^e'),   byte = e4m3(x_r * 2^-e),
 // and where e > e_old the earlier rows become e4m3(old * 2^(e_old - e)).  A row whose key or value is not finite counts
 // for no maximum; its key is stored as NaN and its value as 0.
-// The rotation is that of rope.cu: rotate_half, float32, angles from a table computed in float64.  A key is rounded once,
-// from the rotated float32 numbers to e4m3.
+// The rotation is that of rope.cu: rotate_half, float32, angles from a table computed in float64.  A key's byte is the e4m3
+// number next to its exact rotation by the table's angles.
 //
 // What bounds it: bytes, and for few tokens a chain of dependent loads.  A CTA takes a few tokens and one of two jobs: it
 // rotates some of their query heads, or it stores whole runs of rows of some kv heads: the first token of a request's rows in a
@@ -17,10 +17,11 @@
 // their order does not matter), once to store.  Rows that are not finite are rare: they are marked on the first way, and only
 // where there are any the maxima are taken again without them.
 //
-// Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.5 us, 2048 tokens 8.6 us (20 MB, 2.4 TB/s; copies at
-// 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 70.5 us (285 MB, 4.0 TB/s,
-// 63 % of a copy), in bfloat16 55.6.  These wait for their loads (10 of 16 cycles between two instructions of a warp) at the 32 warps an SM that
+// Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.5 us, 2048 tokens 9.8 us (20 MB, 2.1 TB/s; copies at
+// 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 76.6 us (285 MB, 3.7 TB/s,
+// 58 % of a copy), in bfloat16 63.7.  These wait for their loads (10 of 16 cycles between two instructions of a warp) at the 32 warps an SM that
 // 64 registers leave.  A run's numbers kept in registers between the two ways, and more loads in flight at more registers, were both slower.
+// Rounding the exact rotation costs 8 to 13 % of that: rounded from float32 arithmetic one number in a million was its neighbour.
 #include "q8.cuh"
 
 KLLM_EXPORT_LAST_ERROR(cache_q8)
@@ -77,11 +78,21 @@ template <typename T, int U> __device__ __forceinline__ void store(T* p, const f
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     }
 }
-template <int U> __device__ __forceinline__ void store8(uint8_t* p, const float* v, float mul) {
-    auto four = [&](int i) { return q8_pack2(v[i] * mul, v[i + 1] * mul) | (q8_pack2(v[i + 2] * mul, v[i + 3] * mul) << 16); };
-    if constexpr (U == 1) *p = (uint8_t)(q8_pack2(v[0] * mul, 0.f) & 0xff);
-    else if constexpr (U == 8) *reinterpret_cast<uint2*>(p) = make_uint2(four(0), four(4));
-    else *reinterpret_cast<uint32_t*>(p) = four(0);
+// U numbers times mul as e4m3, four a word
+template <int U> constexpr int kWords = (U + 3) / 4;
+template <int U> __device__ __forceinline__ void pack8(const float* v, float mul, uint32_t (&w)[kWords<U>]) {
+    if constexpr (U == 1) {
+        w[0] = q8_pack2(v[0] * mul, 0.f) & 0xff;
+    } else {
+#pragma unroll
+        for (int i = 0; i < U / 4; i++)
+            w[i] = q8_pack2(v[4 * i] * mul, v[4 * i + 1] * mul) | (q8_pack2(v[4 * i + 2] * mul, v[4 * i + 3] * mul) << 16);
+    }
+}
+template <int U> __device__ __forceinline__ void store8(uint8_t* p, const uint32_t (&w)[kWords<U>]) {
+    if constexpr (U == 1) *p = (uint8_t)w[0];
+    else if constexpr (U == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 template <int U> __device__ __forceinline__ void fill8(uint8_t* p, uint32_t byte) {
     if constexpr (U == 1) *p = (uint8_t)byte;
@@ -118,6 +129,57 @@ template <typename T, int U> __device__ __forceinline__ void turn(const Raw<T, U
     for (int i = 0; i < U; i++) {
         v[i] = turned ? w.x[i] * w.c[i] - w.y[i] * w.s[i] : w.x[i];
         v[U + i] = turned ? w.y[i] * w.c[i] + w.x[i] * w.s[i] : w.y[i];
+    }
+}
+
+// a c - b s with its last bit set where it is not exact and cut towards zero ("to odd"): a further rounding to fewer bits gives what
+// rounding the exact number once gives.  The products' and the sum's errors are exact float32 numbers (fma; two-sum), their sum is off by
+// 2^-46 of the products.
+__device__ __noinline__ float turned_to_odd(float a, float c, float b, float s) {
+    const float p = a * c, n = -b * s;
+    const float ep = fmaf(a, c, -p), en = fmaf(-b, s, -n);
+    const float r = __fadd_rn(p, n), t = __fsub_rn(r, p);
+    const float e = __fadd_rn(__fadd_rn(__fsub_rn(p, __fsub_rn(r, t)), __fsub_rn(n, t)), __fadd_rn(ep, en));
+    const float sum = __fadd_rn(r, e), u = __fsub_rn(sum, r);
+    const float rest = __fadd_rn(__fsub_rn(r, __fsub_rn(sum, u)), __fsub_rn(e, u));
+    if (!(fabsf(sum) < INFINITY)) return r;
+    int bits = __float_as_int(sum);
+    if (rest != 0.f) {
+        if (bits << 1 && (rest < 0.f) != (sum < 0.f)) bits--;
+        bits |= 1;
+    }
+    return __int_as_float(bits);
+}
+// The unit as e4m3.  Turned numbers are within 1.5 last places here (the error of the product that is rounded first is taken off the
+// sum): where a number times 1 - 2^-21 and times 1 + 2^-21 round alike, so does the exact one.  A unit with one that does not
+// (once in 10^4 units) is taken again.
+template <typename T, int U>
+__device__ __forceinline__ void pack_unit(const Raw<T, U>& w, bool turned, float mul, uint32_t (&a)[kWords<U>], uint32_t (&b)[kWords<U>]) {
+    float v[2 * U];
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        v[i] = w.x[i]; v[U + i] = w.y[i];
+        if (turned) {
+            const float p = __fmul_rn(w.y[i], w.s[i]), q = __fmul_rn(w.x[i], w.s[i]);
+            v[i] = __fsub_rn(fmaf(w.x[i], w.c[i], -p), fmaf(w.y[i], w.s[i], -p));
+            v[U + i] = __fadd_rn(fmaf(w.y[i], w.c[i], q), fmaf(w.x[i], w.s[i], -q));
+        }
+    }
+    const float wide = turned ? mul * 0x1p-21f : 0.f;
+    uint32_t a2[kWords<U>], b2[kWords<U>];
+    pack8<U>(v, mul - wide, a); pack8<U>(v, mul + wide, a2);
+    pack8<U>(v + U, mul - wide, b); pack8<U>(v + U, mul + wide, b2);
+    uint32_t differ = 0;
+#pragma unroll
+    for (int i = 0; i < kWords<U>; i++) differ |= (a[i] ^ a2[i]) | (b[i] ^ b2[i]);
+    if (differ) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            v[i] = turned_to_odd(w.x[i], w.c[i], w.y[i], w.s[i]);
+            v[U + i] = turned_to_odd(w.y[i], w.c[i], -w.x[i], w.s[i]);
+        }
+        pack8<U>(v, mul, a);
+        pack8<U>(v + U, mul, b);
     }
 }
 
@@ -223,10 +285,8 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
         const int ke_old = slot ? q8_exponent(kscale[cell]) : Q8_E_MIN, ve_old = slot ? q8_exponent(vscale[cell]) : Q8_E_MIN;
         const T* row0 = src + (int64_t)t * src_stride;
         const float* cs0 = cos_sin + (int64_t)p * rot;
-        auto read = [&](int r, float (&x)[2 * U]) {
-            Raw<T, U> w;
+        auto read = [&](int r, Raw<T, U>& w) {
             read_unit<T, U>(w, row0 + (int64_t)r * src_stride, unit, turned, cs0 + (int64_t)r * rot, half);
-            turn<T, U>(w, turned, x);
         };
         __syncthreads();                                            // the run before is done with the marks and the maxima
         for (int j = tid; j < rows * heads; j += threads) bad[j] = 0;
@@ -236,8 +296,10 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
         int m = 0;
 #pragma unroll (U == 8 ? 2 : 4)
         for (int r = first; mine && r < rows; r += together) {
+            Raw<T, U> w;
             float x[2 * U];
-            read(r, x);
+            read(r, w);
+            turn<T, U>(w, turned, x);
             int mr = 0;
 #pragma unroll
             for (int j = 0; j < 2 * U; j++) mr = max(mr, __float_as_int(x[j]) & 0x7fffffff);
@@ -254,8 +316,10 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
             m = 0;
             for (int r = first; mine && r < rows; r += together) {
                 if (bad[r * heads + h]) continue;
+                Raw<T, U> w;
                 float x[2 * U];
-                read(r, x);
+                read(r, w);
+                turn<T, U>(w, turned, x);
 #pragma unroll
                 for (int j = 0; j < 2 * U; j++) m = max(m, __float_as_int(x[j]) & 0x7fffffff);
             }
@@ -298,10 +362,12 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
                 fill8<U>(dst + unit.at2, key ? 0x7f : 0);
                 continue;
             }
-            float x[2 * U];
-            read(r, x);
-            store8<U>(dst + unit.at, x, mul);
-            store8<U>(dst + unit.at2, x + U, mul);
+            Raw<T, U> w;
+            read(r, w);
+            uint32_t lower[kWords<U>], upper[kWords<U>];
+            pack_unit<T, U>(w, turned, mul, lower, upper);
+            store8<U>(dst + unit.at, lower);
+            store8<U>(dst + unit.at2, upper);
         }
         if (first == 0 && i == 0) {
             kscale[cell] = q8_pow2(ke);
@@ -336,9 +402,9 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
     if (dtype != KLLM_F32 && dtype != KLLM_BF16) KLLM_FAIL("append (8 bits): element type %d", dtype);
     const int es = dtype == KLLM_F32 ? 4 : 2;
     // Eight numbers at a time cost registers (spills) that calls of a few microseconds notice and larger ones do not: 8 tokens of 32 + 2 * 4 heads
-    // of 64 4.3 us against 3.8 with four, 2048 (5 M numbers) 8.9 against 8.7, 3000 of 24 + 2 * 8 of 96 (12 M) 16.9 against 17.4, 3842 of
-    // 32 + 2 * 32 of 128 (47 M) 55.6 against 65.4.
-    const bool many = (int64_t)n_tokens * (n_heads + 2 * n_kv) * hd >= 1 << 23;
+    // of 64 4.3 us against 3.8 with four, 3000 of 24 + 2 * 8 of 96 (12 M numbers) 19.8 against 18.7, 3842 of 32 + 2 * 8 of 128 (24 M) 28.5 against
+    // 29.0, of 32 + 2 * 32 (47 M) 63.7 against 71.7.
+    const bool many = (int64_t)n_tokens * (n_heads + 2 * n_kv) * hd >= 1 << 24;
     const bool eight = many && dtype == KLLM_BF16 && rot % 16 == 0 && !((qo_stride | q_stride | k_stride | v_stride) & 7) &&
                        !(((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cos_sin) & 15) &&
                        !(((uintptr_t)kcache | (uintptr_t)vcache) & 7);

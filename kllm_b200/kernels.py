@@ -1104,7 +1104,8 @@ def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     """Rotary encoding of a step's tokens and the write of their keys and values into a cache in 8 bits
     (csrc/cache_q8.cu): ``q_out`` [n, H*hd] gets the rotated queries (it may be ``q``), the pages of ``kcache`` / ``vcache``
     (float8_e4m3fn [pages, G, page_size, hd]) the rotated keys and the values, ``kscale`` / ``vscale`` (float32 [pages, G])
-    the pages' scales.  A stored number stands for e4m3 * scale.
+    the pages' scales.  A stored number stands for e4m3 * scale; it is the e4m3 number next to the value, or to the exact rotation
+    of the key by the table's angles.
 
     A page's scale is a power of two 2^e, -48 <= e <= 48: the smallest with max|x| <= 448 * 2^e over the rows that are
     stored, and not below that of the rows which the page holds already; these are stored again under a scale that has

@@ -707,16 +707,16 @@ def test_starts_outside_the_rows(dtype):
 
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("H,G,hd,rot,page,starts,lens", [
-    (64, 32, 256, 256, 16, [0, 5, 31], [200, 52, 20]), (64, 64, 96, 48, 24, [7, 0], [300, 180]), (64, 64, 128, 0, 64, [70, 3, 0], [1, 240, 130]),
-    (64, 64, 96, 40, 24, [7, 0], [300, 180])])
+    (64, 32, 256, 256, 16, [0, 5, 31], [400, 92, 40]), (64, 64, 96, 48, 24, [7, 0], [600, 330]), (64, 64, 128, 0, 64, [70, 3, 0], [1, 440, 260]),
+    (64, 64, 96, 40, 24, [7, 0], [600, 330])])
 def test_append_many_numbers(dtype, H, G, hd, rot, page, starts, lens):
-    """Calls of 2^23 numbers and more, which bfloat16 takes eight at a time where the rotary width is a multiple of 16."""
+    """Calls of 2^24 numbers and more, which bfloat16 takes eight at a time where the rotary width is a multiple of 16."""
     n = sum(lens)
-    assert n * (H + 2 * G) * hd >= 2 ** 23
+    assert n * (H + 2 * G) * hd >= 2 ** 24
     c = Cache(starts, lens, G, hd, page, seed=page + hd, fill=False)
     q, k, v = queries(n, H, hd, dtype, 1), queries(n, G, hd, dtype, 2, loud=5.0), queries(n, G, hd, dtype, 3)
     k[4, 7], k[9, hd + 3], v[12, 5], v[30, hd + 60], k[n - 1, 31] = math.inf, math.nan, -math.inf, math.nan, math.nan
-    cs = table_of_angles(400, rot) if rot else None
+    cs = table_of_angles(700, rot) if rot else None
     before = dict(key=(c.k.clone(), c.ks.clone()), value=(c.v.clone(), c.vs.clone()))
     q_out, pos = run_append(c, q, k, v, cs, starts, lens, H, G, hd)
     check_append(c, before, q_out, q, k, v, cs, pos, starts, lens, H, G, hd)
@@ -725,3 +725,23 @@ def test_append_many_numbers(dtype, H, G, hd, rot, page, starts, lens):
     assert torch.equal(q2, q_out)
     for a, b in zip(kept, (c.k.view(torch.uint8), c.v.view(torch.uint8), c.ks, c.vs)):
         assert torch.equal(a.float().nan_to_num(-1.0), b.float().nan_to_num(-1.0))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,G,hd,rot,page,starts,lens", [(64, 64, 128, 128, 16, [3, 0], [400, 300]), (32, 32, 128, 128, 64, [9], [900]),
+                                                         (32, 32, 96, 6, 16, [0], [500])])
+@pytest.mark.parametrize("loud", [2.0, 2.0 ** -13])
+def test_append_rounds_the_exact_rotation(dtype, H, G, hd, rot, page, starts, lens, loud):
+    """Millions of keys without one that went to the wrong side of a border of e4m3, among its subnormals too (rows that one large
+    number keeps small)."""
+    c = Cache(starts, lens, G, hd, page, seed=5, fill=False)
+    n = sum(lens)
+    q, k, v = queries(n, H, hd, dtype, 1), queries(n, G, hd, dtype, 2, loud=loud), queries(n, G, hd, dtype, 3)
+    if loud < 1:
+        k[:, ::hd] = 1.5
+    cs = table_of_angles(1600, rot)
+    before = dict(key=(c.k.clone(), c.ks.clone()))
+    q_out, pos = run_append(c, q, k, v, cs, starts, lens, H, G, hd)
+    kr, vr = plain.turned(k, cs, pos, G, hd), v.cpu().double().view(n, G, hd)
+    want, scale, _ = plain.append(*before["key"], kr, vr, True, c.table, starts, lens)
+    assert torch.equal(c.ks.cpu().double(), scale) and torch.equal(c.k.cpu().float().double(), want)
