@@ -19,8 +19,8 @@
 //
 // Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.5 us, 2048 tokens 9.8 us (20 MB, 2.1 TB/s; copies at
 // 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 76.6 us (285 MB, 3.7 TB/s,
-// 58 % of a copy), in bfloat16 63.7.  These wait for their loads (10 of 16 cycles between two instructions of a warp) at the 32 warps an SM that
-// 64 registers leave.  A run's numbers kept in registers between the two ways, and more loads in flight at more registers, were both slower.
+// 58 % of a copy), in bfloat16 63.7.  These wait for their loads (6 of 12 cycles between two instructions of a warp, issue slots 55 % busy) at the 32
+// warps an SM that 64 registers leave.  A run's numbers kept in registers between the two ways, and more loads in flight at more registers, were both slower.
 // Rounding the exact rotation costs 8 to 13 % of that: rounded from float32 arithmetic one number in a million was its neighbour.
 #include "q8.cuh"
 
