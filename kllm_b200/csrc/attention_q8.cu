@@ -1027,3 +1027,5 @@ extern "C" int kllm_attention_prefill_q8(void* out, const void* q, int64_t q_str
                   max_blocks, n_pages, n_tokens, n_requests, n_heads, n_kv, page_size, window > 0 ? window : 0, PRE_ROWS / gs, scale};
     return dtype == KLLM_F32 ? launch_prefill<float>(a, (cudaStream_t)stream) : launch_prefill<bf16>(a, (cudaStream_t)stream);
 }
+extern "C" int kllm_attention_decode_q8_packed(const void* args) { return call_packed(&kllm_attention_decode_q8, args); }
+extern "C" int kllm_attention_prefill_q8_packed(const void* args) { return call_packed(&kllm_attention_prefill_q8, args); }

@@ -823,3 +823,4 @@ extern "C" int kllm_attention_prefill_q8_tcgen05(void* out, float* part_o, float
     }
     KLLM_LAUNCH_STATUS();
 }
+extern "C" int kllm_attention_prefill_q8_tcgen05_packed(const void* args) { return call_packed(&kllm_attention_prefill_q8_tcgen05, args); }

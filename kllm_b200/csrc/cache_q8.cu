@@ -452,3 +452,4 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
 #undef KLLM_GO
     KLLM_LAUNCH_STATUS();
 }
+extern "C" int kllm_rope_append_q8_packed(const void* args) { return call_packed(&kllm_rope_append_q8, args); }

@@ -18,6 +18,8 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
+#include <utility>
 
 namespace {
 
@@ -216,6 +218,20 @@ void launch_join(void* out, const float* part_o, const float* part_ml, int range
                  int n_requests, cudaStream_t stream) {
     kllm_launch((q8_join_kernel<T, HD>), dim3((unsigned)((n_rows + q8_join_rows<HD> - 1) / q8_join_rows<HD>)), dim3(q8_join_rows<HD> * (HD / 4)), 0,
                 stream, (T*)out, part_o, part_ml, ranges, n_heads, n_rows, q_start, n_requests);
+}
+
+// Calls an entry point with its arguments from a block of 8-byte numbers, one each: addresses and integers as int64, floating-point
+// numbers as double.  A caller in Python packs such a block in a fraction of the time that as many typed arguments take.
+template <typename T> T packed_argument(const int64_t* p) {
+    if constexpr (std::is_pointer_v<T>) return reinterpret_cast<T>((uintptr_t)*p);
+    else if constexpr (std::is_floating_point_v<T>) { double x; memcpy(&x, p, 8); return (T)x; }
+    else return (T)*p;
+}
+template <typename... A, size_t... I> int call_packed(int (*entry)(A...), const int64_t* args, std::index_sequence<I...>) {
+    return entry(packed_argument<A>(args + I)...);
+}
+template <typename... A> [[maybe_unused]] int call_packed(int (*entry)(A...), const void* args) {
+    return call_packed(entry, (const int64_t*)args, std::index_sequence_for<A...>());
 }
 
 // Once per device: more than 48 KB of dynamic shared memory for a kernel.

@@ -1051,7 +1051,7 @@ def _q8_function(library: str, name: str, head_dim: int = 0):
     fn = _q8_functions.get((name, head_dim))
     if fn is None:
         lib = load_library(library, {"KLLM_HD": head_dim} if head_dim else None)
-        fn = _q8_functions[name, head_dim] = (getattr(lib, name), lib)
+        fn = _q8_functions[name, head_dim] = (lib.packed(name), lib)
     return fn
 
 
@@ -1148,8 +1148,8 @@ def rope_append_q8(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
             raise KernelError("rope_append_q8: cos_sin must be contiguous float32 [positions, even rotary width <= head_dim]")
     _q8_device("rope_append_q8", q_out, q, k, v, cos_sin, positions, token_req, q_start, block_table, kcache, vcache, kscale, vscale)
     fn, lib = _q8_function("cache_q8", "kllm_rope_append_q8")
-    rc = fn(q_out.data_ptr(), so, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _p(cos_sin), n_pos, positions.data_ptr(),
-            _p(token_req), q_start.data_ptr(), R, block_table.data_ptr(), blocks, kcache.data_ptr(), vcache.data_ptr(),
+    rc = fn(q_out.data_ptr(), so, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _p(cos_sin) or 0, n_pos, positions.data_ptr(),
+            _p(token_req) or 0, q_start.data_ptr(), R, block_table.data_ptr(), blocks, kcache.data_ptr(), vcache.data_ptr(),
             kscale.data_ptr(), vscale.data_ptr(), pages, n, n_heads, n_kv, head_dim, rot, page_size, code, _stream())
     _check(lib, "cache_q8", rc)
 
@@ -1222,7 +1222,7 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
     window = _q8_window(window)
     bound = min(ctx_bound, window) if window else ctx_bound
     ranges, cluster = decode_q8_parts(n, n_kv, n_heads // n_kv, head_dim, bound, code == 0)
-    part_o = part_ml = None
+    part_o = part_ml = 0
     if ranges > 1:
         parts = torch.empty((n * n_heads * ranges, head_dim + 2), dtype=torch.float32, device=q.device)
         part_o = parts.data_ptr()
@@ -1230,7 +1230,7 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
     pages, _, page_size, _ = kcache.shape
     fn, lib = _q8_function("attention_q8", "kllm_attention_decode_q8", head_dim)
     rc = fn(out.data_ptr(), part_o, part_ml, q.data_ptr(), stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
-            vscale.data_ptr(), positions.data_ptr(), _p(token_req), block_table.data_ptr(), blocks, pages, n, R, n_heads, n_kv,
+            vscale.data_ptr(), positions.data_ptr(), _p(token_req) or 0, block_table.data_ptr(), blocks, pages, n, R, n_heads, n_kv,
             head_dim, page_size, window, scale, ranges, cluster, code, _stream())
     _check(lib, "attention_q8", rc)
     global launches
@@ -1287,7 +1287,7 @@ def attention_prefill_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tenso
     if code == 1 and head_dim in TCGEN05_HEAD_DIMS and USE_TCGEN05 and group <= 128 and out.data_ptr() % 16 == 0:
         bound = min(ctx_bound, window + 256 // group) if window else ctx_bound
         row_tiles, splits = prefill_q8_parts(n, R, n_kv, group, bound, head_dim)
-        part_o = part_ml = None
+        part_o = part_ml = 0
         if splits > 1:
             parts = torch.empty((n * n_heads * splits, head_dim + 2), dtype=torch.float32, device=q.device)
             part_o = parts.data_ptr()

@@ -222,3 +222,32 @@ def test_angles_that_are_no_matrix():
 @pytest.mark.parametrize("window,kept", [(None, 0), (0, 0), (-3, 0), (7, 7), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (2 ** 40 + 5, 2 ** 31 - 1)])
 def test_windows_fit_the_kernels_integers(window, kept):
     assert kernels._q8_window(window) == kept
+
+
+@pytest.mark.parametrize("library,defines,name", [
+    ("cache_q8", None, "kllm_rope_append_q8"), ("attention_q8", {"KLLM_HD": 64}, "kllm_attention_decode_q8"),
+    ("attention_q8", {"KLLM_HD": 64}, "kllm_attention_prefill_q8"), ("attention_q8_tcgen05", {"KLLM_HD": 64}, "kllm_attention_prefill_q8_tcgen05")])
+def test_packed_calls_are_the_typed_ones(library, defines, name):
+    """A head size of 35 or less is refused before a device is asked for, whatever the other arguments are: both forms say the same."""
+    import ctypes
+    import struct
+    lib = kernels.load_library(library, defines)
+    typed, packed, types = getattr(lib, name), lib.packed(name), lib._params[name]
+    error = getattr(lib, "kllm_last_error_" + library)
+    error.restype = ctypes.c_char_p
+    floats = [t in (ctypes.c_float, ctypes.c_double) for t in types]
+    base = [0.5 if f else 35 for f in floats]
+    said = set()
+    for at in range(len(types)):
+        for value in (1, 3, 34, -2):
+            args = list(base)
+            args[at] = float(value) if floats[at] else value
+            a, b = typed(*args), error()
+            c, d = packed(*args), error()
+            assert a == c and b == d, (at, value)
+            said.add((a, b))
+    assert len(said) >= 6
+    with pytest.raises(struct.error):
+        packed(*base[:-1])
+    with pytest.raises(struct.error):
+        packed(*base, 0)
