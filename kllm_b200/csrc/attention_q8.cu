@@ -170,11 +170,9 @@ __device__ __forceinline__ unsigned cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
 }
-// ... for the end of a kernel: orders no memory, where the release above waits for the rows just stored (2400 cycles of a call of 10700).  What
-// was read from the others has arrived: it was stored.
-__device__ __forceinline__ void cluster_leave() {
-    asm volatile("barrier.cluster.arrive.relaxed;\nbarrier.cluster.wait;\n" ::: "memory");
-}
+// ... in two: what this thread did before the arrival is done when the others are past their wait
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;\n" ::: "memory"); }
 __device__ __forceinline__ unsigned peer_addr(const void* p, unsigned rank) {
     unsigned b;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(b) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
@@ -579,34 +577,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     const unsigned C = cluster_size(), rank = cluster_rank();
     if (C > 1) cluster_sync(); else __syncthreads();
     const int range = blockIdx.x / C;
-    for (int u = rank * DEC_WARPS * 32 + tid; u < nh * (HD / 4); u += C * DEC_WARPS * 32) {
-        const int h = u / (HD / 4), d = (u - h * (HD / 4)) * 4;
-        float m = -INFINITY, l = 0.f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (C == 1) {
-            m = s_cta[h][0]; l = s_cta[h][1];
-            x = *reinterpret_cast<const float4*>(so + h * HD + d);
-        } else {
-            float2 ml[8];
-            float4 px[8];
-#pragma unroll
-            for (unsigned c = 0; c < 8; c++) {
-                ml[c] = make_float2(-INFINITY, 0.f);
-                px[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (c < C) {
-                    ml[c] = peer_load2(&s_cta[h][0], c);
-                    px[c] = peer_load4(so + h * HD + d, c);
-                }
-            }
-#pragma unroll
-            for (unsigned c = 0; c < 8; c++) m = fmaxf(m, ml[c].x);
-#pragma unroll
-            for (unsigned c = 0; c < 8; c++) {
-                const float f = part_factor(ml[c].x, ml[c].y, m);
-                l += f * ml[c].y;
-                add_scaled(x, f, px[c]);
-            }
-        }
+    auto put = [&](int h, int d, const float4& x, float m, float l) {
         const int64_t at = (int64_t)token * a.n_heads + head0 + h;
         if (a.ranges == 1) {
             store_row4(reinterpret_cast<T*>(a.out) + at * HD + d, x, l);
@@ -614,8 +585,53 @@ attn_decode_q8_kernel(const DecodeArgs a) {
             *reinterpret_cast<float4*>(a.part_o + (at * a.ranges + range) * HD + d) = x;
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.ranges + range) * 2) = make_float2(m, l);
         }
+    };
+    if (C == 1) {
+        for (int u = tid; u < nh * (HD / 4); u += DEC_WARPS * 32) {
+            const int h = u / (HD / 4), d = (u - h * (HD / 4)) * 4;
+            put(h, d, *reinterpret_cast<const float4*>(so + h * HD + d), s_cta[h][0], s_cta[h][1]);
+        }
+        return;
     }
-    if (C > 1) cluster_leave();          // nobody leaves while another still reads its shared memory
+    // All that is read of the others is read before the arrival, and stored behind it: a CTA leaves when the others have what they read of
+    // it, without waiting for its rows to be stored (one arrival behind the stores: 2400 cycles of a call of 10700).
+    constexpr int SHARE = (NH * (HD / 4) + 2 * DEC_WARPS * 32 - 1) / (2 * DEC_WARPS * 32);       // of a thread, in clusters of two
+    float4 x[SHARE];
+    float m[SHARE], l[SHARE];
+#pragma unroll
+    for (int i = 0; i < SHARE; i++) {
+        const int u = (i * (int)C + (int)rank) * DEC_WARPS * 32 + tid, h = u / (HD / 4), d = (u - h * (HD / 4)) * 4;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+        if (u >= nh * (HD / 4)) continue;
+        float2 ml[8];
+        float4 px[8];
+#pragma unroll
+        for (unsigned c = 0; c < 8; c++) {
+            ml[c] = make_float2(-INFINITY, 0.f);
+            px[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c < C) {
+                ml[c] = peer_load2(&s_cta[h][0], c);
+                px[c] = peer_load4(so + h * HD + d, c);
+            }
+        }
+#pragma unroll
+        for (unsigned c = 0; c < 8; c++) m[i] = fmaxf(m[i], ml[c].x);
+#pragma unroll
+        for (unsigned c = 0; c < 8; c++) {
+            const float f = part_factor(ml[c].x, ml[c].y, m[i]);
+            l[i] += f * ml[c].y;
+            add_scaled(x[i], f, px[c]);
+        }
+    }
+    cluster_arrive();
+#pragma unroll
+    for (int i = 0; i < SHARE; i++) {
+        const int u = (i * (int)C + (int)rank) * DEC_WARPS * 32 + tid, h = u / (HD / 4), d = (u - h * (HD / 4)) * 4;
+        if (u < nh * (HD / 4)) put(h, d, x[i], m[i], l[i]);
+    }
+    cluster_wait();
 }
 
 template <typename T, int NG, bool SPREAD = false>
