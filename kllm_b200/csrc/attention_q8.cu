@@ -37,6 +37,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// ... of a sum that begins
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
@@ -74,7 +80,7 @@ template <int N> __device__ __forceinline__ __half pick(const __half (&p)[N], in
 //
 // Measured, back to back, bfloat16 (% of a copy's 6.45 TB/s): 64 requests of 846 to 4095 keys, 32 heads over 8 of 128, pages of 16: 67.6 us (74 %);
 // one of 131072 keys 53.8 us (77 %); 8 of 2048 keys, 32 over 4 of 64: 8.2 us; one: 5.9 us, a chain of launch, table, tiles and
-// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 16.8 us (40 %; with the parts as products of their own 18.9).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
+// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 17.5 us (38 %).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
 // 64 (16 of a CTA pair an SM as before): 64 x 2048 keys 18.7 us against 19.6, 128 x 1000 23.0 against 18.8.
 
 constexpr int DEC_KT = HD <= 128 ? 32 : 16;              // keys of a warp's tile
@@ -96,9 +102,11 @@ __device__ __forceinline__ int dec_key(int row) { return row ^ ((row >> 1) & 1);
 
 // SPREAD: where a CTA has one or two heads of float32 queries, the parts of a head's queries, and of its weights, are columns
 // of the N side (part p of head h is column 2 p + h) instead of products of their own: a third of the first product's
-// instructions and half of the second's (32 heads of 128, 8 x 2048 keys: 35.0 us against 40.7).
-template <typename T, int NG, bool SPREAD> struct DecodeShape {
-    static constexpr int NQ = SPREAD ? 1 : Parts<T>::Q;
+// instructions and half of the second's (32 heads of 128, 8 x 2048 keys: 35.6 us against more than 40).  Three or four heads: the
+// weights' parts alone (part p of head h is column 4 p + h; both columns have the head's queries): 64 x 2048 keys of 32 heads over 8
+// of 128 59.7 us, with two products a part's sum 85, of which most is four registers too many.
+template <typename T, int NG, int SPREAD> struct DecodeShape {
+    static constexpr int NQ = SPREAD == 2 ? 1 : Parts<T>::Q;
     static constexpr int QREGS = HD / 16 * 2 * NQ * NG;
     static constexpr bool Q_IN_REGS = QREGS <= 32;
     static constexpr int Q_BYTES = Q_IN_REGS ? 0 : HD / 16 * NQ * NG * 32 * 8;
@@ -190,13 +198,14 @@ __device__ __forceinline__ float4 peer_load4(const void* p, unsigned rank) {
 }
 // grid: (ranges * cluster, kv heads * subgroups of heads, tokens), clusters along x; a cluster's CTAs take neighbouring
 // parts of a range and join through distributed shared memory
-template <typename T, int NG, bool SPREAD>
+template <typename T, int NG, int SPREAD>         // heads in their parts' columns: 2, 4, or 0: every part a product
 __global__ void __launch_bounds__(DEC_WARPS * 32, (DecodeShape<T, NG, SPREAD>::CTAS))
 attn_decode_q8_kernel(const DecodeArgs a) {
     using Shape = DecodeShape<T, NG, SPREAD>;
     constexpr int NQ = Shape::NQ, NP = SPREAD ? 1 : Parts<T>::P, NH = 8 * NG;
     constexpr bool Q_IN_REGS = Shape::Q_IN_REGS, WIDE = Parts<T>::Q > 1;
-    static_assert(!SPREAD || (WIDE && NG == 1 && Parts<T>::Q <= 4 && Parts<T>::P <= 4), "four parts of two heads are eight columns");
+    static_assert(SPREAD == 0 || (WIDE && NG == 1 && (SPREAD == 2 ? Parts<T>::Q <= 4 && Parts<T>::P <= 4 : SPREAD == 4 && Parts<T>::P <= 2)),
+                  "the parts of two or four heads are eight columns");
     extern __shared__ __align__(128) unsigned char smem[];
     uint2* sq = reinterpret_cast<uint2*>(smem);                       // the queries as operands: [kk][part][ng][lane]
     float* so = reinterpret_cast<float*>(smem + Shape::Q_BYTES);      // [warps][NH][HD], then the CTA's sum [NH][HD]
@@ -234,58 +243,51 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     // copies differ by constants, where a look-up per row costs a shuffle, a comparison and a 64-bit product each.
     constexpr int COPIES = DEC_KT * PIECES / 32;
     const bool blocks = a.page_size % 16 == 0;
-    int rows[COPIES];                     // of the tile that is being requested; -1: not seen.  In blocks: the first two, a row each
+    // Rows of the tile that is being requested, -1: not seen: of the lane's key, and of the keys whose pieces the lane copies (in blocks: the
+    // first two are a row each).  The latter are handed over once where there are registers, else again for the values: a spilled register
+    // is fetched from L2, as the rings leave no first-level cache.
+    constexpr bool KEEP_ROWS = !WIDE && NG == 1;
+    int row = -1, rows[KEEP_ROWS ? COPIES : 1];
     bool whole = false;
-    auto request_blocks = [&](unsigned dst, const uint8_t* store) {
-        const uint8_t* src[DEC_MT];
+    auto request_rows = [&](unsigned dst, const uint8_t* store, auto is_key) {
+        constexpr bool LOOK = decltype(is_key)::value || !KEEP_ROWS;
+        if (whole) {
+            const uint8_t* src[DEC_MT];
 #pragma unroll
-        for (int b = 0; b < DEC_MT; b++) src[b] = store + (int64_t)rows[b] * HD;
+            for (int b = 0; b < DEC_MT; b++) {
+                const int r = LOOK ? __shfl_sync(0xffffffffu, row, b * 16) : rows[KEEP_ROWS ? b : 0];
+                if constexpr (KEEP_ROWS) rows[b] = r;
+                src[b] = store + (int64_t)r * HD;
+            }
 #pragma unroll
-        for (int i = 0; i < COPIES; i++) {
-            const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
-            const int b = DEC_MT == 2 ? (COPIES % 2 == 0 ? i / (COPIES / 2) : key >> 4) : 0;
-            copy16(dst + key * HD + ((piece ^ dec_swizzle(key)) << 4), (b ? src[DEC_MT - 1] : src[0]) + (u * 16 - b * 16 * HD), true);
+            for (int i = 0; i < COPIES; i++) {
+                const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
+                const int b = DEC_MT == 2 ? (COPIES % 2 == 0 ? i / (COPIES / 2) : key >> 4) : 0;
+                copy16(dst + key * HD + ((piece ^ dec_swizzle(key)) << 4), (b ? src[DEC_MT - 1] : src[0]) + (u * 16 - b * 16 * HD), true);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < COPIES; i++) {
+                const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
+                const int r = LOOK ? __shfl_sync(0xffffffffu, row, key) : rows[KEEP_ROWS ? i : 0];
+                if constexpr (KEEP_ROWS) rows[i] = r;
+                copy16(dst + key * HD + ((piece ^ dec_swizzle(key)) << 4), store + (int64_t)max(r, 0) * HD + piece * 16, r >= 0);
+            }
         }
+        copies_commit();
     };
     auto request_k = [&](int stage, int meta_slot, int page, int slot) {
         const bool there = (unsigned)page < (unsigned)a.n_pages;
         const int cell = there ? page * a.n_kv + kvh : 0;
-        const int row = there ? cell * a.page_size + slot : -1;
+        row = there ? cell * a.page_size + slot : -1;
         if (lane < DEC_KT) {
             copy4(meta + meta_slot * DEC_META + lane * 8, a.kscale + cell, there);
             copy4(meta + meta_slot * DEC_META + lane * 8 + 4, a.vscale + cell, there);
         }
         whole = blocks && __all_sync(0xffffffffu, there);
-        if (whole) {
-            rows[0] = __shfl_sync(0xffffffffu, row, 0);
-            if constexpr (DEC_MT == 2) rows[1] = __shfl_sync(0xffffffffu, row, 16);
-            request_blocks(ring + stage * 2 * DEC_TILE, a.kcache);
-            copies_commit();
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < COPIES; i++) {
-            const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
-            rows[i] = __shfl_sync(0xffffffffu, row, key);
-            copy16(ring + stage * 2 * DEC_TILE + key * HD + ((piece ^ dec_swizzle(key)) << 4),
-                   a.kcache + (int64_t)max(rows[i], 0) * HD + piece * 16, rows[i] >= 0);
-        }
-        copies_commit();
+        request_rows(ring + stage * 2 * DEC_TILE, a.kcache, std::true_type{});
     };
-    auto request_v = [&](int stage) {
-        if (whole) {
-            request_blocks(ring + stage * 2 * DEC_TILE + DEC_TILE, a.vcache);
-            copies_commit();
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < COPIES; i++) {
-            const int u = i * 32 + lane, key = u / PIECES, piece = u % PIECES;
-            copy16(ring + stage * 2 * DEC_TILE + DEC_TILE + key * HD + ((piece ^ dec_swizzle(key)) << 4),
-                   a.vcache + (int64_t)max(rows[i], 0) * HD + piece * 16, rows[i] >= 0);
-        }
-        copies_commit();
-    };
+    auto request_v = [&](int stage) { request_rows(ring + stage * 2 * DEC_TILE + DEC_TILE, a.vcache, std::false_type{}); };
     float o[HD / 16][NG][4];
 #pragma unroll
     for (int i = 0; i < HD / 16; i++)
@@ -309,7 +311,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     float factor[NG][2], m_ref[NG][2], l_run[NG][2];
 #pragma unroll
     for (int ng = 0; ng < NG; ng++) {
-        const int h = SPREAD ? g8 & 1 : ng * 8 + g8;
+        const int h = SPREAD ? g8 & (SPREAD - 1) : ng * 8 + g8;
         float x[HD / 16][4];
         int m = 0;
 #pragma unroll
@@ -326,7 +328,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         const float f = finite ? a.scale * kLog2e * q8_pow2(-row_shift(m)) : __int_as_float(0x7fffffff);   // NaN: the row is
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            factor[ng][i] = __shfl_sync(0xffffffffu, f, (SPREAD ? i : 2 * t4 + i) * 4);
+            factor[ng][i] = __shfl_sync(0xffffffffu, f, (SPREAD == 2 ? i : 2 * t4 + i) * 4);
             m_ref[ng][i] = -INFINITY;
             l_run[ng][i] = 0.f;
         }
@@ -335,7 +337,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
             __half parts[4][NQ];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if constexpr (SPREAD) {
+                if constexpr (SPREAD == 2) {
                     __half all[Parts<T>::Q];
                     split<Parts<T>::Q>(finite ? x[kk][i] * up : 0.f, all);
                     parts[i][0] = pick(all, g8 >> 1);
@@ -413,7 +415,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         }
         __syncwarp();                                                 // everybody has read this tile's keys
         request_k(stage, meta_slot == 0 ? DEC_STAGES : meta_slot - 1, page_now, slot_now);
-        if constexpr (SPREAD) {                       // the parts of a score: every lane of a row has both heads' then
+        if constexpr (SPREAD == 2) {                  // the parts of a score: every lane of a row has both heads' then
 #pragma unroll
             for (int i = 0; i < DEC_MT * 4; i++) {
                 float& x = (&s[0][0][0])[i];
@@ -483,8 +485,8 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                         __half all[2][Parts<T>::P];
                         split<Parts<T>::P>(w[0], all[0]);
                         split<Parts<T>::P>(w[1], all[1]);
-                        h0[0] = pick(all[0], t4);
-                        h1[0] = pick(all[1], t4);
+                        h0[0] = pick(all[0], SPREAD == 2 ? t4 : t4 >> 1);
+                        h1[0] = pick(all[1], SPREAD == 2 ? t4 : t4 >> 1);
                     } else {
                         split<NP>(w[0], h0);
                         split<NP>(w[1], h1);
@@ -515,19 +517,43 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                 }
             }
 #pragma unroll
-            for (int w = 0; w < VW; w++)
+            for (int w = 0; w < VW; w++) {
+                uint32_t va[2][4];                                  // dims 4w, 4w + 1, then 4w + 2, 4w + 3
 #pragma unroll
-                for (int half = 0; half < 2; half++) {              // dims 4w, 4w + 1, then 4w + 2, 4w + 3
+                for (int half = 0; half < 2; half++) {
                     const unsigned sel = half ? 0x7362u : 0x5140u;
                     const uint32_t x = __byte_perm(vr[0][w], vr[1][w], sel), y = __byte_perm(vr[2][w], vr[3][w], sel);
-                    uint32_t a0, a1, a2, a3;
-                    q8_to_f16x4(x, a0, a1);
-                    q8_to_f16x4(y, a2, a3);
+                    q8_to_f16x4(x, va[half][0], va[half][1]);
+                    q8_to_f16x4(y, va[half][2], va[half][3]);
+                }
+                if constexpr (!WIDE) {
+#pragma unroll
+                    for (int half = 0; half < 2; half++)
+#pragma unroll
+                        for (int ng = 0; ng < NG; ng++)
+                            mma16816(o[2 * w + half][ng], va[half][0], va[half][1], va[half][2], va[half][3], pb[mt][0][ng][0], pb[mt][0][ng][1]);
+                } else {
+                    // Beside float32 queries sixteen keys at a time are added to a sum in registers: what the tensor core cuts off one long
+                    // sum added up, over 16001 keys, to three to five times float32 arithmetic's error.  It costs 2 to 8 %, with seven
+                    // or eight heads of 128 a CTA 11 to 19.
+                    float sum[2][NG][4];
 #pragma unroll
                     for (int k = NP - 1; k >= 0; k--)
 #pragma unroll
-                        for (int ng = 0; ng < NG; ng++) mma16816(o[2 * w + half][ng], a0, a1, a2, a3, pb[mt][k][ng][0], pb[mt][k][ng][1]);
+                        for (int half = 0; half < 2; half++)
+#pragma unroll
+                            for (int ng = 0; ng < NG; ng++) {
+                                if (k == NP - 1) mma16816_first(sum[half][ng], va[half][0], va[half][1], va[half][2], va[half][3], pb[mt][k][ng][0], pb[mt][k][ng][1]);
+                                else mma16816(sum[half][ng], va[half][0], va[half][1], va[half][2], va[half][3], pb[mt][k][ng][0], pb[mt][k][ng][1]);
+                            }
+#pragma unroll
+                    for (int half = 0; half < 2; half++)
+#pragma unroll
+                        for (int ng = 0; ng < NG; ng++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[2 * w + half][ng][j] += sum[half][ng][j];
                 }
+            }
         }
         __syncwarp();                                                 // everybody has read this tile's values
         request_v(stage);
@@ -544,17 +570,18 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         for (int j = 0; j < 2; j++) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l_run[ng][j] += __shfl_xor_sync(0xffffffffu, l_run[ng][j], d);
-            const int h = SPREAD ? j : ng * 8 + 2 * t4 + j;
-            if (g8 == 0 && (!SPREAD || t4 == 0)) { s_ml[warp][h][0] = m_ref[ng][j]; s_ml[warp][h][1] = l_run[ng][j]; }
+            const int h = SPREAD == 2 ? j : ng * 8 + 2 * t4 + j;
+            const bool mine = SPREAD == 0 || 2 * t4 < SPREAD;         // of the lanes that hold the head's columns, the first
+            if (g8 == 0 && mine) { s_ml[warp][h][0] = m_ref[ng][j]; s_ml[warp][h][1] = l_run[ng][j]; }
 #pragma unroll
             for (int i = 0; i < HD / 16; i++) {
                 // dims of rows g and g + 8 of step i: neighbours g * HD / 8 + 2 i, + 1
                 float2 v = make_float2(o[i][ng][j], o[i][ng][2 + j]);
                 if constexpr (SPREAD) {
-                    v.x += __shfl_xor_sync(0xffffffffu, v.x, 1);
-                    v.y += __shfl_xor_sync(0xffffffffu, v.y, 1);
+                    v.x += __shfl_xor_sync(0xffffffffu, v.x, SPREAD / 2);
+                    v.y += __shfl_xor_sync(0xffffffffu, v.y, SPREAD / 2);
                 }
-                if (!SPREAD || t4 == 0) *reinterpret_cast<float2*>(so + ((warp * NH + h) * HD + g8 * (HD / 8) + 2 * i)) = v;
+                if (mine) *reinterpret_cast<float2*>(so + ((warp * NH + h) * HD + g8 * (HD / 8) + 2 * i)) = v;
             }
         }
     __syncthreads();
@@ -634,7 +661,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     cluster_wait();
 }
 
-template <typename T, int NG, bool SPREAD = false>
+template <typename T, int NG, int SPREAD = 0>
 int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t stream) {
     constexpr size_t smem = DecodeShape<T, NG, SPREAD>::SMEM;
     static_assert(smem <= 227 * 1024, "shared memory");
@@ -1024,7 +1051,8 @@ extern "C" int kllm_attention_decode_q8(void* out, float* part_o, float* part_ml
         if (a.heads_per_cta > 8)
             return dtype == KLLM_F32 ? launch_decode<float, 2>(a, n_tokens, cluster, s) : launch_decode<bf16, 2>(a, n_tokens, cluster, s);
     }
-    if (dtype == KLLM_F32 && a.heads_per_cta <= 2) return launch_decode<float, 1, true>(a, n_tokens, cluster, s);
+    if (dtype == KLLM_F32 && a.heads_per_cta <= 2) return launch_decode<float, 1, 2>(a, n_tokens, cluster, s);
+    if (dtype == KLLM_F32 && a.heads_per_cta <= 4) return launch_decode<float, 1, 4>(a, n_tokens, cluster, s);
     return dtype == KLLM_F32 ? launch_decode<float, 1>(a, n_tokens, cluster, s) : launch_decode<bf16, 1>(a, n_tokens, cluster, s);
 }
 
