@@ -703,8 +703,8 @@ int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t s
 // the second's operand in registers.
 //
 // This form serves float32 and the head sizes that attention_q8_tcgen05.cu does not; its products are bound by mma.sync and by the
-// chain of a warp's 16 rows.  Measured, one prompt alone, back to back: float32, 2048 tokens of 32 heads over 4 of 64 164 us (105 TFLOP/s
-// counted once; the parts make three products and two of every one), over 8 of 128 294 us (117); 333 tokens 21.6 us (six tiles one
+// chain of a warp's 16 rows.  Measured, one prompt alone, back to back: float32, 2048 tokens of 32 heads over 4 of 64 173 us (99 TFLOP/s
+// counted once; the parts make three products and two of every one), over 8 of 128 313 us (110); 333 tokens 23.8 us (six tiles one
 // behind the other); bfloat16, 2048 tokens of 24 heads over 8 of 96 111 us (174), 16 over 8 of 256 223 us (154).
 
 constexpr int PRE_ROWS = 64, PRE_KEYS = 64, PRE_THREADS = 128;
@@ -732,8 +732,11 @@ struct PrefillArgs {
     float scale;
 };
 
+// CTAs an SM that there are registers for: with two at head size 64, 2048 float32 tokens of 32 heads over 4 took 195 us for 173.
+constexpr int PRE_CTAS = HD <= 32 ? 4 : HD <= 96 ? 3 : 2;
+
 template <typename T>
-__global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const PrefillArgs a) {
+__global__ void __launch_bounds__(PRE_THREADS, PRE_CTAS) attn_prefill_q8_kernel(const PrefillArgs a) {
     constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P;
     constexpr int LOADS = PRE_KEYS * PIECES / PRE_THREADS;   // pieces of K (and of V) a thread carries
     static_assert(PRE_KEYS * PIECES % PRE_THREADS == 0, "pieces per thread");
@@ -878,10 +881,25 @@ __global__ void __launch_bounds__(PRE_THREADS) attn_prefill_q8_kernel(const Pref
             for (int n = 0; n < PRE_KEYS / 16; n++) {
                 uint32_t b[4];
                 ldmatrix4(sk_u + kb_off + (unsigned)(n * 16 * PRE_LD * 2) + kk * 32, b);
+                if constexpr (NQ == 1) {
+                    mma16816(s[2 * n], qa[0][0], qa[0][1], qa[0][2], qa[0][3], b[0], b[1]);
+                    mma16816(s[2 * n + 1], qa[0][0], qa[0][1], qa[0][2], qa[0][3], b[2], b[3]);
+                } else {
+                    // The tensor core cuts its sums; beside float32 queries 16 products at a time are added to a sum in registers (one
+                    // sum over 256 dims was four times as far from 64 bits as the single tokens' scores).  It costs 5 to 11 %.
+                    float part[2][4];
+                    mma16816_first(part[0], qa[NQ - 1][0], qa[NQ - 1][1], qa[NQ - 1][2], qa[NQ - 1][3], b[0], b[1]);
+                    mma16816_first(part[1], qa[NQ - 1][0], qa[NQ - 1][1], qa[NQ - 1][2], qa[NQ - 1][3], b[2], b[3]);
 #pragma unroll
-                for (int j = NQ - 1; j >= 0; j--) {
-                    mma16816(s[2 * n], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b[0], b[1]);
-                    mma16816(s[2 * n + 1], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b[2], b[3]);
+                    for (int j = NQ - 2; j >= 0; j--) {
+                        mma16816(part[0], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b[0], b[1]);
+                        mma16816(part[1], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b[2], b[3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        s[2 * n][j] += part[0][j];
+                        s[2 * n + 1][j] += part[1][j];
+                    }
                 }
             }
         }

@@ -93,6 +93,18 @@ def test_scores_beside_float32_arithmetic(form, H, G, hd):
     hold(form, c, q, H, 3.5 / hd ** 0.5, torch.arange(400 - n, 400, device="cuda"))
 
 
+@pytest.mark.parametrize("H,G,hd", [(8, 2, 128), (4, 4, 160), (8, 2, 192), (4, 4, 256), (16, 2, 256)])
+def test_portions_are_as_near_as_single_tokens(H, G, hd):
+    """The same rows as single tokens and as a portion: their scores are sums of the same sums, of 32 or of 16 products, which are the error
+    at scores of this size.  So they are within half as much again of each other."""
+    c, n = Keys(400, G, hd, 16, seed=hd), 12
+    q = torch.randn(n, H * hd, generator=torch.Generator().manual_seed(hd + 1)).cuda()
+    last, scale = torch.arange(400 - n, 400, device="cuda"), 3.5 / hd ** 0.5
+    want = exact(c, q, H, scale, last)
+    one, portion = (float((kernel(form, c, q, H, scale, last).double() - want).square().mean().sqrt()) for form in ("decode", "prefill"))
+    assert portion <= 1.5 * one, f"{portion:.3g} from 64 bits, single tokens {one:.3g}"
+
+
 @pytest.mark.parametrize("form,H,G,hd,ctx", [("decode", 4, 4, 128, 16001), ("decode", 8, 2, 64, 16001), ("decode", 32, 2, 64, 9000),
                                              ("decode", 4, 1, 256, 9000), ("decode", 2, 2, 32, 30000), ("prefill", 8, 2, 64, 9000),
                                              ("prefill", 4, 1, 256, 5000)])
