@@ -441,7 +441,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                     for (int j = 0; j < 2; j++) {
                         float& x = s[mt][ng][2 * i + j];
                         x = seen ? fmaf(x * scales[0], factor[ng][j], (float)e) : -INFINITY;
-                        grown = grown || x > m_ref[ng][j] + kMoveAt;
+                        grown = grown || x > moves_above(m_ref[ng][j]);
                     }
             }
         if (__any_sync(0xffffffffu, grown)) {
@@ -454,7 +454,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                     for (int mt = 0; mt < DEC_MT; mt++) mx = fmaxf(mx, fmaxf(s[mt][ng][j], s[mt][ng][2 + j]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                    if (mx > m_ref[ng][j] + kMoveAt) {              // the same for every lane of the head
+                    if (mx > moves_above(m_ref[ng][j])) {              // the same for every lane of the head
                         const float corr = m_ref[ng][j] == -INFINITY ? 0.f : exp2f(m_ref[ng][j] - mx);
                         m_ref[ng][j] = mx;
                         l_run[ng][j] *= corr;
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(PRE_THREADS, PRE_CTAS) attn_prefill_q8_kernel(
         for (int i = 0; i < 2; i++) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-            if (mx[i] > m_ref[i] + kMoveAt) {
+            if (mx[i] > moves_above(m_ref[i])) {
                 const float corr = m_ref[i] == -INFINITY ? 0.f : exp2f(m_ref[i] - mx[i]);
                 m_ref[i] = mx[i];
                 l_run[i] *= corr;

@@ -80,6 +80,7 @@ constexpr int PIECES = HD / 16;            // 16-byte pieces of a stored row
 constexpr int LOADS = TILE * PIECES / LOADERS;           // pieces of the keys (of the values) a loader thread carries
 constexpr int KEY_STEP = LOADERS / PIECES;               // its pieces' keys are so far apart
 constexpr int ROW_LANES = HD / 8, ROWS_AT_ONCE = 32 / ROW_LANES;   // rows of 16-bit numbers as a warp reads and writes them
+constexpr float kLoud = 262144.f;          // from 2^18 on float32 numbers are 2^-5 and more apart
 constexpr int E_SPAN = 7;                  // how far a key's exponents may be from its step's
 
 // What the planner says of a step to everybody.  The note of step t is written once the values of step t - PLANS are converted,
@@ -622,6 +623,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             bool last = false;
             int step = 0, buf = x % SBUFS;
             unsigned parity = 0;
+            // The steps, in the way that is sound for references below 2^18.  False: the scores of `step` are beyond it, and nothing of that
+            // step is done.
+            auto steps = [&](auto is_loud) -> bool {
+            constexpr bool LOUD = decltype(is_loud)::value;
             for (; ok && !last; step++) {
                 ok = wait_at(smem_u32(&bar_note[step % NOTES]), (unsigned)(step / NOTES) & 1u, abort_at, a.status, 8) &&
                      wait_at(smem_u32(&bar_s_full[buf]), parity, abort_at, a.status, 9);
@@ -661,13 +666,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                     for (int j = 0; j < 32; j += 2) mx4[(j >> 1) & 3] = max3(mx4[(j >> 1) & 3], s[c][j], s[c][j + 1]);
                 const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 const float mx = top == -INFINITY ? -INFINITY : fmaf(top, f, ev);
-                const bool move = mx > m_ref + kMoveAt;
+                if (!LOUD && __any_sync(0xffffffffu, fabsf(mx) >= kLoud && mx != -INFINITY)) {
+                    last = false;
+                    return false;
+                }
+                const bool move = mx > moves_above(m_ref);
                 float corr = 1.f;
                 if (move) {
                     corr = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
                     m_ref = mx;
                 }
-                const float shift = m_ref == -INFINITY ? ev + kLift : ev - m_ref + kLift;
+                const float ref = m_ref == -INFINITY ? 0.f : m_ref, shift = ev - ref + kLift;
                 // The product of this row tile's step before has to be over.  With two score buffers and two row tiles it was
                 // issued before these scores, and is; otherwise it is waited for, every time (a wait by parity is only sound for
                 // the phase behind the one waited for last).
@@ -701,6 +710,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             float2 p = fma2(make_float2(s[half * 2 + c][j], s[half * 2 + c][j + 1]), f2, shift2);
+                            if (LOUD) {
+                                p.x = fmaf(s[half * 2 + c][j], f, ev) - ref + kLift;
+                                p.y = fmaf(s[half * 2 + c][j + 1], f, ev) - ref + kLift;
+                            }
                             p.x = fast_exp2(p.x);
                             p.y = fast_exp2(p.y);
                             sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], p);
@@ -717,6 +730,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 buf += tiles;
                 if (buf >= SBUFS) { buf -= SBUFS; parity ^= 1u; }
             }
+            return true;
+            };
+            // Near references so large that float32 numbers are whole units apart, s f + (ev - m_ref) in one rounding puts the largest weight
+            // beyond float16: there scores are rounded as the reference was, and then the difference is taken.  A loop of its own, as both
+            // in one cost the usual way registers (8192 tokens of head size 128: 597 to 631 us, one more addition a score always 579; this
+            // 564, of which the look at the maximum is 5).
+            if (!steps(std::false_type{})) steps(std::true_type{});
             if (ok) ok = wait_warp_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 11);
             if (ok) {
                 tc_fence_after();

@@ -85,8 +85,11 @@ __device__ __forceinline__ uint32_t q8_half2(float lo, float hi) {
 
 // ---- what the attention kernels share ----
 
-constexpr float kMoveAt = 8.f;              // the reference moves when the maximum has grown by 2^8
+constexpr float kMoveAt = 7.875f;           // the reference moves when the maximum has grown by more than 2^7.875
 constexpr float kLift = 7.f;                // weights are carried 2^7 up: float16's range below 1
+// What is above this moves the reference m.  Rounded down: where float32 numbers are 2, 4 or 8 apart, m - 7 may be m - 8, and with the
+// maximum at m + 8 a weight would be 2^16, which is no float16 number; it is at most m + 6 so.
+__device__ __forceinline__ float moves_above(float m) { return __fadd_rd(m, kMoveAt); }
 constexpr float kLog2e = 1.4426950408889634f;
 
 // 2^x, the hardware approximation: 2^-22 off at most, far below half a step of what the weight is rounded to or summed with

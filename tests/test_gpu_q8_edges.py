@@ -3,7 +3,10 @@ import dataclasses
 
 import pytest
 
-from test_gpu_q8 import DT, Cache, check, decode, ints, queries
+import torch
+
+import q8_plain as plain
+from test_gpu_q8 import DT, Cache, check, decode, ints, prefill, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +43,75 @@ def test_decode_rows_without_keys_in_clusters(dtype, hd, tokens, bound):
                 check(got[i:i + 1], q[i:i + 1], Rows(c, i), [starts[i]], [1], H, G, hd)
     if tokens == 1:
         assert kernels.decode_q8_parts(1, G, H // G, hd, bound)[0] > 1
+
+
+# ---- loud scores -----------------------------------------------------------------------------------------------------------
+
+PLACES = {"decode": ([99, 70, 200], [1, 1, 1]), "prefill": ([60, 0, 150], [40, 70, 51])}
+
+
+def attend(form, c, q, starts, lens, H, G, hd):
+    return decode(c, q, ints(*starts), H, G, hd) if form == "decode" else prefill(c, q, starts, lens, H, G, hd)
+
+
+@pytest.mark.parametrize("form", PLACES)
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 128, 96])
+@pytest.mark.parametrize("loud", [2.0 ** 16, 2.0 ** 23, 2.0 ** 24, 2.0 ** 25, 2.0 ** 40, 2.0 ** 80])
+def test_scores_beyond_what_float32_counts_in(form, dtype, hd, loud):
+    """Scores near which neighbouring float32 numbers are whole units apart: one key has all the weight, where it is ahead by more than
+    the scores' rounding and by 64 (weights of 2^-92), and the row is that key's values."""
+    H, G = 8, 2
+    starts, lens = PLACES[form]
+    c = Cache(starts, lens, G, hd, 16, seed=5)
+    q = queries(sum(lens), H, hd, dtype, seed=6, loud=loud)
+    got = attend(form, c, q, starts, lens, H, G, hd).cpu().double().view(-1, H, hd)
+    assert bool(torch.isfinite(got).all())
+    k, v = plain.values(c.k, c.ks), plain.values(c.v, c.vs)
+    half, at, alone = 2.0 ** -24 if dtype == "f32" else 2.0 ** -8, 0, 0
+    for r, (old, new) in enumerate(zip(starts, lens)):
+        j = torch.arange(old + new)
+        page, slot = c.table[r].long()[j // 16], j % 16
+        for i in range(new):
+            for h in range(H):
+                keys, vals = k[page[:old + i + 1], h // (H // G), slot[:old + i + 1]], v[page[:old + i + 1], h // (H // G), slot[:old + i + 1]]
+                qh = q[at + i].cpu().double().view(H, hd)[h]
+                s = keys @ qh * hd ** -0.5
+                size = float((keys.abs() @ qh.abs()).max()) * hd ** -0.5
+                top = torch.topk(s, min(2, s.numel()))
+                if s.numel() > 1 and float(top.values[0] - top.values[1]) < 64 + size * 2.0 ** -16:
+                    continue
+                alone += 1
+                want = vals[top.indices[0]]
+                assert bool(((got[at + i, h] - want).abs() <= half * want.abs() + 2.0 ** -24 * vals.abs().amax(dim=0)).all())
+        at += new
+    assert alone > sum(lens) * H // 2
+
+
+@pytest.mark.parametrize("form", PLACES)
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 96])
+@pytest.mark.parametrize("top", range(22, 31))
+@pytest.mark.parametrize("more", [2, 4, 6, 8, 16, 32])
+def test_a_maximum_that_grows_where_numbers_are_far_apart(form, dtype, hd, top, more):
+    """Two keys, tiles apart, at 2^top and a little more in units of log2; all the others are at 0.  The second one's weight is 2^-(their distance) of
+    the first one's whatever the reference is, as far as float32 tells them apart: a distance below half a unit of 2^top's last place is any
+    of 0 and that unit."""
+    far = 130
+    c = Cache([199], [1], 1, hd, 16, seed=1)
+    k, v = (torch.zeros(200, hd) for _ in range(2))
+    k[0, 0], k[far, 0], k[far, 1] = 256.0, 256.0, float(more)
+    v[0], v[far] = 1.0, -1.0
+    for store, rows in ((c.k, k), (c.v, v)):
+        for j in range(200):
+            store.view(torch.uint8)[int(c.table[0, j // 16]), 0, j % 16] = rows[j].to(plain.E4M3).view(torch.uint8).cuda()
+    c.ks.fill_(1.0), c.vs.fill_(1.0)
+    q = torch.zeros(1, hd)
+    q[0, 0], q[0, 1] = 2.0 ** (top - 8), 1.0
+    q = q.to(DT[dtype]).cuda()
+    scale = 0.6931471805599453                              # its product with log2 e is 1 but for float32's rounding
+    got = (decode(c, q, ints(199), 1, 1, hd, scale=scale, bound=1) if form == "decode" else prefill(c, q, [199], [1], 1, 1, hd, scale=scale))
+    ulp = 2.0 ** max(top - 23, -9)
+    out = lambda d: (1 - 2.0 ** d) / (1 + 2.0 ** d)  # noqa: E731
+    lo, hi = out(more + 1.0 * ulp), out(max(more - 1.0 * ulp, 0.0))
+    assert bool(torch.isfinite(got).all()) and bool((got.float() >= lo - 2.0 ** -8).all()) and bool((got.float() <= hi + 2.0 ** -8).all())
