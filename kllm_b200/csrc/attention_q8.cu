@@ -92,7 +92,7 @@ constexpr int KC = HD / (16 * KW);                       // pieces of a key row 
 constexpr int VW = HD / 32;                              // words of a lane's piece of a value row
 constexpr int PIECES = HD / 16;                          // 16-byte pieces of a row
 constexpr int DEC_TILE = DEC_KT * HD;                    // bytes of a tile of keys (or values)
-constexpr int DEC_META = DEC_KT * 8;                     // a tile's scales: (key scale, value scale) per key
+constexpr int DEC_META = DEC_KT * 8;                     // a tile's scales: (key scale, value scale) per key, then what is made of them
 constexpr int DEC_RING = DEC_STAGES * 2 * DEC_TILE + (DEC_STAGES + 1) * DEC_META;
 
 __device__ __forceinline__ int dec_swizzle(int key) {
@@ -248,6 +248,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     // is fetched from L2, as the rings leave no first-level cache.
     constexpr bool KEEP_ROWS = !WIDE && NG == 1;
     int row = -1, rows[KEEP_ROWS ? COPIES : 1];
+    unsigned held = 0;                    // bit i: the lane's key of the i'th tile on its way is seen
     bool whole = false;
     auto request_rows = [&](unsigned dst, const uint8_t* store, auto is_key) {
         constexpr bool LOOK = decltype(is_key)::value || !KEEP_ROWS;
@@ -284,6 +285,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
             copy4(meta + meta_slot * DEC_META + lane * 8, a.kscale + cell, there);
             copy4(meta + meta_slot * DEC_META + lane * 8 + 4, a.vscale + cell, there);
         }
+        held |= (unsigned)there << (DEC_STAGES - 1);
         whole = blocks && __all_sync(0xffffffffu, there);
         request_rows(ring + stage * 2 * DEC_TILE, a.kcache, std::true_type{});
     };
@@ -301,6 +303,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
     for (int i = 0; i <= DEC_STAGES; i++) find(tile_lo + warp + i * DEC_WARPS, page[i], slot[i]);
 #pragma unroll
     for (int i = 0; i < DEC_STAGES; i++) {
+        held >>= 1;
         request_k(i, i, page[i], slot[i]);
         request_v(i);
     }
@@ -364,6 +367,17 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         copies_wait<2 * DEC_STAGES - 1>();                            // this tile's keys and scales
         __syncwarp();
         const unsigned k_at = ring + stage * 2 * DEC_TILE, v_at = k_at + DEC_TILE;
+        // The scales of the lane's key, in their place, as all lanes want them: 2^ek and 2^-ev by their exponents in one word, ev (-inf: not
+        // seen).  What the scores need of them per key and lane is four instructions then.
+        if (lane < DEC_KT) {
+            float scales[2];
+            const unsigned at = meta + meta_slot * DEC_META + lane * 8;
+            read_words<2>(at, reinterpret_cast<uint32_t*>(scales));
+            const int ev = q8_exponent(scales[1]);
+            asm volatile("st.shared.v2.b32 [%0], {%1,%2};\n" ::"r"(at), "r"((q8_exponent(scales[0]) + 127) << 23 | (127 - ev) << 15),
+                         "r"(__float_as_int((held & 1u) ? (float)ev : -INFINITY)) : "memory");
+        }
+        held >>= 1;
         float s[DEC_MT][NG][4], part[DEC_MT][NG][4];
 #pragma unroll
         for (int mt = 0; mt < DEC_MT; mt++)
@@ -430,17 +444,16 @@ attn_decode_q8_kernel(const DecodeArgs a) {
         for (int mt = 0; mt < DEC_MT; mt++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                float scales[2];                    // of the key's page; zeros: not seen
-                read_words<2>(meta + meta_slot * DEC_META + (mt * 16 + i * 8 + dec_key(g8)) * 8, reinterpret_cast<uint32_t*>(scales));
-                const int e = q8_exponent(scales[1]);
-                const bool seen = scales[1] != 0.f;
-                inv[mt][i] = q8_pow2(-e);
+                uint32_t made[2];
+                read_words<2>(meta + meta_slot * DEC_META + (mt * 16 + i * 8 + dec_key(g8)) * 8, made);
+                const float mul = __uint_as_float(made[0] & 0x7f800000u), ev = __uint_as_float(made[1]);
+                inv[mt][i] = __uint_as_float(made[0] << 8 & 0x7f800000u);
 #pragma unroll
                 for (int ng = 0; ng < NG; ng++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         float& x = s[mt][ng][2 * i + j];
-                        x = seen ? fmaf(x * scales[0], factor[ng][j], (float)e) : -INFINITY;
+                        x = ev != -INFINITY ? fmaf(x * mul, factor[ng][j], ev) : -INFINITY;
                         grown = grown || x > moves_above(m_ref[ng][j]);
                     }
             }
@@ -820,7 +833,7 @@ __global__ void __launch_bounds__(PRE_THREADS, PRE_CTAS) attn_prefill_q8_kernel(
         if ((unsigned)page >= (unsigned)a.n_pages) return;
         const int cell = page * a.n_kv + kvh;
         next_row = cell * a.page_size + key - lp * a.page_size;
-        next_mul = a.kscale[cell];
+        next_mul = q8_pow2(q8_exponent(a.kscale[cell]));
         const int e = q8_exponent(a.vscale[cell]);
         next_ev = (float)e;
         next_inv = q8_pow2(-e);

@@ -331,7 +331,7 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
         const int e = key ? ke : ve, e_old = key ? ke_old : ve_old;
         // rows that the page holds already
         if (mine && slot && e != e_old) {
-            const float down = q8_pow2(max(e_old - e, -126));
+            const float down = q8_pow2(e_old - e);
             for (int r = first; r < slot; r += together) {
                 uint8_t* at[2] = {page_rows + (int64_t)r * hd + unit.at, page_rows + (int64_t)r * hd + unit.at2};
 #pragma unroll

@@ -27,8 +27,11 @@ constexpr int Q8_E_MIN = -48, Q8_E_MAX = 48;
 
 // 2^e for the exponents that scales have (and sums of a few)
 __device__ __forceinline__ float q8_pow2(int e) { return __int_as_float((e + 127) << 23); }
-// the exponent of a scale as stored; powers of two only
-__device__ __forceinline__ int q8_exponent(float scale) { return ((__float_as_int(scale) >> 23) & 0xff) - 127; }
+// the exponent of a scale as stored: of the power of two at or below it, within the range (0 is 2^-48, an infinity or NaN 2^48), by every
+// kernel, so that scales which the append did not leave mean the same to all of them
+__device__ __forceinline__ int q8_exponent(float scale) {
+    return min(max(((__float_as_int(scale) >> 23) & 0xff) - 127, Q8_E_MIN), Q8_E_MAX);
+}
 
 // the smallest e in [-48, 48] with m <= 448 * 2^e, from the bits of m >= 0: 448 = 1.75 * 2^8, so a mantissa above
 // 1.75 (0x600000) carries into the exponent

@@ -1206,7 +1206,8 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
                         block_table: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, window: int, scale: float,
                         ctx_bound: int) -> None:
     """Attention of single tokens over a cache in 8 bits (csrc/attention_q8.cu; stores and scales as ``rope_append_q8``
-    leaves them): row t, at ``positions[t]`` of request ``token_req[t]`` (None: request t), sees its request's keys up to
+    leaves them; a scale that it did not is taken for the power of two at or below it, 2^-48 for 0 and 2^48 for what is no number): row
+    t, at ``positions[t]`` of request ``token_req[t]`` (None: request t), sees its request's keys up to
     its own place (``window`` W > 0: the last W of them).  bfloat16 or float32 ``q`` and ``out`` [n, H*hd].  ``ctx_bound``:
     no context is longer; it only decides into how many parts the contexts are cut.  Keys whose table entry names no page
     are not seen; a row that sees none (a negative position, say) becomes zeros.  At most 65535 rows a call."""

@@ -1,8 +1,8 @@
 """The cache in 8 bits where its kernels have to agree with the definition and with each other."""
 import dataclasses
+import math
 
 import pytest
-
 import torch
 
 import q8_plain as plain
@@ -115,3 +115,49 @@ def test_a_maximum_that_grows_where_numbers_are_far_apart(form, dtype, hd, top, 
     out = lambda d: (1 - 2.0 ** d) / (1 + 2.0 ** d)  # noqa: E731
     lo, hi = out(more + 1.0 * ulp), out(max(more - 1.0 * ulp, 0.0))
     assert bool(torch.isfinite(got).all()) and bool((got.float() >= lo - 2.0 ** -8).all()) and bool((got.float() <= hi + 2.0 ** -8).all())
+
+
+# ---- scales --------------------------------------------------------------------------------------------------------------
+
+def cut(scale):
+    """The power of two that the kernels take a scale for."""
+    mantissa, exponent = torch.frexp(scale.abs().nan_to_num(math.inf, math.inf))
+    exponent = torch.where(torch.isfinite(mantissa) & (mantissa > 0), exponent - 1, torch.where(mantissa > 0, 48, -48))
+    return torch.ldexp(torch.ones_like(scale), exponent.clamp(-48, 48))
+
+
+@pytest.mark.parametrize("form", PLACES)
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 96])
+@pytest.mark.parametrize("which", ["ks", "vs"])
+@pytest.mark.parametrize("odd", [0.0, 3.0, 2.0 ** -60, 2.0 ** -140, 2.0 ** 60, math.inf, math.nan])
+def test_scales_that_the_append_does_not_leave(form, dtype, hd, which, odd):
+    """Every form takes a scale for the power of two below it, 2^-48 to 2^48."""
+    H, G = 8, 2
+    starts, lens = PLACES[form]
+    c = Cache(starts, lens, G, hd, 16, seed=5)
+    held = c.table[c.table >= 0].long()
+    getattr(c, which)[held[::3].cuda()] = odd
+    q = queries(sum(lens), H, hd, dtype, seed=6)
+    got = attend(form, c, q, starts, lens, H, G, hd)
+    c.ks[held.cuda()], c.vs[held.cuda()] = cut(c.ks[held.cuda()]), cut(c.vs[held.cuda()])
+    check(got, q, c, starts, lens, H, G, hd)
+
+
+@pytest.mark.parametrize("form", PLACES)
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 128, 96])
+@pytest.mark.parametrize("spread", [3.0, 8.0])
+@pytest.mark.parametrize("page", [16, 5])
+def test_scales_of_keys_and_values_far_apart(form, dtype, hd, spread, page):
+    """Pages whose keys' scales, and values', differ by more than a tile's step takes: the queries are as quiet as the keys are loud,
+    so that no key decides alone."""
+    H, G = 8, 2
+    starts, lens = PLACES[form]
+    c = Cache(starts, lens, G, hd, page, seed=5, spread=0.0)
+    g = torch.Generator().manual_seed(9)
+    for name in ("ks", "vs"):
+        e = (torch.randn(c.ks.shape, generator=g) * spread).round().clamp(-30, 30) - 7
+        setattr(c, name, torch.where(torch.isnan(getattr(c, name).cpu()), math.nan, torch.exp2(e)).cuda())
+    q = queries(sum(lens), H, hd, dtype, seed=6, loud=2.0 ** (-2 * spread))
+    check(attend(form, c, q, starts, lens, H, G, hd), q, c, starts, lens, H, G, hd)
