@@ -13,7 +13,7 @@
 // A row of bfloat16 queries is one float16 operand, exactly, after division by a power of two that brings its largest
 // magnitude to 2^14..2^15; a float32 row is the sum of three (33 bits).  Weights are one float16 (11 bits: half a step is
 // 2^-12, against bfloat16's 2^-9), beside float32 queries two (22 bits).  A row with an infinity or NaN among its queries
-// becomes NaN.
+// becomes NaN, if it sees a key.
 //
 // Keys without a page (a table entry outside the pages, a place behind the table's end) are not seen.  A row that sees no
 // key becomes zeros.

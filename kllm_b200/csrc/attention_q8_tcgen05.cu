@@ -636,8 +636,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
                 tc_fence_after();
                 const Note& note = s_note[step % NOTES];
                 last = note.last != 0;
-                // never 0 (a scale of 0, tiny queries): -inf has to stay -inf; NaN stays
-                const float product = factor * q8_pow2(note.ek), f = product < 1.1754944e-38f ? 1.1754944e-38f : product;
+                // never 0 (a scale of 0, tiny queries) nor NaN (queries that are not finite: numbers of 0): -inf has to stay -inf
+                const float product = factor * q8_pow2(note.ek), f = product >= 1.1754944e-38f ? product : 1.1754944e-38f;
                 const float ev = (float)note.ev, per_sum = q8_pow2(-note.ev);
                 // which of the tile's keys this row sees
                 const int upto = p_row - note.key0 + 1, from = w_row - note.key0;
@@ -737,6 +737,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_q8_tc5_kernel(const A
             // in one cost the usual way registers (8192 tokens of head size 128: 597 to 631 us, one more addition a score always 579; this
             // 564, of which the look at the maximum is 5).
             if (!steps(std::false_type{})) steps(std::true_type{});
+            if (factor != factor && m_ref != -INFINITY) l_run = factor;        // the row is NaN where it saw a key
             if (ok) ok = wait_warp_at(smem_u32(&bar_pv[x]), (unsigned)(step - 1) & 1u, abort_at, a.status, 11);
             if (ok) {
                 tc_fence_after();

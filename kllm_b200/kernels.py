@@ -1210,7 +1210,8 @@ def attention_decode_q8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor
     t, at ``positions[t]`` of request ``token_req[t]`` (None: request t), sees its request's keys up to
     its own place (``window`` W > 0: the last W of them).  bfloat16 or float32 ``q`` and ``out`` [n, H*hd].  ``ctx_bound``:
     no context is longer; it only decides into how many parts the contexts are cut.  Keys whose table entry names no page
-    are not seen; a row that sees none (a negative position, say) becomes zeros.  At most 65535 rows a call."""
+    are not seen; a row that sees none (a negative position, say) becomes zeros, another whose queries hold an infinity or NaN becomes
+    NaN.  At most 65535 rows a call."""
     _check_q8("attention_decode_q8", kcache, vcache, kscale, vscale, block_table, n_heads, n_kv, head_dim)
     code, n, stride = _check_q8_rows("attention_decode_q8", out, q, n_heads, head_dim)
     _check_q8_ints("attention_decode_q8", positions)

@@ -45,6 +45,28 @@ def test_decode_rows_without_keys_in_clusters(dtype, hd, tokens, bound):
         assert kernels.decode_q8_parts(1, G, H // G, hd, bound)[0] > 1
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 128, 96])
+@pytest.mark.parametrize("far", [30, 8000])
+def test_rows_without_keys_are_zeros_whatever_their_queries(dtype, hd, far):
+    H, G = 8, 2
+    starts, lens = [far, -40, 20], [8, 30, 9]
+    c = Cache(starts, lens, G, hd, 16, seed=5)
+    c.table[2, 0] = -1                                     # places 0 to 15 of the last request
+    c.dev_table = c.table.cuda()
+    q = queries(sum(lens), H, hd, dtype, seed=6)
+    q[8:38:2, 3] = math.nan
+    q[9:38:2, 2 * hd + 1] = -math.inf
+    got = prefill(c, q, starts, lens, H, G, hd)
+    assert not got[8:38].any()
+    single = decode(c, q, ints(*range(far, far + 8), *range(-40, -10), *range(20, 29)), H, G, hd, req=ints(*[0] * 8, *[1] * 30, *[2] * 9))
+    assert not single[8:38].any()
+    rest = [i for i in range(47) if not 8 <= i < 38]
+    want, err = plain.attention(q[rest], c.k, c.v, c.ks, c.vs, c.table[[0, 2]], [far, 20], [8, 9], H, G, hd, 0, hd ** -0.5)
+    for t in (got, single):
+        assert bool(((t[rest].cpu().double() - want).abs() <= err).all())
+
+
 # ---- loud scores -----------------------------------------------------------------------------------------------------------
 
 PLACES = {"decode": ([99, 70, 200], [1, 1, 1]), "prefill": ([60, 0, 150], [40, 70, 51])}
