@@ -7,15 +7,16 @@
 // and where e > e_old the earlier rows become e4m3(old * 2^(e_old - e)).  A row whose key or value is not finite counts
 // for no maximum; its key is stored as NaN and its value as 0.
 // The rotation is that of rope.cu: rotate_half, float32, angles from a table computed in float64.  A key's byte is the e4m3
-// number next to its exact rotation by the table's angles.
+// number next to its exact rotation by the table's angles, and its page's scale follows the exact rotation too.
 //
 // What bounds it: bytes, and for few tokens a chain of dependent loads.  A CTA takes a few tokens and one of two jobs: it
 // rotates some of their query heads, or it stores whole runs of rows of some kv heads: the first token of a request's rows in a
 // page (the request's first token of the step, or slot 0) does it for all of them, so that exactly one CTA touches a (page,
 // kv head) and its scale.  A thread keeps its place in the rows and walks the rows, without a division per unit.  A run is
 // read twice, the second time from the first-level cache: once for the largest magnitudes (integer maxima in shared memory:
-// their order does not matter), once to store.  Rows that are not finite are rare: they are marked on the first way, and only
-// where there are any the maxima are taken again without them.
+// their order does not matter), once to store.  Rows that are not finite are rare, as are maxima beside a border of the scales: the former
+// are marked on the first way, and only where there are any of either the maxima are taken again, without those rows and from the exact
+// rotation.
 //
 // Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.5 us, 2048 tokens 9.8 us (20 MB, 2.1 TB/s; copies at
 // 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 76.6 us (285 MB, 3.7 TB/s,
@@ -150,6 +151,16 @@ __device__ __noinline__ float turned_to_odd(float a, float c, float b, float s) 
     }
     return __int_as_float(bits);
 }
+template <typename T, int U> __device__ __forceinline__ void turn_to_odd(const Raw<T, U>& w, float (&v)[2 * U]) {
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        v[i] = turned_to_odd(w.x[i], w.c[i], w.y[i], w.s[i]);
+        v[U + i] = turned_to_odd(w.y[i], w.c[i], -w.x[i], w.s[i]);
+    }
+}
+// Whether a largest magnitude (its bits) is so near to a border of the scales, 448 * 2^e, that the exact one may be beyond it: a pair
+// turned in float32 arithmetic by angles on a circle is off by 1.5 last places of its larger number.
+__device__ __forceinline__ bool beside_border(int bits) { return (unsigned)((bits & 0x7fffff) - 0x5ffffc) <= 8u; }
 // The unit as e4m3.  Turned numbers are within 1.5 last places here (the error of the product that is rounded first is taken off the
 // sum): where a number times 1 - 2^-21 and times 1 + 2^-21 round alike, so does the exact one.  A unit with one that does not
 // (once in 10^4 units) is taken again.
@@ -173,11 +184,7 @@ __device__ __forceinline__ void pack_unit(const Raw<T, U>& w, bool turned, float
 #pragma unroll
     for (int i = 0; i < kWords<U>; i++) differ |= (a[i] ^ a2[i]) | (b[i] ^ b2[i]);
     if (differ) {
-#pragma unroll
-        for (int i = 0; i < U; i++) {
-            v[i] = turned_to_odd(w.x[i], w.c[i], w.y[i], w.s[i]);
-            v[U + i] = turned_to_odd(w.y[i], w.c[i], -w.x[i], w.s[i]);
-        }
+        turn_to_odd<T, U>(w, v);
         pack8<U>(v, mul, a);
         pack8<U>(v + U, mul, b);
     }
@@ -309,7 +316,9 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
         if (mine) atomicMax(&s_max[h][key], m);
         __syncthreads();
         const bool any = s_any != 0;
-        if (any) {                                                  // the same for all threads
+        bool again = any;
+        for (int j = 0; j < heads; j++) again = again || (rot > 0 && beside_border(s_max[j][1]));
+        if (again) {                                                // the same for all threads: without those rows, from the exact rotation
             __syncthreads();
             if (tid < 2 * kMaxHeads) s_max[tid >> 1][tid & 1] = 0;
             __syncthreads();
@@ -319,7 +328,8 @@ rope_append_q8_kernel(T* q_out, int64_t qo_stride, const T* q, int64_t q_stride,
                 Raw<T, U> w;
                 float x[2 * U];
                 read(r, w);
-                turn<T, U>(w, turned, x);
+                turn<T, U>(w, false, x);
+                if (turned) turn_to_odd<T, U>(w, x);
 #pragma unroll
                 for (int j = 0; j < 2 * U; j++) m = max(m, __float_as_int(x[j]) & 0x7fffffff);
             }

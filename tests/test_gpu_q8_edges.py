@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import q8_plain as plain
-from test_gpu_q8 import DT, Cache, check, decode, ints, prefill, queries
+from test_gpu_q8 import DT, Cache, check, decode, ints, prefill, queries, run_append, table_of_angles
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +183,55 @@ def test_scales_of_keys_and_values_far_apart(form, dtype, hd, spread, page):
         setattr(c, name, torch.where(torch.isnan(getattr(c, name).cpu()), math.nan, torch.exp2(e)).cuda())
     q = queries(sum(lens), H, hd, dtype, seed=6, loud=2.0 ** (-2 * spread))
     check(attend(form, c, q, starts, lens, H, G, hd), q, c, starts, lens, H, G, hd)
+
+
+# ---- append ---------------------------------------------------------------------------------------------------------------
+
+def hold_append(c, before, k, v, cs, pos, starts, lens, G, hd):
+    """Equality with the exact rotation rounded once, of every number and scale."""
+    n = sum(lens)
+    kr, vr = plain.turned(k[:n], cs, pos[:n], G, hd), v[:n].cpu().double().view(n, G, hd)
+    for (store, scale), kept, is_key in (((c.k, c.ks), before[0], True), ((c.v, c.vs), before[1], False)):
+        want, sc, _ = plain.append(*kept, kr, vr, is_key, c.table, starts, lens)
+        assert torch.equal(scale.cpu().double().nan_to_num(-1.0), sc.nan_to_num(-1.0))
+        assert torch.equal(store.cpu().float().double().nan_to_num(1e6), want.nan_to_num(1e6))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,G,hd,rot", [(4, 2, 64, 64), (4, 2, 64, 6), (64, 64, 96, 48)])
+@pytest.mark.parametrize("step", [0, 7])
+@pytest.mark.parametrize("by", [1.0, 2.0 ** -9])
+def test_a_pages_scale_follows_the_exact_rotation(dtype, H, G, hd, rot, step, by):
+    """Keys that the rotation turns to 448 2^e and 2^-39 of it more, which float32 does not hold: they belong under the next scale.  As much
+    less, they do not."""
+    n = 32 if G < 64 else 960
+    starts, lens = [step], [n]
+    c = Cache(starts, lens, G, hd, 16, seed=3, fill=False)
+    cs = torch.zeros(n + step, rot, device="cuda")
+    cs[:, :rot // 2], cs[:, rot // 2:] = 1.0, 2.0 ** -20
+    k = queries(n, G, hd, dtype, 2, loud=by)
+    for g in range(G):
+        for r in range(n):
+            if r % 16 == 3 and g % 3 < 2:                 # a page's largest: just above, just below, none
+                k[r, g * hd] = 448.0 * by
+                k[r, g * hd + rot // 2] = (-2.0 ** -10 if g % 3 == 0 else 2.0 ** -10) * by
+    q, v = queries(n, H, hd, dtype, 1), queries(n, G, hd, dtype, 3)
+    before = [(c.k.clone(), c.ks.clone()), (c.v.clone(), c.vs.clone())]
+    q_out, pos = run_append(c, q, k, v, cs, starts, lens, H, G, hd)
+    hold_append(c, before, k, v, cs, pos, starts, lens, G, hd)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,G,hd,rot", [(8, 2, 64, 64), (4, 4, 128, 128), (3, 1, 32, 32), (10, 2, 96, 48), (8, 1, 256, 256), (4, 2, 64, 6),
+                                        (8, 8, 64, 2)])
+@pytest.mark.parametrize("page,starts,lens", [(16, [0], [1]), (16, [0, 5, 31], [40, 12, 2]), (5, [3, 0], [17, 9]), (64, [10, 100, 0], [1, 1, 1]),
+                                              (256, [0, 130], [200, 150]), (1, [2, 0], [3, 4])])
+def test_append_to_the_bit(dtype, H, G, hd, rot, page, starts, lens):
+    for seed in range(3):
+        c = Cache(starts, lens, G, hd, page, seed=page + hd + seed, fill=False)
+        n = sum(lens)
+        q, k, v = queries(n, H, hd, dtype, 7 * seed + 1), queries(n, G, hd, dtype, 7 * seed + 2, loud=5.0), queries(n, G, hd, dtype, 7 * seed + 3)
+        cs = table_of_angles(400, rot)
+        before = [(c.k.clone(), c.ks.clone()), (c.v.clone(), c.vs.clone())]
+        q_out, pos = run_append(c, q, k, v, cs, starts, lens, H, G, hd)
+        hold_append(c, before, k, v, cs, pos, starts, lens, G, hd)
