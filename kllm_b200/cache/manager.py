@@ -35,6 +35,7 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
+from ..kernels import Q8_MAX_PAGE
 from ..parts.context import LayerCache
 from ..parts.spec import PagedKVNeed, StateNeed
 
@@ -158,6 +159,8 @@ class CacheManager:
                             item.value_heads != item.n_kv_heads or item.value_dim > item.head_dim)):
                         raise ValueError(f"cache slot {slot}: {item.value_heads} value heads of {item.value_dim} under "
                                          f"{item.n_kv_heads} key heads of {item.head_dim}")
+                    if self.eight_bits and page_size > Q8_MAX_PAGE:
+                        raise ValueError(f"pages of {page_size} tokens: a cache in 8 bits takes at most {Q8_MAX_PAGE}")
                     if self.eight_bits and not item.eight_bits:
                         raise ValueError(f"cache slot {slot}: this kind of layer does not take a cache in 8 bits "
                                          f"({item.n_kv_heads} key heads of {item.head_dim})")
