@@ -100,13 +100,24 @@ class DecoderModel:
         the arrangement keeps something of its own."""
         needs = []
         for slot in range(self.n_cache_slots):
-            block = self.blocks[self._writer_block[slot]]
-            need = (block if hasattr(block, "cache_need") else block.mixer).cache_need()
-            if isinstance(need, PagedKVNeed) and need.eight_bits and not all(
-                    getattr(self.blocks[c.block].mixer.cache_need(), "eight_bits", False) for c in self.schedule if c.cache == slot):
-                need = dataclasses.replace(need, eight_bits=False)      # another layer reads this slot, and cannot
+            need = self._need_of(self.blocks[self._writer_block[slot]])
+            readers = [self.blocks[c.block] for c in self.schedule if c.cache == slot]
+            if not all(any(paged) and all(paged) for paged in map(self._eight_bits_of, readers)):
+                # a layer that reads this slot cannot: then the one that writes it must not
+                wide = lambda n: dataclasses.replace(n, eight_bits=False) if isinstance(n, PagedKVNeed) else n  # noqa: E731
+                need = [wide(n) for n in need] if isinstance(need, (list, tuple)) else wide(need)
             needs.append(need)
         return needs
+
+    @staticmethod
+    def _need_of(block):
+        part = block if hasattr(block, "cache_need") else getattr(block, "mixer", None)
+        return part.cache_need() if part is not None else None
+
+    def _eight_bits_of(self, block):
+        """Of every paged cache that the block asks for: whether its kernels take 8 bits."""
+        need = self._need_of(block)
+        return [n.eight_bits for n in (need if isinstance(need, (list, tuple)) else [need]) if isinstance(n, PagedKVNeed)]
 
     # ---- one step --------------------------------------------------------
     def forward(self, ctx: StepContext, caches: List[LayerCache]) -> Optional[torch.Tensor]:
