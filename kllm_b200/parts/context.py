@@ -55,6 +55,6 @@ class LayerCache:
     state: Optional[torch.Tensor]        # [slots, *state shape]
     writes: bool = True
     page_size: int = 0
+    states: Dict[str, torch.Tensor] = field(default_factory=dict)   # further states of the layer by name, [slots, *shape]
     k_scale: Optional[torch.Tensor] = None   # a cache in 8 bits: float32 [pages, kv heads], and k, v are float8_e4m3fn
     v_scale: Optional[torch.Tensor] = None
-    states: Dict[str, torch.Tensor] = field(default_factory=dict)   # further states of the layer by name, [slots, *shape]

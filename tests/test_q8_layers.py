@@ -70,3 +70,11 @@ def test_every_reader_of_a_slot_is_asked(writer, reader):
 def test_a_reader_without_a_mixer_does_not_take_it():
     model = shared_slot(None, lambda i, b: Bare() if i == 1 else b)
     assert [taken(n) for n in model.cache_needs()] == [[False], [True]]
+
+
+def test_a_layers_view_is_built_as_before():
+    """Positions of the fields that were there before the scales."""
+    from kllm_b200.parts.context import LayerCache
+    states = {"conv": torch.zeros(1)}
+    c = LayerCache(None, None, None, None, True, 16, states)
+    assert c.page_size == 16 and c.states is states and c.k_scale is None and c.v_scale is None
