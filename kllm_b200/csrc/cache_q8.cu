@@ -395,8 +395,9 @@ void launch(dim3 grid, int threads, size_t smem, cudaStream_t s, A... a) {
 
 // q_out [n, heads*hd] at qo_stride (may be q itself), q/k/v rows dense at their strides, element type dtype; cos_sin float32
 // [n_pos, rot] (rot 0: no rotation); token_req may be NULL (token t is request t's only one); caches [pages, n_kv, page, hd]
-// e4m3, scales float32 [pages, n_kv].  Nothing is read or stored for a token whose position is negative, outside the
-// table of angles, or without a page.
+// e4m3, scales float32 [pages, n_kv].  Nothing is stored in the caches for a token whose position is negative or outside the table of
+// angles, or that has no page.  Its query: of a position outside the table only what is not rotated is written, and that only where
+// q_out is not q; a query of a token without a page is rotated and written like any other.
 extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q, int64_t q_stride, const void* k,
                                    int64_t k_stride, const void* v, int64_t v_stride, const float* cos_sin, int n_pos,
                                    const int* positions, const int* token_req, const int* q_start, int n_requests,
