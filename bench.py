@@ -244,6 +244,8 @@ def main():
                     help="layer sizes; other than the default it is a measurement at further sizes, not the bench line")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"],
                     help="float32: the whole line is measured on the true 32-bit path (not the bench line)")
+    ap.add_argument("--cache-dtype", default="", choices=["", "float8_e4m3fn"],
+                    help="keep keys and values in 8 bits (default: the dtype of the weights); not the benchmark's line")
     ap.add_argument("--repeats", type=int, default=0, help="how often the K-step region is timed (0: 5, or 3 for K > 40)")
     ap.add_argument("--prefill-tokens", type=int, default=2048, help="length of the timed prompt")
     ap.add_argument("--no-points", action="store_true", help="skip the further points and the prefill")
@@ -310,7 +312,7 @@ def main():
         pages = max(batch_limit * (-(-ctx // page)), -(-args.prefill_tokens // page)) + 8
         return Options(dtype=dtype, max_seq=max(ctx, args.prefill_tokens), block_size=page, num_blocks=pages,
                        max_batch=batch_limit, max_step_tokens=max(args.prefill_tokens, batch_limit),
-                       cuda_graphs=not args.no_graphs)
+                       cuda_graphs=not args.no_graphs, cache_dtype=args.cache_dtype)
 
     tmp = None
     if args.shape == "tinyllama-1.1b":
@@ -475,7 +477,8 @@ def main():
                            "vocab": cfg["vocab_size"], "page_size": page,
                            "l2": f"step reads {step_bytes / 1e9:.1f} GB > 126 MB L2, no flush",
                            "peaks": pk["source"], "repeats": R,
-                           "timing": "median of the repeats of K steps; CUDA events, wall clock for e2e"},
+                           "timing": "median of the repeats of K steps; CUDA events, wall clock for e2e"}
+                | ({"cache_dtype": args.cache_dtype} if args.cache_dtype else {}),
                 "spread": {"repeats": R, "min_ms": round(min(run["dev_all"]), 4), "max_ms": round(max(run["dev_all"]), 4)},
                 "clocks": run["clocks"],
                 "e2e": {"value": round(B / (run["e2e_ms"] * 1e-3), 1), "unit": "tokens/s",
