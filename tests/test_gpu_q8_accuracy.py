@@ -116,6 +116,19 @@ def test_long_contexts_beside_float32_arithmetic(form, H, G, hd, ctx):
     hold(form, c, q, H, 0.5 / hd ** 0.5, torch.arange(ctx - n, ctx, device="cuda"))
 
 
+@pytest.mark.parametrize("H,G,hd,ctx", [(4, 4, 96, 131072), (4, 4, 160, 100000), (4, 4, 256, 60000)])
+def test_long_contexts_of_bfloat16_portions(H, G, hd, ctx):
+    """What is left of the error beside the output's rounding: weights, 2^-12 each, of many thousand keys, and a float32 rounding a tile, which
+    are 2^-19 together.  A sum of the tensor core that all keys join is cut by up to 2^-23 at every sixteen of them, to one side."""
+    c, n = Keys(ctx, G, hd, 64, seed=hd, positive=True), 16
+    q = (torch.randn(n, H * hd, generator=torch.Generator().manual_seed(1)) * 0.05).bfloat16().cuda()
+    last = torch.arange(ctx - n, ctx, device="cuda")
+    want = exact(c, q, H, hd ** -0.5, last)
+    far = lambda t: float(((t.double() - want) / want).square().mean().sqrt())  # noqa: E731
+    here, rounding = far(kernel("prefill", c, q, H, hd ** -0.5, last)), far(want.bfloat16())
+    assert here <= 1.01 * rounding, f"{here:.4g} from 64 bits, rounding alone {rounding:.4g}"
+
+
 @pytest.mark.parametrize("form", ["decode", "prefill"])
 @pytest.mark.parametrize("H,G,hd", [(2, 2, 64), (4, 1, 64), (2, 1, 128)])
 def test_queries_keep_all_their_bits(form, H, G, hd):
