@@ -6,7 +6,7 @@
 // where ek, ev are the exponents of the page's scales.  A value page's exponent goes into the weight's: with a reference M,
 //     w_j = 2^(s_j + ev(j) - M + 7),   l = sum_j w_j 2^-ev(j),   O = sum_j w_j v8_j,   out = O / l,
 // so that one exponential a score serves both sums, whatever the pages' scales are.  The reference follows the running
-// maximum of s_j + ev(j) and is moved only when that has grown by more than 8: w stays below 2^15, a float16 number, and
+// maximum of s_j + ev(j) and is moved only when that has grown by more than 7.875: w stays below 2^15, a float16 number, and
 // what is smaller than 2^-32 of the largest weight is lost.
 //
 // Products run on the tensor cores in float16 with float32 sums (mma.sync m16n8k16): e4m3 numbers are float16 numbers.
@@ -78,9 +78,9 @@ template <int N> __device__ __forceinline__ __half pick(const __half (&p)[N], in
 // transposition in registers (movmatrix).  Row r of a tile is key r ^ (r >> 1 & 1) of it, and the 16-byte pieces of key j lie
 // at piece ^ swizzle(j): with both, neither kind of read meets a bank twice at head sizes 64 and 128.
 //
-// Measured, back to back, bfloat16 (% of a copy's 6.45 TB/s): 64 requests of 846 to 4095 keys, 32 heads over 8 of 128, pages of 16: 67.6 us (74 %);
-// one of 131072 keys 53.8 us (77 %); 8 of 2048 keys, 32 over 4 of 64: 8.2 us; one: 5.9 us, a chain of launch, table, tiles and
-// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 17.5 us (38 %).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
+// Measured, back to back, bfloat16 (% of a copy's 6.45 TB/s): 64 requests of 846 to 4095 keys, 32 heads over 8 of 128, pages of 16: 69.9 us (72 %);
+// one of 131072 keys 54.2 us (77 %); 8 of 2048 keys, 32 over 4 of 64: 8.6 us; one: 6.2 us, a chain of launch, table, tiles and
+// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 17.8 us (37 %).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
 // 64 (16 of a CTA pair an SM as before): 64 x 2048 keys 18.7 us against 19.6, 128 x 1000 23.0 against 18.8.
 
 constexpr int DEC_KT = HD <= 128 ? 32 : 16;              // keys of a warp's tile
@@ -102,9 +102,9 @@ __device__ __forceinline__ int dec_key(int row) { return row ^ ((row >> 1) & 1);
 
 // SPREAD: where a CTA has one or two heads of float32 queries, the parts of a head's queries, and of its weights, are columns
 // of the N side (part p of head h is column 2 p + h) instead of products of their own: a third of the first product's
-// instructions and half of the second's (32 heads of 128, 8 x 2048 keys: 35.6 us against more than 40).  Three or four heads: the
+// instructions and half of the second's (32 heads of 128, 8 x 2048 keys: 36.7 us against more than 40).  Three or four heads: the
 // weights' parts alone (part p of head h is column 4 p + h; both columns have the head's queries): 64 x 2048 keys of 32 heads over 8
-// of 128 59.7 us, with two products a part's sum 85, of which most is four registers too many.
+// of 128 60.8 us, with two products 85, of which most is what registers were missing.
 template <typename T, int NG, int SPREAD> struct DecodeShape {
     static constexpr int NQ = SPREAD == 2 ? 1 : Parts<T>::Q;
     static constexpr int QREGS = HD / 16 * 2 * NQ * NG;
@@ -716,9 +716,9 @@ int launch_decode(const DecodeArgs& a, int n_tokens, int cluster, cudaStream_t s
 // the second's operand in registers.
 //
 // This form serves float32 and the head sizes that attention_q8_tcgen05.cu does not; its products are bound by mma.sync and by the
-// chain of a warp's 16 rows.  Measured, one prompt alone, back to back: float32, 2048 tokens of 32 heads over 4 of 64 173 us (99 TFLOP/s
-// counted once; the parts make three products and two of every one), over 8 of 128 313 us (110); 333 tokens 23.8 us (six tiles one
-// behind the other); bfloat16, 2048 tokens of 24 heads over 8 of 96 111 us (174), 16 over 8 of 256 223 us (154).
+// chain of a warp's 16 rows.  Measured, one prompt alone, back to back: float32, 2048 tokens of 32 heads over 4 of 64 172 us (100 TFLOP/s
+// counted once; the parts make three products and two of every one), over 8 of 128 310 us (111); 333 tokens 23.4 us (six tiles one
+// behind the other); bfloat16, 2048 tokens of 24 heads over 8 of 96 114 us (170), 16 over 8 of 256 222 us (155).
 
 constexpr int PRE_ROWS = 64, PRE_KEYS = 64, PRE_THREADS = 128;
 constexpr int PRE_LD = HD + 8;                            // halves of a row in shared memory: eight rows on eight bank groups
@@ -745,7 +745,7 @@ struct PrefillArgs {
     float scale;
 };
 
-// CTAs an SM that there are registers for: with two at head size 64, 2048 float32 tokens of 32 heads over 4 took 195 us for 173.
+// CTAs an SM that there are registers for: with two at head size 64, 2048 float32 tokens of 32 heads over 4 took 195 us for 172.
 constexpr int PRE_CTAS = HD <= 32 ? 4 : HD <= 96 ? 3 : 2;
 
 template <typename T>

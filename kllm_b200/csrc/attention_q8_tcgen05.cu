@@ -25,12 +25,12 @@
 // one tile are hardly ever so far apart).  So a step has one factor for its scores, one shift for its weights and one
 // for the sum, none of them per score.
 //
-// The output accumulates in TMEM; a row's reference is moved only when its maximum has grown by 2^8 (then the row of the
+// The output accumulates in TMEM; a row's reference is moved only when its maximum has grown by more than 2^7.875 (then the row of the
 // accumulator is read, rescaled and written back between two products).  Few row tiles behind a long context are cut
 // over the keys: every part leaves its unscaled rows, references and sums, which a second kernel joins in order.
 //
-// Measured, back to back: one prompt of 8192 tokens, 32 heads over 4 of 64: 416 us (661 TFLOP/s), over 8 of 128: 558 us (985, 59 % of a
-// library product's 1671); 2048 tokens: 39 and 53 us; 512 behind 7680 over 8 of 128: 88 us.  A step of two row tiles takes 4300 cycles at
+// Measured, back to back: one prompt of 8192 tokens, 32 heads over 4 of 64: 423 us (650 TFLOP/s), over 8 of 128: 565 us (973, 58 % of a
+// library product's 1671); 2048 tokens: 39.6 and 54 us; 512 behind 7680 over 8 of 128: 89 us.  A step of two row tiles takes 4300 cycles at
 // head size 128 (3300 at 64), of which the tensor core is busy for 2048 (1024) and the exponentials for 2048: a row tile's own chain of
 // scores, maximum, exponentials (1700, at 16 a cycle 1024 alone) and product bounds it, with two softmax warps a scheduler to
 // interleave.  Slower: two threads a row (8192 tokens, head size 64: 525 us against 419), a cubic for some of the exponentials (446 to

@@ -18,9 +18,9 @@
 // are marked on the first way, and only where there are any of either the maxima are taken again, without those rows and from the exact
 // rotation.
 //
-// Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.5 us, 2048 tokens 9.8 us (20 MB, 2.1 TB/s; copies at
-// 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 76.6 us (285 MB, 3.7 TB/s,
-// 58 % of a copy), in bfloat16 63.7.  These wait for their loads (6 of 12 cycles between two instructions of a warp, issue slots 55 % busy) at the 32
+// Measured, back to back: 8 tokens of 32 + 2 * 4 heads of 64 in bfloat16 3.6 us, 2048 tokens 9.5 us (20 MB, 2.2 TB/s; copies at
+// 6.45 TB/s would take 3.2); 3842 tokens in float32 of 32 + 2 * 32 heads of 128 in 9 portions on pages of 16 76.3 us (285 MB, 3.7 TB/s,
+// 58 % of a copy), in bfloat16 63.0.  These wait for their loads (6 of 12 cycles between two instructions of a warp, issue slots 57 % busy) at the 32
 // warps an SM that 64 registers leave.  A run's numbers kept in registers between the two ways, and more loads in flight at more registers, were both slower.
 // Rounding the exact rotation costs 8 to 13 % of that: rounded from float32 arithmetic one number in a million was its neighbour.
 #include "q8.cuh"
@@ -423,7 +423,7 @@ extern "C" int kllm_rope_append_q8(void* q_out, int64_t qo_stride, const void* q
                       !(((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & (4 * es - 1)) &&
                       !((uintptr_t)cos_sin & 15) && !(((uintptr_t)kcache | (uintptr_t)vcache) & 3);
     // A CTA a token where every request brings one, else one for sixteen.  kv heads a CTA: as many as its threads cover, at most
-    // four, as long as there are runs enough for two CTAs an SM and the run stays in the first-level cache beside those of the SM's
+    // four, as long as there are runs enough for two CTAs on each of the 148 SMs and the run stays in the first-level cache beside those of the SM's
     // other CTAs until it is read again.  Microseconds for 3842 tokens in 9 portions with 1, 2, 4, 8 heads of 128 a CTA: float32, 32 kv
     // heads, pages of 16 (16 KB a head) 88, 73, 70, 79, pages of 64 76, 77, 81, 119; bfloat16 (four numbers at a time), 8 kv heads, pages of 16
     // 34, 29, 27, 31; 4 x 2048 tokens, pages of 64 69, 64, 68, 68.
