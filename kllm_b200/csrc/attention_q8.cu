@@ -80,8 +80,9 @@ template <int N> __device__ __forceinline__ __half pick(const __half (&p)[N], in
 //
 // Measured, back to back, bfloat16 (% of a copy's 6.45 TB/s): 64 requests of 846 to 4095 keys, 32 heads over 8 of 128, pages of 16: 69.9 us (72 %);
 // one of 131072 keys 54.2 us (77 %); 8 of 2048 keys, 32 over 4 of 64: 8.6 us; one: 6.2 us, a chain of launch, table, tiles and
-// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 17.8 us (37 %).  With loads straight into registers the first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size
-// 64 (16 of a CTA pair an SM as before): 64 x 2048 keys 18.7 us against 19.6, 128 x 1000 23.0 against 18.8.
+// joins.  Float32, 5 requests of 604 to 1501 keys, 32 heads of 128: 17.8 us (37 %).  With loads straight into registers the
+// first took 131 us: a warp then waits for each of its tiles.  Eight warps a CTA at head size 64 (16 of a CTA pair an SM as before): 64 x 2048
+// keys 18.7 us against 19.6, 128 x 1000 23.0 against 18.8.
 
 constexpr int DEC_KT = HD <= 128 ? 32 : 16;              // keys of a warp's tile
 constexpr int DEC_MT = DEC_KT / 16;
@@ -548,7 +549,7 @@ attn_decode_q8_kernel(const DecodeArgs a) {
                 } else {
                     // Beside float32 queries sixteen keys at a time are added to a sum in registers: what the tensor core cuts off one long
                     // sum added up, over 16001 keys, to three to five times float32 arithmetic's error.  It costs 2 to 8 %, with seven
-                    // or eight heads of 128 a CTA 11 to 19.
+                    // or eight heads of 128 a CTA 10 to 18.
                     float sum[2][NG][4];
 #pragma unroll
                     for (int k = NP - 1; k >= 0; k--)
